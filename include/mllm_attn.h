@@ -12,6 +12,7 @@
  *   mllm_*_paged_bf16           the same four over a paged KV cache (block tables)
  *   mllm_*_varlen_*             epilogue and prefill over packed sequences of different
  *                               lengths (several prompts in one launch each)
+ *   mllm_*_kv8                  epilogue, read-back and decode over an 8-bit paged KV cache
  *   mllm_sample                 Sampler::Sample on the device (penalty, greedy / top-k / top-p)
  *
  * plus the RoPE table builder and RoPE apply that back the `mllm::RoPE` facade.
@@ -363,6 +364,80 @@ MLLM_API int mllm_prefill_attention_varlen_paged_bf16(const void* q, const mllm_
                                                       int num_heads, int num_kv_heads, int head_dim, int total_q,
                                                       int max_q_len, float softmax_scale, void* out,
                                                       mllm_stream_t stream);
+
+/* ----------------------------------------------------------------------------------------
+ * 8-bit paged KV cache.  A K or V row of one token and kv head is head_dim e4m3 values and one
+ * exponent byte e + 127: the row stands for value * 2^e.  e is the smallest integer in [-100, 120]
+ * with max|row| <= 448 * 2^e (over the row's finite elements); values are rounded to nearest, ties
+ * to even; an infinity or NaN is stored as NaN.  Every stored row is exact in bf16.
+ *   k_pool / v_pool: bytes; element (block, head, row, d) at block*block_stride +
+ *       head*head_stride + row*row_stride + d, strides multiples of 16 bytes, 16-byte aligned.
+ *   k_exp / v_exp: bytes; row's exponent at block*exp_block_stride + head*exp_head_stride + row,
+ *       strides multiples of 16 bytes, 16-byte aligned.
+ *   block_size (a multiple of 128), num_blocks, block_table, table_stride, max_blocks_per_seq: as
+ *       mllm_paged_kv.  Rows past a sequence's length may hold any bytes.
+ *
+ * mllm_qkv_epilogue_varlen_paged_kv8: per-head RMSNorm of q and k (both weights or neither), RoPE,
+ *   and the append of k and v, all in fp32 with one rounding at the end (bf16 for q, e4m3 for k
+ *   and v; mllm_qkv_epilogue_varlen_paged_bf16 rounds to bf16 after the norm as the reference
+ *   does).  Arguments as that call's, but:
+ *   rope_cos / rope_sin: fp32 [total_tokens, head_dim], one row per token, or both NULL: the angles
+ *       are computed from positions (int64 [total_tokens]) and rope_theta.
+ *   q_out: token t's head h at q_out + t*q_out_st + h*q_out_sh (multiples of 4 elements), so
+ *       that it can be written as [heads, tokens, d] for prefill or [tokens, heads, d] for decode.
+ *   cache_start: int32 device [batch], required.
+ *   A token outside the ranges cu_seqlens describes is left out: none of its rows is written.  A
+ *   cache row past the block table, or a table entry outside the pool, records
+ *   MLLM_ERR_DEVICE_LENGTH and is not written (its q row is).
+ *
+ * mllm_kv8_read_bf16: cache rows first_rows[b] .. kv_lens[b] - 1 (first_rows NULL: from row 0) of
+ *   every sequence as bf16, exactly: row first_rows[b] + r at out + b*out_sb + h*out_sh + r*out_st
+ *   (multiples of 8 elements, 16-byte aligned), for r < rows; rows at or past kv_lens[b] are zero.
+ *
+ * mllm_decode_attention_paged_kv8: one query row per sequence (q bf16 [batch, num_heads, head_dim])
+ *   over its cache rows 0 .. kv_lens[b] - 1 (int32 device, required, 0 <= kv_lens[b] <=
+ *   max_kv_len; an empty sequence gives zeros) -> out bf16 [batch, num_heads * head_dim].
+ *   head_dim 64 or 128, at most 8 query heads per kv head.  workspace:
+ *   mllm_decode_attention_kv8_workspace_size() bytes, 256-byte aligned; its contents need not be
+ *   initialised and nothing is kept in it between calls, but two calls that may run at the same
+ *   time need two workspaces. */
+typedef struct mllm_paged_kv8 {
+    void* k_pool;
+    void* v_pool;
+    int64_t block_stride;
+    int64_t head_stride;
+    int64_t row_stride;
+    void* k_exp;
+    void* v_exp;
+    int64_t exp_block_stride;
+    int64_t exp_head_stride;
+    int32_t num_blocks;
+    int32_t block_size;
+    const int32_t* block_table;
+    int64_t table_stride;
+    int32_t max_blocks_per_seq;
+} mllm_paged_kv8;
+
+MLLM_API int mllm_qkv_epilogue_varlen_paged_kv8(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st,
+                                                int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh,
+                                                int total_tokens, int num_heads, int num_kv_heads, int head_dim,
+                                                const int64_t* positions, double rope_theta, const float* rope_cos,
+                                                const float* rope_sin, const void* q_norm_weight,
+                                                const void* k_norm_weight, double rms_norm_eps, void* q_out,
+                                                int64_t q_out_st, int64_t q_out_sh, const mllm_paged_kv8* kv,
+                                                const int32_t* cu_seqlens, int batch, const int32_t* cache_start,
+                                                mllm_stream_t stream);
+
+MLLM_API int mllm_kv8_read_bf16(const mllm_paged_kv8* kv, const int32_t* first_rows, const int32_t* kv_lens, int batch,
+                                int num_kv_heads, int head_dim, int rows, void* k_out, void* v_out, int64_t out_sb,
+                                int64_t out_sh, int64_t out_st, mllm_stream_t stream);
+
+MLLM_API size_t mllm_decode_attention_kv8_workspace_size(int num_heads, int num_kv_heads, int head_dim);
+
+MLLM_API int mllm_decode_attention_paged_kv8(const void* q, const mllm_paged_kv8* kv, const int32_t* kv_lens, int batch,
+                                             int num_heads, int num_kv_heads, int head_dim, int max_kv_len,
+                                             float softmax_scale, void* out, void* workspace, size_t workspace_bytes,
+                                             mllm_stream_t stream);
 
 /* ----------------------------------------------------------------------------------------
  * Token sampling on the device.  Replaces src/core/runtime/Sampler.cpp:49-232

@@ -43,6 +43,18 @@ class PagedKV(C.Structure):
 
 _kv = C.POINTER(PagedKV)
 
+
+class PagedKV8(C.Structure):
+    """struct mllm_paged_kv8 (include/mllm_attn.h): an 8-bit paged KV cache's pools, exponents and block table."""
+    _fields_ = [("k_pool", C.c_void_p), ("v_pool", C.c_void_p), ("block_stride", C.c_int64),
+                ("head_stride", C.c_int64), ("row_stride", C.c_int64), ("k_exp", C.c_void_p), ("v_exp", C.c_void_p),
+                ("exp_block_stride", C.c_int64), ("exp_head_stride", C.c_int64), ("num_blocks", C.c_int32),
+                ("block_size", C.c_int32), ("block_table", C.c_void_p), ("table_stride", C.c_int64),
+                ("max_blocks_per_seq", C.c_int32)]
+
+
+_kv8 = C.POINTER(PagedKV8)
+
 # name -> (restype, argtypes); mirrors include/mllm_attn.h one to one
 SIGNATURES = {
     "mllm_attn_abi_version": (_i, []),
@@ -79,6 +91,11 @@ SIGNATURES = {
     "mllm_prefill_attention_varlen_bf16": (_i, [_p, _p, _p, _i64, _i64, _i64, _i64, _p, _p, _i, _i, _i, _i, _i,
                                                 _i, _f, _p, _p]),
     "mllm_prefill_attention_varlen_paged_bf16": (_i, [_p, _kv, _p, _p, _i, _i, _i, _i, _i, _i, _f, _p, _p]),
+    "mllm_qkv_epilogue_varlen_paged_kv8": (_i, [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _i, _i, _i, _i, _p, _d,
+                                                _p, _p, _p, _p, _d, _p, _i64, _i64, _kv8, _p, _i, _p, _p]),
+    "mllm_kv8_read_bf16": (_i, [_kv8, _p, _p, _i, _i, _i, _i, _p, _p, _i64, _i64, _i64, _p]),
+    "mllm_decode_attention_kv8_workspace_size": (_sz, [_i, _i, _i]),
+    "mllm_decode_attention_paged_kv8": (_i, [_p, _kv8, _p, _i, _i, _i, _i, _i, _f, _p, _p, _sz, _p]),
     "mllm_linear_workspace_size": (_sz, [_i, _i, C.POINTER(C.c_int64), _i64]),
     "mllm_linear_bf16": (_i, [_p, _i64, _i, _i64, _i, C.POINTER(C.c_void_p), C.POINTER(C.c_int64),
                               C.POINTER(C.c_int64), _p, _i64, _p, _sz, _p]),

@@ -99,6 +99,31 @@ int encode_kv_map(CUtensorMap* map, const void* base, int64_t d, int64_t rows, i
     return MLLM_OK;
 }
 
+int encode_kv8_map(CUtensorMap* map, const void* base, int64_t d, int64_t rows, int64_t heads, int64_t blocks,
+                   int64_t stride_row, int64_t stride_head, int64_t stride_block, uint32_t box_rows) {
+    auto fn = get_encode_fn();
+    if (!fn) return fail(MLLM_ERR_CUDA, "cuTensorMapEncodeTiled entry point unavailable");
+    if (!aligned(base, 16)) return fail(MLLM_ERR_INVALID_ARGUMENT, "TMA base address must be 16-byte aligned");
+    for (int64_t st : {stride_row, stride_head, stride_block}) {
+        if (st % 16 != 0 || st <= 0)
+            return fail(MLLM_ERR_INVALID_ARGUMENT, "8-bit cache strides must be positive multiples of 16 bytes");
+    }
+    cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)rows, (cuuint64_t)heads, (cuuint64_t)blocks};
+    cuuint64_t strides[3] = {(cuuint64_t)stride_row, (cuuint64_t)stride_head, (cuuint64_t)stride_block};
+    cuuint32_t box[4] = {(cuuint32_t)d, box_rows, 1, 1};
+    cuuint32_t elem_strides[4] = {1, 1, 1, 1};
+    CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(base), dims, strides, box, elem_strides,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, d == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        char buf[160];
+        snprintf(buf, sizeof(buf), "cuTensorMapEncodeTiled (8-bit cache) failed (%d) dims=%lld,%lld,%lld,%lld", (int)r,
+                 (long long)d, (long long)rows, (long long)heads, (long long)blocks);
+        return fail(MLLM_ERR_INVALID_ARGUMENT, buf);
+    }
+    return MLLM_OK;
+}
+
 int encode_u8_map(CUtensorMap* map, const void* base, int64_t cols, int64_t rows, int64_t stride_row,
                   uint32_t box_cols, uint32_t box_rows, bool swizzle128) {
     auto fn = get_encode_fn();
@@ -149,11 +174,12 @@ extern "C" const char* mllm_attn_last_error(void) { return t_last_error.c_str();
 
 extern "C" int mllm_attn_device_status(mllm_stream_t stream) {
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    constexpr int kReaders = 5;
-    unsigned v[kReaders] = {0u, 0u, 0u, 0u, 0u};
+    constexpr int kReaders = 7;
+    unsigned v[kReaders] = {};
     int (*readers[kReaders])(cudaStream_t, unsigned*) = {read_clear_status_decode, read_clear_status_prefill,
                                                          read_clear_status_epilogue, read_clear_status_peer,
-                                                         read_clear_status_linear};
+                                                         read_clear_status_linear, read_clear_status_kv8_rows,
+                                                         read_clear_status_decode_stream};
     for (int i = 0; i < kReaders; ++i) {
         const int e = readers[i](s, &v[i]);
         if (e != 0) return check_cuda((cudaError_t)e, "read device status");

@@ -1,0 +1,745 @@
+// Decode attention with an even split of the cached rows over the GPU (one query per sequence), for
+//   the 8-bit paged cache (kv8.cuh), and
+//   the rows of a bf16 paged cache behind a prefix that the batch shares (shared_prefix.cu does the prefix).
+//
+// Work split.  The tiles of all (sequence, kv head) pairs, pair after pair, form one line of tiles; CTA i of G
+// takes tiles i*per .. (i+1)*per - 1 of it, per = ceil(tiles / G).  Every CTA streams the same number of bytes
+// whatever the lengths are, the plan is computed on the device from the lengths (a captured graph follows them),
+// and there is no counter to keep between calls.  A CTA's range cuts at most its first and its last pair, so the
+// partial results need two slots a CTA, whatever the lengths; a pair that lies in one CTA is written directly.
+// stream_combine_kernel joins the cut pairs in CTA order (deterministic).
+//
+// Per tile (8-bit: 128 rows, bf16: 64; both 32 KB of K and V at D = 128) with the cached rows as the M side:
+//   S^T = K Q^T      mma.sync m16n8k16, A = 16 cached rows (ldmatrix), B = the group's <= 8 query heads: no half of
+//                    the MMA is padding, as it is with the heads on the M side
+//   softmax          online in the exp2 domain; a thread holds two heads, the reduction runs over its 8 row lanes
+//   O^T += V^T P^T   A = V^T by ldmatrix.trans, B = P^T: the C fragment of S^T turned by movmatrix
+// An 8-bit row becomes halves in registers (one cvt per two values, exact).  ldmatrix moves 16-bit units, so a
+// thread gets four neighbouring columns of K instead of two pairs eight apart; Q's fragments are loaded in the same
+// permuted order, which leaves the contraction unchanged.  For V^T the transposed units hold two columns of two
+// rows; one byte permute sorts them, and output columns 2i and 2i + 1 land in the two row halves of the MMA.
+// q is scaled per head by a power of two into the range of a half (exact for elements within 2^-27 of the head's
+// largest; smaller ones lose bits that lie 2^-40 below it) and the scale is taken out of S in fp32.
+// Row scales: S gets 2^ek before the softmax.  2^ev multiplies P, so P^T = exp2(s + ev - mo) with mo the running
+// maximum of s + ev: the largest weight times scale is 1 and none overflows a half, however the rows' scales
+// differ; the sum l uses exp2(s - m) with its own maximum in fp32.  P is rounded to a half (2^-11), to bf16 for a
+// bf16 cache, since A and B of an MMA have one type; both sums stay fp32.
+//
+// Bound: HBM (2 (D + 1) bytes a row and kv head; 4 D for bf16).  Rows past the end of a sequence are masked to
+// -inf in S and zeroed in V (any bits may lie there); TMA boxes wholly past the end are not loaded.
+#include <algorithm>
+#include <cmath>
+
+#include "decode_stream.cuh"
+#include "kv8.cuh"
+
+namespace mllm_b200 {
+namespace {
+
+constexpr int kBoxRows = 64;
+constexpr int kConsumerWarps = 4;
+constexpr int kThreads = (kConsumerWarps + 1) * 32;
+constexpr int kPad = 8;            // floats between the merge rows of two heads (bank spread)
+
+template <int D, bool k8>
+struct Cfg {
+    static constexpr int kTile = k8 ? 128 : 64;                 // rows per stage
+    static constexpr int kWarpRows = kTile / kConsumerWarps;    // 32 or 16
+    static constexpr int kRowBytes = k8 ? D : 2 * D;
+    static constexpr int kBoxBytesRow = kRowBytes < 128 ? kRowBytes : 128;
+    static constexpr int kColBoxes = kRowBytes / kBoxBytesRow;
+    static constexpr int kRowBoxes = kTile / kBoxRows;
+    static constexpr int kBoxBytes = kBoxRows * kBoxBytesRow;
+    static constexpr int kTileBytes = kTile * kRowBytes;        // K or V
+    static constexpr int kStageBytes = 2 * kTileBytes;
+    static constexpr int kStages = kStageBytes >= 32768 ? 3 : 6;
+    static constexpr int kExpBytes = k8 ? 2 * kTile : 0;        // K and V exponents of a stage
+    static constexpr int kRedFloats = (kConsumerWarps - 1) * kMaxGroup * (D + kPad);
+    static constexpr int kSmemBytes = kStages * (kStageBytes + kExpBytes) + kRedFloats * 4 +
+                                      3 * kConsumerWarps * kMaxGroup * 4 + 2 * kStages * 8 + 1024;
+    static_assert(2 * (kSmemBytes + 1024) <= 233472, "two CTAs per SM no longer fit");
+};
+
+// 16-byte chunk c of row r of a box: the swizzle TMA applied (128-byte rows, or 64-byte rows).
+template <int ROWB>
+__device__ __forceinline__ uint32_t swz_chunk(uint32_t r, uint32_t c) {
+    return ROWB == 128 ? r * 128u + ((c ^ (r & 7u)) << 4) : r * 64u + ((c ^ ((r >> 1) & 3u)) << 4);
+}
+
+__device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                              uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Transposes an 8 x 8 matrix of 16-bit values held one row per four lanes.
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Bulk copy of a few contiguous bytes (16-byte aligned, a multiple of 16) into shared memory.
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_u32(bar))
+        : "memory");
+}
+
+// A pair's stretch of this CTA's tiles.
+struct Walk {
+    int b, g;
+    int left;              // tiles of the CTA still to come, this stretch included
+    int pos;               // first tile of this stretch on the line of tiles
+    int t0, t1;            // tiles of the pair: this stretch
+    SeqTiles s;            // the pair's rows and tiles
+    __device__ __forceinline__ bool whole() const { return t0 == 0 && t1 == s.tiles; }
+};
+
+template <int TILE>
+__device__ __forceinline__ void walk_open(const StreamArgs& a, Walk& w) {
+    w.t1 = min(w.s.tiles, w.t0 + w.left);
+}
+
+// Moves to the next pair with tiles; false when the CTA's tiles are done.
+template <int TILE>
+__device__ __forceinline__ bool walk_next(const StreamArgs& a, Walk& w) {
+    w.left -= w.t1 - w.t0;
+    w.pos += w.t1 - w.t0;
+    if (w.left <= 0) return false;
+    if (++w.g == a.Hkv) {
+        w.g = 0;
+        do {
+            if (++w.b >= a.B) return false;
+            w.s = seq_tiles<TILE>(a, w.b);
+        } while (w.s.tiles == 0);
+    }
+    w.t0 = 0;
+    walk_open<TILE>(a, w);
+    return true;
+}
+
+template <int D, bool k8>
+__global__ void __launch_bounds__(kThreads, 2)
+    stream_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                         StreamArgs a, Kv8View kv) {
+    using C = Cfg<D, k8>;
+    constexpr int NS = C::kStages;
+    constexpr int TILE = C::kTile;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* s_exp = smem + NS * C::kStageBytes;                       // [NS][K exps | V exps]
+    float* red_o = reinterpret_cast<float*>(s_exp + NS * C::kExpBytes);
+    float* red_m = red_o + C::kRedFloats;                              // [4][8]
+    float* red_l = red_m + kConsumerWarps * kMaxGroup;
+    float* red_mo = red_l + kConsumerWarps * kMaxGroup;
+    uint64_t* full = reinterpret_cast<uint64_t*>(red_mo + kConsumerWarps * kMaxGroup);
+    uint64_t* empty = full + NS;
+    __shared__ int s_plan[5];   // tiles of this CTA, its first tile, that tile's sequence and place in it, tiles per pair
+
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < NS; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], kConsumerWarps);
+        }
+        mbar_fence_init();
+    }
+    // Behind a prefix kernel (after_prefix) nothing here depends on that kernel, which has itself waited for
+    // everything before it and then let this grid start: the wait moves to the end of the kernel.
+    if (!a.after_prefix) pdl_wait();
+    pdl_trigger();
+    if (warp == 0) {
+        const int total = total_tiles<TILE>(a, lane);
+        const int per = tiles_per_cta(total, gridDim.x, a.min_tiles);
+        const int p0 = min(total, (int)blockIdx.x * per);
+        const int n = min(per, total - p0);
+        int before = 0;   // tiles of the sequences before this batch of 32
+        if (n > 0) {
+            for (int base = 0; base < a.B; base += 32) {
+                const int mine = base + lane < a.B ? seq_tiles<TILE>(a, base + lane).tiles * a.Hkv : 0;
+                int incl = mine;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int up = __shfl_up_sync(0xffffffffu, incl, o);
+                    if (lane >= o) incl += up;
+                }
+                const unsigned past = __ballot_sync(0xffffffffu, before + incl > p0);
+                if (past != 0) {
+                    if (lane == __ffs(past) - 1) {
+                        const int off = p0 - (before + incl - mine);
+                        const int tiles = mine / a.Hkv;
+                        s_plan[2] = base + lane;
+                        s_plan[3] = off;          // tile within the sequence's kv heads
+                        s_plan[4] = tiles;
+                    }
+                    break;
+                }
+                before += __shfl_sync(0xffffffffu, incl, 31);
+            }
+        }
+        if (lane == 0) {
+            s_plan[0] = n;
+            s_plan[1] = p0;
+        }
+    }
+    __syncthreads();
+    Walk w;
+    w.left = s_plan[0];
+    w.pos = s_plan[1];
+    if (w.left > 0) {
+        w.b = s_plan[2];
+        w.g = s_plan[3] / s_plan[4];
+        w.t0 = s_plan[3] - w.g * s_plan[4];
+        w.s = seq_tiles<TILE>(a, w.b);
+        walk_open<TILE>(a, w);
+    }
+
+    if (warp == kConsumerWarps) {
+        // ------------------------------ producer ------------------------------
+        if (lane == 0 && w.left > 0) {
+            tma_prefetch_desc(&tmK);
+            tma_prefetch_desc(&tmV);
+            int stage = 0;
+            uint32_t phase = 0;
+            bool alive = true;
+            do {
+                for (int t = w.t0; t < w.t1 && alive; ++t) {
+                    const int row0 = (w.s.first_tile + t) * TILE;
+                    const int boxes = C::kRowBoxes == 1 ? 1 : min(C::kRowBoxes, (w.s.len - row0 + kBoxRows - 1) / kBoxRows);
+                    int blk, row;
+                    kv_locate(a.lay, w.b, row0, blk, row);   // a bad table entry reads block 0 (and is recorded)
+                    if (!mbar_wait(&empty[stage], phase ^ 1)) { alive = false; break; }
+                    uint8_t* kdst = smem + stage * C::kStageBytes;
+                    uint8_t* vdst = kdst + C::kTileBytes;
+                    mbar_arrive_expect_tx(&full[stage],
+                                          (uint32_t)boxes * 2u * (C::kColBoxes * C::kBoxBytes + (k8 ? kBoxRows : 0)));
+                    for (int rb = 0; rb < boxes; ++rb) {
+#pragma unroll
+                        for (int cb = 0; cb < C::kColBoxes; ++cb) {
+                            const int off = (rb * C::kColBoxes + cb) * C::kBoxBytes;
+                            const int col = cb * (k8 ? 128 : 64);
+                            tma_load_4d(kdst + off, &tmK, &full[stage], col, row + rb * kBoxRows, w.g, blk);
+                            tma_load_4d(vdst + off, &tmV, &full[stage], col, row + rb * kBoxRows, w.g, blk);
+                        }
+                    }
+                    if constexpr (k8) {
+                        uint8_t* edst = s_exp + stage * C::kExpBytes;
+                        const int64_t eoff = blk * kv.e_sb + w.g * kv.e_sh + row;
+                        bulk_load(edst, kv.k_exp + eoff, boxes * kBoxRows, &full[stage]);
+                        bulk_load(edst + TILE, kv.v_exp + eoff, boxes * kBoxRows, &full[stage]);
+                    }
+                    if (++stage == NS) { stage = 0; phase ^= 1; }
+                }
+            } while (alive && walk_next<TILE>(a, w));
+        }
+    } else if (w.left > 0) {
+        // -------------------------------- consumers --------------------------------
+        const int grp = lane >> 2;   // row lane (and head of the Q fragment)
+        const int tig = lane & 3;    // heads 2 tig, 2 tig + 1
+        constexpr int CH = C::kRowBytes / 16;            // 16-byte chunks of a row
+        constexpr int KS = D / 16;                       // k-steps of S^T, and m-blocks of O^T
+        constexpr int NB = C::kWarpRows / 16;            // 16-row blocks of this warp
+        const int mi = lane >> 3, ri = lane & 7;
+        int stage = 0;
+        uint32_t phase = 0;
+        bool alive = true;
+        do {
+            // Q as the B operand: column n = head grp; two values per register along head_dim
+            uint32_t qb[KS][2];
+            float sc0, sc1;          // log2-domain scales of heads 2 tig and 2 tig + 1
+            {
+                const bool ok = grp < a.n_rep;
+                const __nv_bfloat16* qrow = a.q + ((int64_t)w.b * a.H + (int64_t)w.g * a.n_rep + (ok ? grp : 0)) * D;
+                if constexpr (k8) {
+                    float x[KS][4];
+                    float amax = 0.f;
+#pragma unroll
+                    for (int ks = 0; ks < KS; ++ks) {
+                        const uint2 raw = *reinterpret_cast<const uint2*>(qrow + ks * 16 + tig * 4);
+                        const float2 lo = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.x));
+                        const float2 hi = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.y));
+                        x[ks][0] = ok ? lo.x : 0.f;
+                        x[ks][1] = ok ? lo.y : 0.f;
+                        x[ks][2] = ok ? hi.x : 0.f;
+                        x[ks][3] = ok ? hi.y : 0.f;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) amax = fmaxf(amax, fabsf(x[ks][e]));
+                    }
+                    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+                    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+                    const int eq = max((int)(__float_as_uint(amax) >> 23) - 127 - 13, kExpMin);
+                    const float inv = pow2i(-eq);
+#pragma unroll
+                    for (int ks = 0; ks < KS; ++ks) {
+                        qb[ks][0] = pack_f16x2(x[ks][0] * inv, x[ks][1] * inv);
+                        qb[ks][1] = pack_f16x2(x[ks][2] * inv, x[ks][3] * inv);
+                    }
+                    const float qs = pow2i(eq) * a.scale_log2;
+                    sc0 = __shfl_sync(0xffffffffu, qs, 8 * tig);
+                    sc1 = __shfl_sync(0xffffffffu, qs, 8 * tig + 4);
+                } else {
+#pragma unroll
+                    for (int ks = 0; ks < KS; ++ks) {
+                        const uint32_t lo = *reinterpret_cast<const uint32_t*>(qrow + ks * 16 + tig * 2);
+                        const uint32_t hi = *reinterpret_cast<const uint32_t*>(qrow + ks * 16 + tig * 2 + 8);
+                        qb[ks][0] = ok ? lo : 0u;
+                        qb[ks][1] = ok ? hi : 0u;
+                    }
+                    sc0 = sc1 = a.scale_log2;
+                }
+            }
+            float o[KS][4];
+#pragma unroll
+            for (int i = 0; i < KS; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+            float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, mo[2] = {-INFINITY, -INFINITY};
+
+            for (int t = w.t0; t < w.t1; ++t) {
+                if (!mbar_wait(&full[stage], phase)) { alive = false; break; }
+                uint8_t* kst = smem + stage * C::kStageBytes;
+                uint8_t* vst = kst + C::kTileBytes;
+                const uint32_t kbase = smem_u32(kst), vbase = smem_u32(vst);
+                const int row0 = warp * C::kWarpRows;                 // this warp's rows within the tile
+                const int tile_row = (w.s.first_tile + t) * TILE;     // cache row of the tile's row 0
+                const int valid = w.s.len - tile_row;                 // rows of the tile before the end
+                const int lo_row = a.first_row - tile_row;            // rows before this one belong to the prefix
+                auto chunk_addr = [&](uint32_t base, int row, int c) -> uint32_t {
+                    constexpr int CPB = C::kBoxBytesRow / 16;
+                    const int box = (row >> 6) * C::kColBoxes + c / CPB;
+                    return base + box * C::kBoxBytes + swz_chunk<C::kBoxBytesRow>(row & 63, c % CPB);
+                };
+
+                // ---- S^T = K Q^T ----
+                float sa[NB][4];
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+                    sa[nb][0] = sa[nb][1] = sa[nb][2] = sa[nb][3] = 0.f;
+                    const int row = row0 + nb * 16 + 8 * (mi & 1) + ri;
+#pragma unroll
+                    for (int c = 0; c < CH; c += 2) {
+                        uint32_t r0, r1, r2, r3;
+                        ldsm_x4(chunk_addr(kbase, row, c + (mi >> 1)), r0, r1, r2, r3);
+                        if constexpr (k8) {
+                            mma_f16_16816(sa[nb], e4m3x2_to_f16x2((uint16_t)r0), e4m3x2_to_f16x2((uint16_t)r1),
+                                          e4m3x2_to_f16x2((uint16_t)(r0 >> 16)), e4m3x2_to_f16x2((uint16_t)(r1 >> 16)),
+                                          qb[c][0], qb[c][1]);
+                            mma_f16_16816(sa[nb], e4m3x2_to_f16x2((uint16_t)r2), e4m3x2_to_f16x2((uint16_t)r3),
+                                          e4m3x2_to_f16x2((uint16_t)(r2 >> 16)), e4m3x2_to_f16x2((uint16_t)(r3 >> 16)),
+                                          qb[c + 1][0], qb[c + 1][1]);
+                        } else {
+                            mma_bf16_16816(sa[nb], r0, r1, r2, r3, qb[c / 2][0], qb[c / 2][1]);
+                        }
+                    }
+                }
+
+                // ---- online softmax: element (nb, h, e) is row row0 + 16 nb + 8 h + grp, head 2 tig + e ----
+                float ev[NB][2];
+                float mt[2] = {-INFINITY, -INFINITY}, mot[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int r = row0 + nb * 16 + 8 * h + grp;
+                        const bool in = r < valid && r >= lo_row;
+                        float ks = 1.f;
+                        ev[nb][h] = 0.f;
+                        if constexpr (k8) {
+                            const uint8_t* ex = s_exp + stage * C::kExpBytes;
+                            ks = exp_byte_scale(ex[r]);
+                            ev[nb][h] = (float)((int)ex[TILE + r] - 127);
+                        }
+                        const float v0 = in ? sa[nb][2 * h] * sc0 * ks : -INFINITY;
+                        const float v1 = in ? sa[nb][2 * h + 1] * sc1 * ks : -INFINITY;
+                        sa[nb][2 * h] = v0;
+                        sa[nb][2 * h + 1] = v1;
+                        mt[0] = fmaxf(mt[0], v0);
+                        mt[1] = fmaxf(mt[1], v1);
+                        if constexpr (k8) {
+                            mot[0] = fmaxf(mot[0], v0 + ev[nb][h]);
+                            mot[1] = fmaxf(mot[1], v1 + ev[nb][h]);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int off = 4; off < 32; off <<= 1) {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        mt[e] = fmaxf(mt[e], __shfl_xor_sync(0xffffffffu, mt[e], off));
+                        if constexpr (k8) mot[e] = fmaxf(mot[e], __shfl_xor_sync(0xffffffffu, mot[e], off));
+                    }
+                }
+                float mu[2], mou[2], oscale[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float mn = fmaxf(m[e], mt[e]);
+                    mu[e] = mn == -INFINITY ? 0.f : mn;
+                    l[e] *= ex2_approx(m[e] - mu[e]);
+                    if constexpr (k8) {
+                        const float mon = fmaxf(mo[e], mot[e]);
+                        mou[e] = mon == -INFINITY ? 0.f : mon;
+                        oscale[e] = ex2_approx(mo[e] - mou[e]);
+                        mo[e] = mon;
+                    } else {
+                        mou[e] = mu[e];
+                        oscale[e] = ex2_approx(m[e] - mu[e]);
+                    }
+                    m[e] = mn;
+                }
+                uint32_t pb[NB][2];
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float p0 = ex2_approx(sa[nb][2 * h] - mu[0]);
+                        const float p1 = ex2_approx(sa[nb][2 * h + 1] - mu[1]);
+                        l[0] += p0;
+                        l[1] += p1;
+                        uint32_t packed;
+                        if constexpr (k8) {
+                            packed = pack_f16x2(ex2_approx(sa[nb][2 * h] + ev[nb][h] - mou[0]),
+                                                ex2_approx(sa[nb][2 * h + 1] + ev[nb][h] - mou[1]));
+                        } else {
+                            packed = pack_bf16x2(p0, p1);
+                        }
+                        pb[nb][h] = movmatrix_trans(packed);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < KS; ++i) {
+                    o[i][0] *= oscale[0];
+                    o[i][1] *= oscale[1];
+                    o[i][2] *= oscale[0];
+                    o[i][3] *= oscale[1];
+                }
+
+                // ---- rows past the end: zero this warp's V rows (any bit pattern may lie there) ----
+                if (valid < row0 + C::kWarpRows) {
+                    for (int i = lane; i < C::kWarpRows * CH; i += 32) {
+                        const int r = row0 + i / CH, c = i % CH;
+                        if (r >= valid)
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(chunk_addr(vbase, r, c)), "r"(0)
+                                         : "memory");
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                }
+
+                // ---- O^T += V^T P^T ----
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+                    const int row = row0 + nb * 16 + 8 * (mi & 1) + ri;
+#pragma unroll
+                    for (int c = 0; c < CH; c += 2) {
+                        uint32_t r0, r1, r2, r3;
+                        ldsm_x4_trans(chunk_addr(vbase, row, c + (mi >> 1)), r0, r1, r2, r3);
+                        if constexpr (k8) {
+                            r0 = __byte_perm(r0, 0u, 0x3120);
+                            r1 = __byte_perm(r1, 0u, 0x3120);
+                            r2 = __byte_perm(r2, 0u, 0x3120);
+                            r3 = __byte_perm(r3, 0u, 0x3120);
+                            mma_f16_16816(o[c], e4m3x2_to_f16x2((uint16_t)r0), e4m3x2_to_f16x2((uint16_t)(r0 >> 16)),
+                                          e4m3x2_to_f16x2((uint16_t)r1), e4m3x2_to_f16x2((uint16_t)(r1 >> 16)),
+                                          pb[nb][0], pb[nb][1]);
+                            mma_f16_16816(o[c + 1], e4m3x2_to_f16x2((uint16_t)r2), e4m3x2_to_f16x2((uint16_t)(r2 >> 16)),
+                                          e4m3x2_to_f16x2((uint16_t)r3), e4m3x2_to_f16x2((uint16_t)(r3 >> 16)),
+                                          pb[nb][0], pb[nb][1]);
+                        } else {
+                            mma_bf16_16816(o[c / 2], r0, r2, r1, r3, pb[nb][0], pb[nb][1]);
+                        }
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&empty[stage]);
+                if (++stage == NS) { stage = 0; phase ^= 1; }
+            }
+            if (!alive) break;
+
+            // ---- merge the four warps ----
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1) {
+                l[0] += __shfl_xor_sync(0xffffffffu, l[0], off);
+                l[1] += __shfl_xor_sync(0xffffffffu, l[1], off);
+            }
+            if (grp == 0) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    red_m[warp * kMaxGroup + 2 * tig + e] = m[e];
+                    red_l[warp * kMaxGroup + 2 * tig + e] = l[e];
+                    red_mo[warp * kMaxGroup + 2 * tig + e] = k8 ? mo[e] : m[e];
+                }
+            }
+            // column of o[i][2h + .]: 8-bit rows 16 i + 2 grp + h, bf16 rows 16 i + 8 h + grp
+            auto o_col = [&](int i, int h) -> int { return k8 ? 16 * i + 2 * grp + h : 16 * i + 8 * h + grp; };
+            if (warp > 0) {
+                float* dst = red_o + (warp - 1) * kMaxGroup * (D + kPad);
+#pragma unroll
+                for (int i = 0; i < KS; ++i) {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        dst[(2 * tig + e) * (D + kPad) + o_col(i, 0)] = o[i][e];
+                        dst[(2 * tig + e) * (D + kPad) + o_col(i, 1)] = o[i][2 + e];
+                    }
+                }
+            }
+            asm volatile("bar.sync 1, %0;" ::"n"(kConsumerWarps * 32) : "memory");
+            if (warp == 0) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int h = 2 * tig + e;
+                    float M = red_m[h], MO = red_mo[h];
+#pragma unroll
+                    for (int v = 1; v < kConsumerWarps; ++v) {
+                        M = fmaxf(M, red_m[v * kMaxGroup + h]);
+                        MO = fmaxf(MO, red_mo[v * kMaxGroup + h]);
+                    }
+                    const float Mu = M == -INFINITY ? 0.f : M, MOu = MO == -INFINITY ? 0.f : MO;
+                    float L = 0.f, ow[kConsumerWarps];
+#pragma unroll
+                    for (int v = 0; v < kConsumerWarps; ++v) {
+                        L += red_l[v * kMaxGroup + h] * ex2_approx(red_m[v * kMaxGroup + h] - Mu);
+                        ow[v] = ex2_approx(red_mo[v * kMaxGroup + h] - MOu);
+                    }
+                    // the stretch's own attention row (normalised), and log2 of its weight
+                    const float f = L != 0.f ? ex2_approx(MOu - Mu) / L : 0.f;
+#pragma unroll
+                    for (int i = 0; i < KS; ++i) {
+#pragma unroll
+                        for (int hh = 0; hh < 2; ++hh) {
+                            float* at = red_o + h * (D + kPad) + o_col(i, hh);
+                            float x = o[i][2 * hh + e] * ow[0];
+#pragma unroll
+                            for (int v = 1; v < kConsumerWarps; ++v) x += at[(v - 1) * kMaxGroup * (D + kPad)] * ow[v];
+                            *at = x * f;
+                        }
+                    }
+                    if (grp == 0) red_l[h] = L != 0.f ? Mu + log2f(L) : -INFINITY;
+                }
+            }
+            asm volatile("bar.sync 1, %0;" ::"n"(kConsumerWarps * 32) : "memory");
+            // ---- write the stretch's rows: final, or a partial ----
+            if (w.whole() && !a.prefix_parts) {
+                __nv_bfloat16* orow = a.out + ((int64_t)w.b * a.H + (int64_t)w.g * a.n_rep) * D;
+                for (int i = threadIdx.x; i < a.n_rep * (D / 2); i += kConsumerWarps * 32) {
+                    const int h = i / (D / 2), d = 2 * (i % (D / 2));
+                    *reinterpret_cast<uint32_t*>(orow + h * D + d) =
+                        pack_bf16x2(red_o[h * (D + kPad) + d], red_o[h * (D + kPad) + d + 1]);
+                }
+            } else {
+                // a whole pair's row (joined with the prefix) has a slot of its own; a cut pair takes the
+                // CTA's first slot if the CTA begins in it, else the second
+                const int64_t slot = w.whole() ? 2 * (int64_t)gridDim.x + (int64_t)w.b * a.Hkv + w.g
+                                               : 2 * (int64_t)blockIdx.x + (w.pos == s_plan[1] ? 0 : 1);
+                float* po = a.part_o + slot * a.n_rep * D;
+                for (int i = threadIdx.x; i < a.n_rep * (D / 4); i += kConsumerWarps * 32) {
+                    const int h = i / (D / 4), d = 4 * (i % (D / 4));
+                    *reinterpret_cast<float4*>(po + h * D + d) =
+                        *reinterpret_cast<const float4*>(red_o + h * (D + kPad) + d);
+                }
+                if (threadIdx.x < a.n_rep) a.part_lse[slot * a.n_rep + threadIdx.x] = red_l[threadIdx.x];
+            }
+            asm volatile("bar.sync 1, %0;" ::"n"(kConsumerWarps * 32) : "memory");
+        } while (walk_next<TILE>(a, w));
+    }
+    if (a.after_prefix) pdl_wait();   // so that this grid ends after the prefix kernel's
+}
+
+// Joins the parts of every (sequence, query head): the stretches of the cut pairs and, with a shared prefix, the
+// prefix's parts.  A part is a normalised row and log2 of its weight: out = sum_i 2^(e_i - M) row_i / sum_i 2^(e_i - M).
+// One CTA a (query head, sequence), thread d column d, parts in a fixed order.
+template <int D, int TILE>
+__global__ void __launch_bounds__(D) stream_combine_kernel(StreamArgs a, int grid) {
+    __shared__ float s_red[D / 32];
+    __shared__ int s_tiles[2][D / 32];
+    pdl_wait();
+    const int h = blockIdx.x, b = blockIdx.y, g = h / a.n_rep, r = h - g * a.n_rep;
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    // tiles of all sequences, and of those before b
+    int all = 0, before = 0;
+    for (int i = t; i < a.B; i += D) {
+        const int n = seq_tiles<TILE>(a, i).tiles;
+        all += n;
+        if (i < b) before += n;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        all += __shfl_xor_sync(0xffffffffu, all, o);
+        before += __shfl_xor_sync(0xffffffffu, before, o);
+    }
+    if (lane == 0) {
+        s_tiles[0][warp] = all;
+        s_tiles[1][warp] = before;
+    }
+    __syncthreads();
+    all = before = 0;
+#pragma unroll
+    for (int w = 0; w < D / 32; ++w) {
+        all += s_tiles[0][w];
+        before += s_tiles[1][w];
+    }
+    const SeqTiles s = seq_tiles<TILE>(a, b);
+    __nv_bfloat16* orow = a.out + ((int64_t)b * a.H + h) * D;
+    const int n_pre = s.short_len ? 0 : a.prefix_parts;
+    if (s.tiles == 0 && n_pre == 0) {   // nothing to attend to
+        orow[t] = __float2bfloat16_rn(0.f);
+        return;
+    }
+    const int per = tiles_per_cta(all * a.Hkv, grid, a.min_tiles);
+    const int p0 = before * a.Hkv + g * s.tiles, p1 = p0 + s.tiles;
+    const int c0 = p0 / per, c1 = s.tiles ? (p1 - 1) / per : c0 - 1;
+    const int own = c1 - c0 + 1;
+    if (own == 1 && n_pre == 0) return;   // written directly
+    const int n = own + n_pre;
+    auto part = [&](int i) -> int64_t {   // index of part i's row in part_o and part_lse
+        if (i >= own) return a.prefix_base + (((int64_t)(i - own) * a.Hkv + g) * a.B + b) * a.n_rep + r;
+        const int c = c0 + i;
+        const int64_t slot = own == 1 ? 2 * (int64_t)grid + (int64_t)b * a.Hkv + g : 2 * (int64_t)c + (c * per >= p0 ? 0 : 1);
+        return slot * a.n_rep + r;
+    };
+    float mx = -INFINITY;
+    for (int i = t; i < n; i += D) mx = fmaxf(mx, a.part_lse[part(i)]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    if (lane == 0) s_red[warp] = mx;
+    __syncthreads();
+    float M = s_red[0];
+#pragma unroll
+    for (int w = 1; w < D / 32; ++w) M = fmaxf(M, s_red[w]);
+    if (M == -INFINITY) M = 0.f;
+    float acc = 0.f, sum = 0.f;
+    constexpr int U = 8;   // parts whose loads are in flight together
+    for (int i0 = 0; i0 < n; i0 += U) {
+        float v[U], e[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const bool in = i0 + u < n;
+            const int64_t p = in ? part(i0 + u) : 0;
+            v[u] = in ? a.part_o[p * D + t] : 0.f;
+            e[u] = in ? a.part_lse[p] : -INFINITY;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const float wgt = ex2_approx(e[u] - M);
+            acc += wgt * v[u];
+            sum += wgt;
+        }
+    }
+    orow[t] = __float2bfloat16_rn(sum > 0.f || sum != sum ? acc / sum : 0.f);
+}
+
+constexpr int kMaxGrid = 2 * 160;
+
+int stream_grid(int num_sms) { return std::min(2 * num_sms, kMaxGrid); }
+
+}  // namespace
+
+size_t stream_part_rows(int batch, int num_kv_heads, bool shared) {
+    return 2 * (size_t)kMaxGrid + (shared ? (size_t)batch * num_kv_heads : 0);
+}
+
+size_t stream_workspace_bytes(int n_rep, int D, size_t part_rows) {
+    return (part_rows * n_rep * (size_t)(D + 1) * 4 + 255) & ~size_t(255);
+}
+
+namespace {
+
+template <int D, bool k8>
+int launch_stream_d(StreamArgs& a, const Kv8View& kv, const CUtensorMap& tmK, const CUtensorMap& tmV, int num_sms,
+                    cudaStream_t s) {
+    using C = Cfg<D, k8>;
+    a.min_tiles = k8 ? 1 : 2;
+    // no more CTAs than tiles there can be
+    const int64_t most = (int64_t)a.B * a.Hkv * ((a.max_len + C::kTile - 1) / C::kTile);
+    if (most > 0x7fffffffLL - 65536) return fail(MLLM_ERR_UNSUPPORTED, "decode_attention: batch too large for one call");
+    const int grid = (int)std::min<int64_t>(stream_grid(num_sms), std::max<int64_t>(most, 1));
+    auto kern = stream_decode_kernel<D, k8>;
+    if (int st = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes),
+                            "stream_decode smem attribute"))
+        return st;
+    if (int st = check_cuda(launch_pdl(kern, dim3(grid), dim3(kThreads), C::kSmemBytes, s, tmK, tmV, a, kv),
+                            "stream_decode_kernel launch"))
+        return st;
+    return check_cuda(launch_pdl(stream_combine_kernel<D, C::kTile>, dim3(a.H, a.B), dim3(D), 0, s, a, grid),
+                      "stream_combine_kernel launch");
+}
+
+}  // namespace
+
+int launch_stream_bf16(StreamArgs& a, int head_dim, const CUtensorMap& tmK, const CUtensorMap& tmV, int num_sms,
+                       cudaStream_t s) {
+    return head_dim == 128 ? launch_stream_d<128, false>(a, Kv8View{}, tmK, tmV, num_sms, s)
+                           : launch_stream_d<64, false>(a, Kv8View{}, tmK, tmV, num_sms, s);
+}
+
+MLLM_DEFINE_STATUS_READER(decode_stream)
+
+}  // namespace mllm_b200
+
+using namespace mllm_b200;
+
+extern "C" size_t mllm_decode_attention_kv8_workspace_size(int num_heads, int num_kv_heads, int head_dim) {
+    if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads || head_dim <= 0) return 0;
+    return stream_workspace_bytes(num_heads / num_kv_heads, head_dim, stream_part_rows(0, num_kv_heads, false));
+}
+
+extern "C" int mllm_decode_attention_paged_kv8(const void* q, const mllm_paged_kv8* kv, const int32_t* kv_lens, int batch,
+                                               int num_heads, int num_kv_heads, int head_dim, int max_kv_len,
+                                               float softmax_scale, void* out, void* workspace, size_t workspace_bytes,
+                                               mllm_stream_t stream) {
+    MLLM_NVTX_RANGE("mllm_decode_attention_paged_kv8");
+    if (batch < 0 || num_heads <= 0 || num_kv_heads <= 0 || max_kv_len <= 0)
+        return fail(MLLM_ERR_INVALID_ARGUMENT, "decode_attention_kv8: bad sizes");
+    if (num_heads % num_kv_heads != 0)
+        return fail(MLLM_ERR_INVALID_ARGUMENT, "Attention: num_heads must be divisible by num_kv_heads.");
+    if (head_dim != 64 && head_dim != 128)
+        return fail(MLLM_ERR_UNSUPPORTED, "decode_attention_kv8: head_dim must be 64 or 128");
+    const int n_rep = num_heads / num_kv_heads;
+    if (n_rep > kMaxGroup) return fail(MLLM_ERR_UNSUPPORTED, "decode_attention_kv8: GQA group larger than 8");
+    if (batch > 65535) return fail(MLLM_ERR_UNSUPPORTED, "decode_attention_kv8: more than 65535 sequences");
+    if (!(softmax_scale > 0.f) || !std::isfinite(softmax_scale))
+        return fail(MLLM_ERR_INVALID_ARGUMENT, "decode_attention_kv8: softmax_scale must be positive");
+    StreamArgs a = {};
+    Kv8View view;
+    if (int st = paged_layout8(kv, max_kv_len, head_dim, "decode_attention_kv8", &a.lay, &view)) return st;
+    if (batch == 0) return ok();
+    if (!q || !out || !kv_lens) return fail(MLLM_ERR_INVALID_ARGUMENT, "decode_attention_kv8: null pointer");
+    if (!aligned(q, 8) || !aligned(out, 4))
+        return fail(MLLM_ERR_INVALID_ARGUMENT, "decode_attention_kv8: q/out misaligned");
+    if (!workspace || !aligned(workspace, 256) ||
+        workspace_bytes < mllm_decode_attention_kv8_workspace_size(num_heads, num_kv_heads, head_dim))
+        return fail(MLLM_ERR_WORKSPACE, "decode_attention_kv8: workspace missing, misaligned or smaller than "
+                                        "mllm_decode_attention_kv8_workspace_size()");
+    int num_sms = 0;
+    if (int st = require_sm100(&num_sms)) return st;
+    CUtensorMap tmK, tmV;
+    if (int st = encode_kv8_map(&tmK, kv->k_pool, head_dim, kv->block_size, num_kv_heads, kv->num_blocks, kv->row_stride,
+                                kv->head_stride, kv->block_stride, kBoxRows))
+        return st;
+    if (int st = encode_kv8_map(&tmV, kv->v_pool, head_dim, kv->block_size, num_kv_heads, kv->num_blocks, kv->row_stride,
+                                kv->head_stride, kv->block_stride, kBoxRows))
+        return st;
+    a.q = (const __nv_bfloat16*)q;
+    a.kv_lens = kv_lens;
+    a.out = (__nv_bfloat16*)out;
+    a.B = batch;
+    a.H = num_heads;
+    a.Hkv = num_kv_heads;
+    a.n_rep = n_rep;
+    a.max_len = max_kv_len;
+    a.scale_log2 = (float)((double)softmax_scale * 1.4426950408889634);
+    a.part_o = static_cast<float*>(workspace);
+    a.part_lse = a.part_o + stream_part_rows(0, num_kv_heads, false) * n_rep * head_dim;
+    if (int st = head_dim == 128 ? launch_stream_d<128, true>(a, view, tmK, tmV, num_sms, (cudaStream_t)stream)
+                                 : launch_stream_d<64, true>(a, view, tmK, tmV, num_sms, (cudaStream_t)stream))
+        return st;
+    return ok();
+}

@@ -1,0 +1,76 @@
+// The argument block and the plan of the even-split decode (decode_stream.cu), shared with the shared-prefix
+// decode (shared_prefix.cu).
+#pragma once
+
+#include "common.cuh"
+#include "host_util.h"
+#include "kv_layout.cuh"
+
+namespace mllm_b200 {
+
+constexpr int kMaxGroup = 8;       // query heads per kv head (the N side of the MMAs)
+
+struct StreamArgs {
+    const __nv_bfloat16* q;        // [B, H, D]
+    const int32_t* kv_lens;        // [B]
+    __nv_bfloat16* out;            // [B, H * D]
+    float* part_o;                 // parts: rows of D floats ...
+    float* part_lse;               // ... and log2 of their weights
+    int B, H, Hkv, n_rep, max_len;
+    int min_tiles;                 // tiles a CTA takes at least
+    float scale_log2;
+    KvLayout lay;
+    // shared prefix: rows before first_row are the prefix kernel's, which leaves prefix_parts parts a query row at
+    // row prefix_base of the parts: [part][kv head][sequence][head of the group]
+    int first_row;
+    int prefix_parts;
+    int64_t prefix_base;
+    int after_prefix;              // the grid was let in by the prefix kernel
+};
+
+// Rows [first_row, len) of a sequence in tiles of TILE cache rows.  A length outside [0, max_len] is recorded and
+// clamped; a sequence shorter than the prefix (an empty one too) has no rows here, and no prefix either.
+struct SeqTiles {
+    int len, first_tile, tiles;
+    bool short_len;
+};
+
+template <int TILE>
+__device__ __forceinline__ SeqTiles seq_tiles(const StreamArgs& a, int b) {
+    SeqTiles s;
+    int len = a.kv_lens[b];
+    if (len < 0 || len > a.max_len || (len > 0 && len < a.first_row)) {
+        record_error(kErrBadLength);
+        len = len < 0 ? 0 : min(len, a.max_len);
+    }
+    s.short_len = len < a.first_row;
+    s.len = len;
+    s.first_tile = a.first_row / TILE;
+    s.tiles = len > a.first_row ? (len + TILE - 1) / TILE - s.first_tile : 0;
+    return s;
+}
+
+// Tiles of all pairs (the lanes of a full warp, lane given); the host has checked that the most there can be
+// plus a grid fits 31 bits.
+template <int TILE>
+__device__ __forceinline__ int total_tiles(const StreamArgs& a, int lane) {
+    int n = 0;
+    for (int b = lane; b < a.B; b += 32) n += seq_tiles<TILE>(a, b).tiles;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+    return n * a.Hkv;
+}
+
+__device__ __forceinline__ int tiles_per_cta(int total, int grid, int min_tiles) {
+    return max((total + grid - 1) / grid, min_tiles);
+}
+
+// Rows of parts the even-split decode writes: two slots a CTA, and with a shared prefix one per pair.
+size_t stream_part_rows(int batch, int num_kv_heads, bool shared);
+size_t stream_workspace_bytes(int n_rep, int D, size_t part_rows);
+
+// Runs the split and the combine kernel over a bf16 paged cache.
+int launch_stream_bf16(StreamArgs& a, int head_dim, const CUtensorMap& tmK, const CUtensorMap& tmV, int num_sms,
+                       cudaStream_t s);
+
+}  // namespace mllm_b200

@@ -60,6 +60,8 @@ int read_clear_status_prefill(cudaStream_t s, unsigned* out);
 int read_clear_status_epilogue(cudaStream_t s, unsigned* out);
 int read_clear_status_peer(cudaStream_t s, unsigned* out);
 int read_clear_status_linear(cudaStream_t s, unsigned* out);
+int read_clear_status_kv8_rows(cudaStream_t s, unsigned* out);
+int read_clear_status_decode_stream(cudaStream_t s, unsigned* out);
 
 // Encodes a 4-D bf16 tensor map {d (inner), rows, heads, batch} with 128-byte swizzle and a
 // {box_d, box_rows, box_heads, 1} box.  Strides are in elements and need not be ordered (a
@@ -68,6 +70,11 @@ int read_clear_status_linear(cudaStream_t s, unsigned* out);
 int encode_kv_map(CUtensorMap* map, const void* base, int64_t d, int64_t rows, int64_t heads, int64_t batch,
                   int64_t stride_row, int64_t stride_head, int64_t stride_batch, uint32_t box_d,
                   uint32_t box_rows, uint32_t box_heads = 1);
+
+// Encodes a 4-D byte tensor map {d (inner), rows, heads, blocks} of an 8-bit cache pool with a {d, box_rows, 1, 1}
+// box: 128-byte swizzle for d = 128, 64-byte swizzle for d = 64.  Strides are in bytes.
+int encode_kv8_map(CUtensorMap* map, const void* base, int64_t d, int64_t rows, int64_t heads, int64_t blocks,
+                   int64_t stride_row, int64_t stride_head, int64_t stride_block, uint32_t box_rows);
 
 // Encodes a 2-D byte tensor map {cols (inner), rows} with row stride `stride_row` bytes and a
 // {box_cols, box_rows} box (as a 4-D map with unit outer dimensions, so that the 4-D load helper

@@ -13,6 +13,8 @@ tensors are required and anything else raises RuntimeError, like the reference's
   Attention.forward       src/core/runtime/Attention.h:29-86
   Attention.forward_projected  src/core/runtime/Attention.h:100-326 (+ optional fused QK-norm,
                           which the reference does in TransformerBlock.h:103-134)
+  PagedKVCache8           8-bit paged cache (no reference counterpart): the functions below take it
+                          wherever they take a PagedKVCache
   attention_block         the attention half of TransformerBlock::Forward (h -> attention out)
 """
 from __future__ import annotations
@@ -25,6 +27,7 @@ import torch
 from . import abi
 
 BF16 = torch.bfloat16
+FP8 = torch.float8_e4m3fn
 
 
 def _check_cuda_bf16(name: str, t: torch.Tensor) -> None:
@@ -194,12 +197,15 @@ class PagedKVCache:
         blocks = self._blocks[seq]
         if blocks:
             idx = torch.tensor(blocks, dtype=torch.long, device=self.k_pool.device)
-            self.k_pool.index_fill_(0, idx, 0)
-            self.v_pool.index_fill_(0, idx, 0)
+            self._zero_blocks(idx)
             self._free.extend(reversed(blocks))
         self._blocks[seq] = []
         self._host_lengths[seq] = 0
         self.lengths[seq] = 0
+
+    def _zero_blocks(self, idx: torch.Tensor) -> None:
+        self.k_pool.index_fill_(0, idx, 0)
+        self.v_pool.index_fill_(0, idx, 0)
 
     def move(self, src: int, dst: int) -> None:
         """Hand sequence `src`'s blocks and length to the empty row `dst` (its block-table row is
@@ -319,6 +325,61 @@ class PagedSlot(PagedKVCache):
         return self._parent.gather(self._row(seq), rows)
 
 
+class PagedKVCache8(PagedKVCache):
+    """PagedKVCache whose rows are held in 8 bits (the mllm_paged_kv8 layout): e4m3 values
+    [num_blocks, Hkv, block_size, D] and one exponent byte per row [num_blocks, Hkv, block_size],
+    a little over half the memory and the decode time of the bf16 cache.  A row stands for
+    value * 2^(exponent - 127); rows are quantised as they are appended."""
+
+    def __init__(self, num_blocks: int, num_kv_heads: int, head_dim: int, block_size: int = 256,
+                 max_seqs: int = 64, max_blocks_per_seq: int | None = None, device="cuda"):
+        # the base class with pools of no size: its block bookkeeping is the same
+        super().__init__(num_blocks, num_kv_heads, 0, block_size, max_seqs, max_blocks_per_seq, device)
+        shape = (num_blocks, num_kv_heads, block_size)
+        self.k_pool = torch.zeros((*shape, head_dim), dtype=torch.uint8, device=device).view(FP8)
+        self.v_pool = torch.zeros((*shape, head_dim), dtype=torch.uint8, device=device).view(FP8)
+        self.k_exp = torch.zeros(shape, dtype=torch.uint8, device=device)
+        self.v_exp = torch.zeros(shape, dtype=torch.uint8, device=device)
+        self.one_each = torch.arange(max_seqs + 1, dtype=torch.int32, device=device)   # cu_seqlens of a decode step
+
+    def _zero_blocks(self, idx: torch.Tensor) -> None:
+        for t in (self.k_pool.view(torch.uint8), self.v_pool.view(torch.uint8), self.k_exp, self.v_exp):
+            t.index_fill_(0, idx, 0)
+
+    def slot(self, seq: int, count: int = 1) -> "PagedSlot8":
+        return PagedSlot8(self, seq, count)
+
+    def descriptor(self) -> abi.PagedKV8:
+        s, e = self.k_pool.stride(), self.k_exp.stride()
+        if self.v_pool.stride() != s or self.v_exp.stride() != e:
+            raise RuntimeError("PagedKVCache8: K and V pools must have the same layout")
+        return abi.PagedKV8(self.k_pool.data_ptr(), self.v_pool.data_ptr(), s[0], s[1], s[2], self.k_exp.data_ptr(),
+                            self.v_exp.data_ptr(), e[0], e[1], self.num_blocks, self.block_size,
+                            self.block_table.data_ptr(), self.block_table.stride(0), self.max_blocks_per_seq)
+
+    def gather(self, seq: int, rows: int):
+        """K and V rows [Hkv, rows, D] of sequence `seq` as fp32 values (for tests)."""
+        idx = torch.tensor(self.blocks_of(seq)[: -(-rows // self.block_size)], dtype=torch.long,
+                           device=self.k_pool.device)
+        out = []
+        for pool, exps in ((self.k_pool, self.k_exp), (self.v_pool, self.v_exp)):
+            v = pool.view(torch.uint8)[idx].view(FP8).float().transpose(0, 1).flatten(1, 2)[:, :rows]
+            e = exps[idx].transpose(0, 1).flatten(1, 2)[:, :rows]
+            out.append(torch.ldexp(v, (e.int() - 127).unsqueeze(-1)))
+        return out[0], out[1]
+
+
+class PagedSlot8(PagedSlot, PagedKVCache8):
+    """PagedSlot of an 8-bit cache."""
+
+    def __init__(self, parent: PagedKVCache8, seq: int, count: int = 1):
+        PagedSlot.__init__(self, parent, seq, count)
+        self.k_exp, self.v_exp, self.one_each = parent.k_exp, parent.v_exp, parent.one_each
+
+    def gather(self, seq: int, rows: int):
+        return PagedKVCache8.gather(self, seq, rows)
+
+
 class DecodeWorkspace:
     """Grow-only, zero-filled device scratch for the split-K decode partials (the C ABI never
     allocates).  Its 256-byte header must start at zero; every call leaves it zero."""
@@ -383,6 +444,175 @@ def _capturing() -> bool:
     return True
 
 
+def _check_int(name: str, t: torch.Tensor, n: int, dtype, device) -> None:
+    """A contiguous device vector of exactly n whole numbers."""
+    if t.device != device or t.dtype != dtype or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
+        raise RuntimeError(f"{name}: expected a contiguous {dtype} tensor of {n} elements on {device}")
+
+
+class _on_device:
+    """Makes a tensor's device the current one around a call, if it is not already: the library
+    launches on the current device, in torch's current stream of it."""
+
+    def __init__(self, t: torch.Tensor):
+        self.idx = t.device.index
+        self.prev = None
+
+    def __enter__(self):
+        cur = torch.cuda.current_device()
+        if cur != self.idx:
+            self.prev = cur
+            torch.cuda.set_device(self.idx)
+
+    def __exit__(self, *exc):
+        if self.prev is not None:
+            torch.cuda.set_device(self.prev)
+        return False
+
+
+def qkv_epilogue_kv8(q, k, v, kv_cache: PagedKVCache8, cu_seqlens: torch.Tensor, start: torch.Tensor, positions=None,
+                     rope_theta: float = 1e4, rope_table=None, q_norm_weight=None, k_norm_weight=None,
+                     eps: float = 1e-6, out: torch.Tensor | None = None) -> torch.Tensor:
+    """The QKV epilogue over an 8-bit cache: per-head QK-RMSNorm (optional), RoPE, and the
+    quantising append of K and V.  q [T, H, D], k/v [T, Hkv, D] bf16 (strided views of the
+    projections, D contiguous); sequence b owns the tokens cu_seqlens[b] .. cu_seqlens[b+1] - 1
+    (int32 device [n + 1]) and they go to its cache rows from start[b] (int32 device [n]) on, whose
+    blocks must be reserved; tokens behind the last sequence are left out.  Angles: rope_table =
+    (cos, sin) fp32 [T, D], or positions int64 [T] and rope_theta.  Returns Q [T, H, D] (rotated);
+    `out` takes it in another layout.  The cache's lengths are the caller's to advance; the
+    functions below do both."""
+    for n, t in (("q", q), ("k", k), ("v", v)):
+        _check_cuda_bf16(n, t)
+        if t.dim() != 3 or t.stride(2) != 1:
+            raise RuntimeError(f"Attention: {n} must be rank-3 [T, h, D] with D contiguous")
+    if not isinstance(kv_cache, PagedKVCache8):
+        raise RuntimeError("qkv_epilogue_kv8: needs a PagedKVCache8")
+    T, H, D = q.shape
+    Hkv = k.shape[1]
+    if k.shape != (T, Hkv, D) or v.shape != k.shape:
+        raise RuntimeError("Attention: k and v must be [T, num_kv_heads, D] for q's T and D")
+    if kv_cache.k_pool.shape[1] != Hkv or kv_cache.k_pool.shape[3] != D:
+        raise RuntimeError("Attention: the cache has other kv heads or another head_dim")
+    dev = q.device
+    if k.device != dev or v.device != dev or kv_cache.k_pool.device != dev:
+        raise RuntimeError("Attention: q, k, v and the cache must be on one device")
+    n = start.numel()
+    if n > kv_cache.block_table.shape[0]:
+        raise RuntimeError("Attention: more sequences than the cache has rows for")
+    _check_int("cu_seqlens", cu_seqlens, n + 1, torch.int32, dev)
+    _check_int("start", start, n, torch.int32, dev)
+    cos = sin = None
+    if rope_table is not None:
+        cos, sin = rope_table
+        for t in (cos, sin):
+            if t.device != dev or t.dtype != torch.float32 or t.shape != (T, D) or not t.is_contiguous():
+                raise RuntimeError("RoPE: tables must be contiguous fp32 [T, D] on q's device")
+    else:
+        if positions is None:
+            raise RuntimeError("RoPE: positions or rope_table required")
+        _check_int("positions", positions, T, torch.int64, dev)
+    if (q_norm_weight is None) != (k_norm_weight is None):
+        raise RuntimeError("Attention: give both q/k norm weights or neither")
+    qn = kn = None
+    if q_norm_weight is not None:
+        qn, kn = (w if w.dtype == BF16 and w.is_contiguous() else w.to(BF16).contiguous()
+                  for w in (q_norm_weight, k_norm_weight))
+        if qn.shape != (D,) or kn.shape != (D,) or qn.device != dev or kn.device != dev:
+            raise RuntimeError("Attention: norm weights must be [D] on q's device")
+    if out is None:
+        out = torch.empty((T, H, D), dtype=BF16, device=dev)
+    elif out.shape != q.shape or out.dtype != BF16 or out.device != dev or out.stride(2) != 1:
+        raise RuntimeError("Attention: out must be bf16 [T, H, D] with D contiguous on q's device")
+    with _on_device(q):
+        abi.call("mllm_qkv_epilogue_varlen_paged_kv8", _ptr(q), q.stride(0), q.stride(1), _ptr(k), k.stride(0),
+                 k.stride(1), _ptr(v), v.stride(0), v.stride(1), T, H, Hkv, D, None if cos is not None else _ptr(positions),
+                 float(rope_theta), _ptr(cos), _ptr(sin), _ptr(qn), _ptr(kn), float(eps), _ptr(out), out.stride(0),
+                 out.stride(1), C.byref(kv_cache.descriptor()), _ptr(cu_seqlens), n, _ptr(start), abi.stream_handle())
+    return out
+
+
+def kv8_read(kv_cache: PagedKVCache8, lens: torch.Tensor, rows: int, first: torch.Tensor | None = None):
+    """Cached rows as bf16, exactly: rows first[b] (default 0) .. lens[b] - 1 of sequence b (int32
+    device vectors) at rows 0 .. of its part of K and V [n, Hkv, rows, D]; rows past the end of a
+    sequence are zero."""
+    if not isinstance(kv_cache, PagedKVCache8):
+        raise RuntimeError("kv8_read: needs a PagedKVCache8")
+    dev = kv_cache.k_pool.device
+    n = lens.numel()
+    if rows < 0 or n > kv_cache.block_table.shape[0]:
+        raise RuntimeError("kv8_read: negative rows, or more sequences than the cache has rows for")
+    _check_int("lens", lens, n, torch.int32, dev)
+    if first is not None:
+        _check_int("first", first, n, torch.int32, dev)
+    _, Hkv, _, D = kv_cache.k_pool.shape
+    k = torch.empty((n, Hkv, rows, D), dtype=BF16, device=dev)
+    v = torch.empty_like(k)
+    with _on_device(k):
+        abi.call("mllm_kv8_read_bf16", C.byref(kv_cache.descriptor()), _ptr(first), _ptr(lens), n, Hkv, D, rows, _ptr(k),
+                 _ptr(v), Hkv * rows * D, rows * D, D, abi.stream_handle())
+    return k, v
+
+
+def _decode_kv8(q: torch.Tensor, kv_cache: PagedKVCache8, num_kv_heads: int, max_kv_len: int) -> torch.Tensor:
+    """decode_attention over an 8-bit cache: q [B, H, D] contiguous."""
+    B, H, D = q.shape
+    if q.device != kv_cache.k_pool.device:
+        raise RuntimeError("Attention: q and the cache must be on one device")
+    if kv_cache.k_pool.shape[1] != num_kv_heads or kv_cache.k_pool.shape[3] != D or B > kv_cache.block_table.shape[0]:
+        raise RuntimeError("Attention: the cache has other kv heads, another head_dim or fewer sequences")
+    out = torch.empty((B, 1, H * D), dtype=BF16, device=q.device)
+    # a workspace of the call's own, from torch's stream-ordered allocator (a captured graph's from its pool)
+    nbytes = abi.load().mllm_decode_attention_kv8_workspace_size(H, num_kv_heads, D)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    with _on_device(q):
+        abi.call("mllm_decode_attention_paged_kv8", _ptr(q), C.byref(kv_cache.descriptor()), _ptr(kv_cache.lengths), B, H,
+                 num_kv_heads, D, max_kv_len, 1.0 / math.sqrt(D), _ptr(out), _ptr(ws), nbytes, abi.stream_handle())
+    return out
+
+
+def _flat_tokens(t: torch.Tensor) -> torch.Tensor:
+    """[B, h, S, D] -> [B * S, h, D] (a view where the strides allow it)."""
+    B, h, S, D = t.shape
+    return t.transpose(1, 2).reshape(B * S, h, D)
+
+
+def _epilogue_kv8_batch(q, k, v, cache: PagedKVCache8, positions, rope_theta, qn, kn, eps, rope_table, out):
+    """qkv_epilogue of [B, h, S, D] tensors into an 8-bit cache whose blocks are reserved, from its present
+    device lengths on; `out` [B * S, H, D] takes Q."""
+    B, H, S, D = q.shape
+    pos = table = None
+    if rope_table is not None:
+        table = tuple(t.to(torch.float32) for t in rope_table)
+        if table[0].shape[0] != B * S:
+            table = tuple(t.repeat(B, 1) for t in table)
+        table = tuple(t.contiguous() for t in table)
+    else:
+        pos = positions.to(torch.int64)
+        if pos.numel() == B * S:
+            pos = pos.reshape(-1).contiguous()
+        else:
+            pos = (pos.reshape(1, -1) if pos.dim() < 2 else pos).expand(B, S).reshape(-1)
+    cu = cache.one_each[:B + 1] if S == 1 else torch.arange(0, B * S + 1, S, dtype=torch.int32, device=q.device)
+    qkv_epilogue_kv8(_flat_tokens(q), _flat_tokens(k), _flat_tokens(v), cache, cu, cache.lengths[:B], pos, rope_theta,
+                     table, qn, kn, eps, out)
+
+
+def _prefill_kv8(q: torch.Tensor, cache: PagedKVCache8, cu_dev: torch.Tensor, B: int, max_q: int, num_kv_heads: int):
+    """Causal attention of packed Q [H, T, D] over an 8-bit cache: the sequences' rows are read back (exactly) into
+    bf16 staging and go through the varlen prefill kernel, so a row sees the values every later step sees."""
+    H, T, D = q.shape
+    out = torch.empty((T, H * D), dtype=BF16, device=q.device)
+    if T == 0:
+        return out
+    lens = cache.lengths[:B]
+    rows = max(cache.host_lengths()[:B])
+    kst, vst = kv8_read(cache, lens, rows)
+    abi.call("mllm_prefill_attention_varlen_bf16", _ptr(q), _ptr(kst), _ptr(vst), num_kv_heads * rows * D, rows * D, D,
+             rows, _ptr(cu_dev), _ptr(lens), B, H, num_kv_heads, D, T, max_q, 1.0 / math.sqrt(D), _ptr(out),
+             abi.stream_handle())
+    return out
+
+
 def qkv_epilogue(q, k, v, kv_cache: KVCache, positions: torch.Tensor, rope_theta: float,
                  q_norm_weight=None, k_norm_weight=None, eps: float = 1e-6,
                  rope_table=None) -> torch.Tensor:
@@ -397,6 +627,14 @@ def qkv_epilogue(q, k, v, kv_cache: KVCache, positions: torch.Tensor, rope_theta
     Hkv = k.shape[1]
     if H % Hkv != 0:
         raise RuntimeError("Attention: num_heads must be divisible by num_kv_heads.")
+    if isinstance(kv_cache, PagedKVCache8):
+        for b in range(B):
+            kv_cache.reserve(b, kv_cache.host_lengths()[b] + S)
+        packed = torch.empty((H, B * S, D), dtype=BF16, device=q.device)   # the layout the packed prefill reads
+        _epilogue_kv8_batch(q, k, v, kv_cache, positions, rope_theta, q_norm_weight, k_norm_weight, eps, rope_table,
+                            packed.transpose(0, 1))
+        kv_cache.advance(S, batch=B)
+        return packed.view(H, B, S, D).transpose(0, 1)
     q_out = torch.empty((B, H, S, D), dtype=BF16, device=q.device)
     pos = positions.to(torch.int64)
     if pos.dim() == 1:
@@ -442,6 +680,10 @@ def qkv_epilogue(q, k, v, kv_cache: KVCache, positions: torch.Tensor, rope_theta
 def prefill_attention(q: torch.Tensor, kv_cache: KVCache, num_kv_heads: int) -> torch.Tensor:
     """Causal attention of Q [B,H,S,D] (the newest S rows) over the cache -> [B, S, H*D]."""
     B, H, S, D = q.shape
+    if isinstance(kv_cache, PagedKVCache8):
+        cu = torch.arange(0, B * S + 1, S, dtype=torch.int32, device=q.device) if S else None
+        packed = q.transpose(0, 1).reshape(H, B * S, D)
+        return _prefill_kv8(packed, kv_cache, cu, B, S, num_kv_heads).view(B, S, H * D)
     out = torch.empty((B, S, H * D), dtype=BF16, device=q.device)
     if isinstance(kv_cache, PagedKVCache):
         kv = kv_cache.descriptor()
@@ -495,6 +737,13 @@ def qkv_epilogue_packed(q, k, v, kv_cache, q_lens: list[int], rope_theta: float,
     pos = positions.to(device=q.device, dtype=torch.int64).contiguous()
     if pos.numel() != T:
         raise RuntimeError("packed sequences: one position per token")
+    if isinstance(kv_cache, PagedKVCache8):
+        q_out = torch.empty((H, T, D), dtype=BF16, device=q.device)
+        start = kv_cache.lengths[:B].clone()
+        kv_cache.advance(list(q_lens), batch=B)
+        qkv_epilogue_kv8(q, k, v, kv_cache, cu_dev, start, pos.reshape(-1), rope_theta, None, q_norm_weight,
+                         k_norm_weight, eps, q_out.transpose(0, 1))
+        return q_out
     qn = kn = None
     if q_norm_weight is not None:
         qn = q_norm_weight.to(BF16).contiguous()
@@ -528,8 +777,10 @@ def prefill_attention_packed(q: torch.Tensor, kv_cache, q_lens: list[int], num_k
     cu, cu_dev = _cu_seqlens(q_lens, q.device)
     if cu[-1] != T:
         raise RuntimeError("packed sequences: q_lens must sum to the token count")
-    out = torch.empty((T, H * D), dtype=BF16, device=q.device)
     max_q = max(q_lens) if q_lens else 0
+    if isinstance(kv_cache, PagedKVCache8):
+        return _prefill_kv8(q.contiguous(), kv_cache, cu_dev, B, max_q, num_kv_heads)
+    out = torch.empty((T, H * D), dtype=BF16, device=q.device)
     kv_lens = kv_cache.lengths[:B]
     if isinstance(kv_cache, PagedKVCache):
         kv = kv_cache.descriptor()
@@ -553,6 +804,9 @@ def decode_attention(q: torch.Tensor, kv_cache: KVCache, num_kv_heads: int,
         qq = qq.contiguous()
     L = max_kv_len or max(kv_cache.host_lengths()[:B])
     L = min(L, kv_cache.capacity)
+    if isinstance(kv_cache, PagedKVCache8):
+        _check_cuda_bf16("q", qq)
+        return _decode_kv8(qq, kv_cache, num_kv_heads, L)
     out = torch.empty((B, 1, H * D), dtype=BF16, device=q.device)
     lib = abi.load()
     nbytes = lib.mllm_decode_attention_workspace_size(B, H, num_kv_heads, D, L)
@@ -569,6 +823,26 @@ def decode_attention(q: torch.Tensor, kv_cache: KVCache, num_kv_heads: int,
     return out
 
 
+def _decode_step_kv8(q, k, v, cache: PagedKVCache8, positions, rope_theta, num_kv_heads, qn, kn, eps, rope_table):
+    """decode_step over an 8-bit cache: the epilogue appends at the device lengths, which then advance."""
+    B, H, _, D = q.shape
+    capturing = _capturing()
+    if capturing and cache.capture_max_len is None:
+        raise RuntimeError("decode_step: set the cache's capture_max_len before capturing a graph")
+    if not capturing:   # raises before any launch if the pool is full
+        for b in range(B):
+            cache.reserve(b, cache.host_lengths()[b] + 1)
+    q_rot = torch.empty((B, H, D), dtype=BF16, device=q.device)
+    _epilogue_kv8_batch(q, k, v, cache, positions, rope_theta, qn, kn, eps, rope_table, q_rot)
+    if capturing:
+        cache.lengths[:B] += 1
+        L = cache.capture_max_len
+    else:
+        cache.advance(1, batch=B)
+        L = max(cache.host_lengths()[:B])
+    return _decode_kv8(q_rot, cache, num_kv_heads, min(L, cache.capacity))
+
+
 def decode_step(q, k, v, kv_cache: KVCache, positions: torch.Tensor, rope_theta: float, num_kv_heads: int,
                 q_norm_weight=None, k_norm_weight=None, eps: float = 1e-6, rope_table=None) -> torch.Tensor:
     """One new token per sequence through the fused step: QK-RMSNorm (optional) + RoPE + KV
@@ -582,6 +856,9 @@ def decode_step(q, k, v, kv_cache: KVCache, positions: torch.Tensor, rope_theta:
     B, H, _, D = q.shape
     if H % num_kv_heads != 0:
         raise RuntimeError("Attention: num_heads must be divisible by num_kv_heads.")
+    if isinstance(kv_cache, PagedKVCache8):
+        return _decode_step_kv8(q, k, v, kv_cache, positions, rope_theta, num_kv_heads, q_norm_weight, k_norm_weight,
+                                eps, rope_table)
     pos = positions.to(torch.int64).reshape(-1)
     pos_sb = 0 if pos.numel() == 1 else pos.stride(0)
     cos = sin = None
