@@ -12,6 +12,7 @@
  *   mllm_*_paged_bf16           the same four over a paged KV cache (block tables)
  *   mllm_*_varlen_*             epilogue and prefill over packed sequences of different
  *                               lengths (several prompts in one launch each)
+ *   mllm_decode_attention_shared_paged_bf16  decode for a batch that shares a prefix
  *   mllm_*_kv8                  epilogue, read-back and decode over an 8-bit paged KV cache
  *   mllm_sample                 Sampler::Sample on the device (penalty, greedy / top-k / top-p)
  *
@@ -438,6 +439,26 @@ MLLM_API int mllm_decode_attention_paged_kv8(const void* q, const mllm_paged_kv8
                                              int num_heads, int num_kv_heads, int head_dim, int max_kv_len,
                                              float softmax_scale, void* out, void* workspace, size_t workspace_bytes,
                                              mllm_stream_t stream);
+
+/* ----------------------------------------------------------------------------------------
+ * Decode attention over a paged cache for a batch that shares a prefix: cache rows 0 ..
+ * prefix_len - 1 are the same for every sequence of the call (a system prompt, a document) and are
+ * read through block-table row 0, once for the whole batch; rows prefix_len .. kv_lens[b] - 1 are
+ * each sequence's own, through its own table row.  The result is that of
+ * mllm_decode_attention_paged_bf16 over caches that hold equal rows there; whether the tables share
+ * the blocks or hold copies makes no difference.  prefix_len 0 is the plain decode.
+ *   q, out, head_dim, group size, softmax_scale: as mllm_decode_attention_paged_bf16, q 16-byte
+ *       aligned.  kv_lens: int32 device [batch], required, prefix_len <= kv_lens[b] <= max_kv_len;
+ *       0 gives zeros; any other length records MLLM_ERR_DEVICE_LENGTH.
+ *   workspace: mllm_decode_attention_shared_workspace_size() bytes, 256-byte aligned, contents need not
+ *       be initialised; calls that may run at the same time need separate ones. */
+MLLM_API size_t mllm_decode_attention_shared_workspace_size(int batch, int num_heads, int num_kv_heads, int head_dim,
+                                                            int prefix_len);
+
+MLLM_API int mllm_decode_attention_shared_paged_bf16(const void* q, const mllm_paged_kv* kv, const int32_t* kv_lens,
+                                                     int prefix_len, int batch, int num_heads, int num_kv_heads,
+                                                     int head_dim, int max_kv_len, float softmax_scale, void* out,
+                                                     void* workspace, size_t workspace_bytes, mllm_stream_t stream);
 
 /* ----------------------------------------------------------------------------------------
  * Token sampling on the device.  Replaces src/core/runtime/Sampler.cpp:49-232

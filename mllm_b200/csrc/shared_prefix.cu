@@ -1,0 +1,521 @@
+// Decode attention for a batch whose sequences share their first rows (a system prompt, a document).
+//
+// With P shared rows the plain decode reads them once per sequence.  Here the query rows of all sequences of one
+// kv head meet the prefix together: a [B * n_rep, D] x [D, P] product per kv head, which reads the prefix once and
+// is work for the tensor cores; every sequence's own rows go through the even-split decode (decode_stream.cu), and
+// its combine kernel joins the parts of both by their maxima and sums.
+//
+// prefix_kernel: one CTA per (kv head, block of query rows, stretch of the prefix); the machinery is that of the
+// prefill kernel (tcgen05.mma M = 128, scores and O in tensor memory, one softmax thread per row, TMA ring with
+// separate K and V barriers), without a causal bound and with two forms:
+//   two query tiles (kPair): 256 query rows share every K/V tile.  For batches of more than 128 rows, where the
+//       tensor and exponential work per K/V byte is what bounds.
+//   one query tile: 128 rows, and the two softmax groups take alternate K/V tiles, each with its own running
+//       maximum, sum and O.  With so few rows the kernel is bound by the K/V bytes; alternating keeps one tile's
+//       products running under the other's softmax, and the Q tile not needed makes room for a third stage.
+// A query tile holds floor(128 / n_rep) sequences with their n_rep heads, fetched by one TMA box
+// {64 columns, n_rep heads, sequences}; rows behind them are never looked at.  Warps without a valid row skip
+// their softmax.  The stretches leave normalised fp32 rows and log2 weights.
+// The rows of the last K/V tile behind the prefix are other rows of the block: K's are masked, V's read as zero
+// through a tensor map that ends with the prefix, so that their contents cannot matter.
+//
+// P is bf16 for the second product (A and B of an MMA have one type, and V is bf16); sums and O are fp32.
+#include <algorithm>
+#include <cmath>
+
+#include "common.cuh"
+#include "decode_stream.cuh"
+#include "host_util.h"
+#include "kv_layout.cuh"
+#include "tcgen05.cuh"
+
+namespace mllm_b200 {
+namespace {
+
+constexpr int kBM = 128;            // query rows per tile
+constexpr int kBN = 128;            // cache rows per K/V tile
+constexpr int kThreads = 384;       // {producer, MMA, 2 idle warps}, softmax group 0, softmax group 1
+// The register split of the prefill kernel: 128 x 72 + 256 x 216 = 384 x 168.
+constexpr uint32_t kLaunchRegs = 168;
+constexpr uint32_t kLowRegs = 72;
+constexpr uint32_t kHighRegs = 216;
+static_assert(128 * kLowRegs + 256 * kHighRegs <= kThreads * kLaunchRegs, "register split exceeds the launch");
+constexpr int kBox = kBN * 128;     // one 128-row x 64-column bf16 box (16 KB)
+constexpr uint32_t kTmemCols = 512; // S_0, S_1, O_0, O_1 of 128 columns
+constexpr float kRescaleThreshold = 8.0f;  // log2 units: O is rescaled only when the maximum grows by more
+
+template <int D, bool kPair>
+struct PrefixCfg {
+    static constexpr int kBoxes = D / 64;
+    static constexpr int kTileBytes = kBoxes * kBox;                 // one Q, K or V tile
+    static constexpr int kQTiles = kPair ? 2 : 1;
+    static constexpr int kStages = D == 128 ? (kPair ? 2 : 3) : 4;
+    static constexpr int kSmemBytes = (kQTiles + 2 * kStages) * kTileBytes + 256 + 1024;
+    static_assert((1 + 4 * kStages + 6) * 8 + 4 <= 256, "barrier area too small");
+    static_assert(kSmemBytes <= 232448, "more shared memory than a CTA has");
+};
+
+struct PrefixArgs {
+    float* part_o;       // [parts][Hkv][B][n_rep][D]
+    float* part_lse;     // [parts][Hkv][B][n_rep]
+    int B, Hkv, n_rep, seqs;   // seqs: sequences per query tile
+    int prefix, n_tiles, per;  // K/V tiles of the prefix; tiles per stretch
+    int mblocks;
+    float scale_log2;
+    KvLayout lay;
+};
+
+__device__ __forceinline__ uint32_t col_s(int i) { return (uint32_t)(i * kBN); }
+__device__ __forceinline__ uint32_t col_o(int i) { return (uint32_t)(2 * kBN + i * 128); }
+
+template <int D, bool kPair>
+__global__ void __launch_bounds__(kThreads, 1)
+    prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                  const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmVend, PrefixArgs a) {
+    using C = PrefixCfg<D, kPair>;
+    constexpr int ST = C::kStages;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* sQ = smem;
+    uint8_t* sKV = sQ + C::kQTiles * C::kTileBytes;      // [ST][K | V]
+    uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + ST * 2 * C::kTileBytes);
+    uint64_t* q_full = bars;
+    uint64_t* k_full = bars + 1;
+    uint64_t* k_empty = k_full + ST;
+    uint64_t* v_full = k_empty + ST;
+    uint64_t* v_empty = v_full + ST;
+    uint64_t* s_full = v_empty + ST;    // [2]
+    uint64_t* p_full = s_full + 2;      // [2] 128 arrivals
+    uint64_t* o_done = p_full + 2;      // [2]
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_done + 2);
+
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    const int g = blockIdx.x % a.Hkv;
+    const int mb = blockIdx.x / a.Hkv;
+    const int split = blockIdx.y;
+    const int first = split * a.per;                     // K/V tiles first .. first + n - 1
+    const int n = min(a.per, a.n_tiles - first);
+    // Step k of softmax group i works on tile k (pair form) or 2 k + i (alternating); group i has steps[i] steps.
+    int steps[2];
+    if (kPair) {
+        steps[0] = n;
+        steps[1] = (2 * mb + 1) * a.seqs < a.B ? n : 0;   // a last block may hold one query tile
+    } else {
+        steps[0] = (n + 1) / 2;
+        steps[1] = n / 2;
+    }
+
+    if (threadIdx.x == 0) {
+        mbar_init(q_full, 1);
+        for (int s = 0; s < ST; ++s) {
+            mbar_init(&k_full[s], 1);
+            mbar_init(&k_empty[s], 1);
+            mbar_init(&v_full[s], 1);
+            mbar_init(&v_empty[s], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], 128);
+            mbar_init(&o_done[i], 1);
+        }
+        mbar_fence_init();
+    }
+    if (warp == 1) {
+        tmem_alloc(tmem_slot, kTmemCols);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    pdl_wait();
+    pdl_trigger();   // the decode of the sequences' own rows may fill SMs as these CTAs leave them
+
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLowRegs));
+        if (warp == 0) {
+            // ------------------------------- TMA producer -------------------------------
+            if (lane == 0) {
+                tma_prefetch_desc(&tmQ);
+                tma_prefetch_desc(&tmK);
+                tma_prefetch_desc(&tmV);
+                const int q_tiles = kPair && steps[1] > 0 ? 2 : 1;
+                const uint32_t q_box = 128u * (uint32_t)(a.n_rep * a.seqs);   // bytes of one 64-column box
+                mbar_arrive_expect_tx(q_full, (uint32_t)q_tiles * C::kBoxes * q_box);
+                for (int i = 0; i < q_tiles; ++i)
+                    for (int bx = 0; bx < C::kBoxes; ++bx)
+                        tma_load_4d(sQ + i * C::kTileBytes + bx * kBox, &tmQ, q_full, bx * 64, g * a.n_rep,
+                                    ((kPair ? 2 * mb : mb) + i) * a.seqs, 0);
+                for (int j = 0; j < n; ++j) {
+                    const int stage = j % ST;
+                    const uint32_t phase = ((j / ST) & 1) ^ 1;
+                    uint8_t* sk = sKV + stage * 2 * C::kTileBytes;
+                    uint8_t* sv = sk + C::kTileBytes;
+                    int blk, row;
+                    kv_locate(a.lay, 0, (int64_t)(first + j) * kBN, blk, row);   // a bad entry reads block 0
+                    const CUtensorMap* mv = first + j == a.n_tiles - 1 ? &tmVend : &tmV;
+                    if (!mbar_wait(&k_empty[stage], phase)) break;
+                    mbar_arrive_expect_tx(&k_full[stage], C::kTileBytes);
+#pragma unroll
+                    for (int bx = 0; bx < C::kBoxes; ++bx)
+                        tma_load_4d(sk + bx * kBox, &tmK, &k_full[stage], bx * 64, row, g, blk);
+                    if (!mbar_wait(&v_empty[stage], phase)) break;
+                    mbar_arrive_expect_tx(&v_full[stage], C::kTileBytes);
+#pragma unroll
+                    for (int bx = 0; bx < C::kBoxes; ++bx)
+                        tma_load_4d(sv + bx * kBox, mv, &v_full[stage], bx * 64, row, g, blk);
+                }
+            }
+        } else if (warp == 1) {
+            // ------------------------------- MMA issuer -------------------------------
+            if (lane == 0) {
+                constexpr uint32_t idesc_s = idesc_bf16_f32(kBM, kBN, false);
+                constexpr uint32_t idesc_o = idesc_bf16_f32(kBM, D, true);
+                constexpr uint32_t desc_hi = smem_desc_hi_sw128(1024);
+                auto tile_of = [&](int i, int k) { return kPair ? k : 2 * k + i; };
+                auto issue_s = [&](int i, int j) {
+                    const uint32_t qd = smem_desc_lo(smem_u32(sQ + (kPair ? i : 0) * C::kTileBytes), 16);
+                    const uint32_t kd = smem_desc_lo(smem_u32(sKV + (j % ST) * 2 * C::kTileBytes), 16);
+#pragma unroll
+                    for (int ks = 0; ks < D / 16; ++ks) {
+                        const uint32_t off = (uint32_t)(((ks >> 2) * kBox + (ks & 3) * 32) >> 4);
+                        tc_mma_ss_w(tmem + col_s(i), qd + off, kd + off, desc_hi, idesc_s, ks > 0 ? 1u : 0u);
+                    }
+                    tc_commit(&s_full[i]);
+                };
+                // K tile j has been read by every product that needs it: free it if it will be refilled
+                auto free_k = [&](int j) { if (j + ST < n) tc_commit(&k_empty[j % ST]); };
+                bool alive = mbar_wait(q_full, 0);
+                for (int i = 0; i < 2 && alive; ++i) {
+                    if (steps[i] == 0) continue;
+                    const int j = tile_of(i, 0);
+                    if ((i == 0 || !kPair) && !mbar_wait(&k_full[j % ST], (j / ST) & 1)) { alive = false; break; }
+                    tc_fence_after();
+                    issue_s(i, j);
+                    if (!kPair || i == 1 || steps[1] == 0) free_k(j);
+                }
+                for (int k = 0; k < steps[0] && alive; ++k) {
+                    bool v_ready = false, k_ready = false;
+                    for (int i = 0; i < 2 && alive; ++i) {
+                        if (k >= steps[i]) continue;
+                        const int j = tile_of(i, k);
+                        if (!mbar_wait(&p_full[i], k & 1)) { alive = false; break; }
+                        if (!kPair || !v_ready) {
+                            if (!mbar_wait(&v_full[j % ST], (j / ST) & 1)) { alive = false; break; }
+                            v_ready = true;
+                        }
+                        tc_fence_after();
+                        const uint32_t vd = smem_desc_lo(smem_u32(sKV + (j % ST) * 2 * C::kTileBytes + C::kTileBytes), kBox);
+#pragma unroll
+                        for (int ks = 0; ks < kBN / 16; ++ks)
+                            tc_mma_ts_w(tmem + col_o(i), tmem + col_s(i) + ks * 8, vd + (uint32_t)((ks * 16 * 128) >> 4),
+                                        desc_hi, idesc_o, (k > 0 || ks > 0) ? 1u : 0u);
+                        const bool last_use = !kPair || i == 1 || steps[1] == 0;
+                        if (last_use && j + ST < n) tc_commit(&v_empty[j % ST]);
+                        if (k + 1 < steps[i]) {
+                            const int jn = tile_of(i, k + 1);
+                            if (!kPair || !k_ready) {
+                                if (!mbar_wait(&k_full[jn % ST], (jn / ST) & 1)) { alive = false; break; }
+                                tc_fence_after();
+                                k_ready = true;
+                            }
+                            issue_s(i, jn);   // overwrites P_i(k) only after the product above read it
+                            if (last_use) free_k(jn);
+                        } else {
+                            tc_commit(&o_done[i]);
+                        }
+                    }
+                }
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kHighRegs));
+        // --------------------------------- softmax ---------------------------------
+        const int grp = (warp - 4) >> 2;
+        const int quad = warp & 3;               // TMEM lane quadrant of this warp
+        const int row = quad * 32 + lane;
+        const int qt = kPair ? 2 * mb + grp : mb;
+        const int b = qt * a.seqs + row / a.n_rep;
+        const bool valid = row < a.seqs * a.n_rep && b < a.B;
+        const bool work = __any_sync(0xffffffffu, valid);   // a warp without a valid row only keeps the barriers going
+        const uint32_t t_lane = tmem + ((uint32_t)(quad * 32) << 16);
+        const uint32_t t_s = t_lane + col_s(grp);
+        const uint32_t t_o = t_lane + col_o(grp);
+        constexpr int kAcc = 8;
+        float m_run = -INFINITY, l_run = 0.f;
+        bool alive = true;
+        const int ns = grp == 0 ? steps[0] : steps[1];
+        for (int k = 0; k < ns; ++k) {
+            if (!mbar_wait(&s_full[grp], k & 1)) { alive = false; break; }
+            tc_fence_after();
+            if (work) {
+                const int j = first + (kPair ? k : 2 * k + grp);
+                float sv[kBN];
+#pragma unroll
+                for (int c = 0; c < kBN / 32; ++c)
+                    tmem_ld32(t_s + c * 32, *reinterpret_cast<float(*)[32]>(&sv[c * 32]));
+                tmem_wait_ld();
+                const int lim = a.prefix - j * kBN;     // columns before this one are prefix rows
+                if (lim < kBN) {
+#pragma unroll
+                    for (int c = 0; c < kBN; ++c) sv[c] = c < lim ? sv[c] : -INFINITY;
+                }
+                float mx[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) mx[i] = fmaxf(sv[2 * i], sv[2 * i + 1]);
+#pragma unroll
+                for (int c = 8; c < kBN; c += 8)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) mx[i] = fmax3(mx[i], sv[c + 2 * i], sv[c + 2 * i + 1]);
+                mx[0] = fmax3(mx[0], mx[1], fmaxf(mx[2], mx[3]));
+                const float mt = mx[0] * a.scale_log2;
+                const float m_new = fmaxf(m_run, mt);
+                const bool grow = (m_new - m_run) > kRescaleThreshold;   // true on the first tile
+                float m_use = grow ? m_new : m_run;
+                if (m_use == -INFINITY) m_use = 0.f;
+                const float alpha = grow ? ex2_approx(m_run - m_use) : 1.f;
+                if (k > 0 && __any_sync(0xffffffffu, grow)) {
+                    // the product of step k - 1 is complete (S of step k completed after it)
+#pragma unroll
+                    for (int c = 0; c < D / 32; ++c) {
+                        float o[32];
+                        tmem_ld32(t_o + c * 32, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] *= alpha;
+                        tmem_st32(t_o + c * 32, o);
+                    }
+                }
+                const float neg_m = -m_use;
+                float sum[kAcc];
+#pragma unroll
+                for (int i = 0; i < kAcc; ++i) sum[i] = 0.f;
+#pragma unroll
+                for (int c = 0; c < kBN / 32; ++c) {
+                    uint32_t pk[16];
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) {
+                        float x0, x1;
+                        fma2(x0, x1, sv[c * 32 + e], sv[c * 32 + e + 1], a.scale_log2, a.scale_log2, neg_m, neg_m);
+                        const float p0 = ex2_approx(x0);
+                        const float p1 = ex2_approx(x1);
+                        add2(sum[(e >> 1) % 4 * 2], sum[(e >> 1) % 4 * 2 + 1], p0, p1);
+                        pk[e >> 1] = pack_bf16x2(p0, p1);
+                    }
+                    tmem_st16(t_s + c * 16, pk);
+                }
+                tmem_wait_st();
+                add2(sum[0], sum[1], sum[2], sum[3]);
+                add2(sum[4], sum[5], sum[6], sum[7]);
+                add2(sum[0], sum[1], sum[4], sum[5]);
+                l_run = l_run * alpha + (sum[0] + sum[1]);
+                m_run = m_use;
+            }
+            tc_fence_before();
+            mbar_arrive(&p_full[grp]);
+        }
+        if (ns > 0 && alive && mbar_wait(&o_done[grp], 0) && work) {
+            tc_fence_after();
+            const float inv_l = l_run != 0.f ? 1.f / l_run : 0.f;
+            const int part = kPair ? split : 2 * split + grp;
+            const int64_t prow = (((int64_t)part * a.Hkv + g) * a.B + b) * a.n_rep + row % a.n_rep;
+            float* dst = a.part_o + prow * D;
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+                float o[32];
+                tmem_ld32(t_o + c * 32, o);
+                tmem_wait_ld();
+                if (valid) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4)
+                        *reinterpret_cast<float4*>(dst + c * 32 + i) =
+                            make_float4(o[i] * inv_l, o[i + 1] * inv_l, o[i + 2] * inv_l, o[i + 3] * inv_l);
+                }
+            }
+            if (valid) a.part_lse[prow] = l_run != 0.f ? m_run + log2f(l_run) : -INFINITY;
+        } else if (!kPair && ns == 0 && valid) {
+            // a stretch of one tile has no tile for the second group: an empty part
+            const int64_t prow = (((int64_t)(2 * split + grp) * a.Hkv + g) * a.B + b) * a.n_rep + row % a.n_rep;
+            for (int i = 0; i < D; i += 4) *reinterpret_cast<float4*>(a.part_o + prow * D + i) = make_float4(0.f, 0.f, 0.f, 0.f);
+            a.part_lse[prow] = -INFINITY;
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, kTmemCols);
+    }
+}
+
+// The split of the prefix: query tiles of `seqs` sequences, pairs of them when one does not hold the batch, and as
+// many stretches as fill the SMs once.
+struct PrefixPlan {
+    int seqs, mblocks, splits, per, parts;
+    bool pair;
+};
+
+PrefixPlan plan_prefix(int B, int Hkv, int n_rep, int prefix, int num_sms) {
+    PrefixPlan p;
+    p.seqs = kBM / n_rep;
+    const int q_tiles = (B + p.seqs - 1) / p.seqs;
+    p.pair = q_tiles > 1;
+    p.mblocks = p.pair ? (q_tiles + 1) / 2 : 1;
+    const int n_tiles = (prefix + kBN - 1) / kBN;
+    const int most = std::max(1, num_sms / (Hkv * p.mblocks));
+    p.per = (n_tiles + most - 1) / most;
+    p.splits = p.per ? (n_tiles + p.per - 1) / p.per : 0;
+    p.parts = p.pair ? p.splits : 2 * p.splits;
+    return p;
+}
+
+constexpr int kMaxSms = 160;
+
+size_t shared_part_rows(int B, int H, int Hkv, int prefix) {
+    // parts of the prefix for the most SMs a GPU may have: more SMs never give fewer parts
+    const int n_rep = H / Hkv;
+    size_t parts = 0;
+    if (prefix > 0) {
+        const PrefixPlan p = plan_prefix(B, Hkv, n_rep, prefix, kMaxSms);
+        const int most = std::max(1, kMaxSms / (Hkv * p.mblocks));
+        parts = (size_t)(p.pair ? 1 : 2) * std::min(most, (prefix + kBN - 1) / kBN);
+    }
+    return (stream_part_rows(B, Hkv, true) + parts * Hkv * B) * n_rep;
+}
+
+template <int D, bool kPair>
+int launch_prefix_d(const PrefixArgs& a, const PrefixPlan& p, const CUtensorMap& tmQ, const CUtensorMap& tmK,
+                    const CUtensorMap& tmV, const CUtensorMap& tmVend, cudaStream_t s) {
+    auto kern = prefix_kernel<D, kPair>;
+    // setmaxnreg is only safe if the compiled kernel launches with the registers the split was sized for
+    static int regs_ok = -1;
+    if (regs_ok < 0) {
+        cudaFuncAttributes attr;
+        if (int st = check_cuda(cudaFuncGetAttributes(&attr, (const void*)kern), "prefix_kernel attributes")) return st;
+        regs_ok = (uint32_t)attr.numRegs >= kLaunchRegs ? MLLM_OK : MLLM_ERR_UNSUPPORTED;
+    }
+    if (regs_ok != MLLM_OK) return fail(regs_ok, "prefix_kernel: compiled with fewer registers than its split needs");
+    const int smem = PrefixCfg<D, kPair>::kSmemBytes;
+    if (int st = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
+                            "prefix_kernel smem attribute"))
+        return st;
+    return check_cuda(launch_pdl(kern, dim3(a.Hkv * p.mblocks, p.splits), dim3(kThreads), smem, s, tmQ, tmK, tmV, tmVend, a),
+                      "prefix_kernel launch");
+}
+
+}  // namespace
+
+MLLM_DEFINE_STATUS_READER(shared_prefix)
+
+}  // namespace mllm_b200
+
+using namespace mllm_b200;
+
+extern "C" size_t mllm_decode_attention_shared_workspace_size(int batch, int num_heads, int num_kv_heads, int head_dim,
+                                                              int prefix_len) {
+    if (batch <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads || head_dim <= 0 ||
+        prefix_len < 0 || num_heads / num_kv_heads > kMaxGroup)
+        return 0;
+    return (shared_part_rows(batch, num_heads, num_kv_heads, prefix_len) * (size_t)(head_dim + 1) * 4 + 255) & ~size_t(255);
+}
+
+extern "C" int mllm_decode_attention_shared_paged_bf16(const void* q, const mllm_paged_kv* kv, const int32_t* kv_lens,
+                                                       int prefix_len, int batch, int num_heads, int num_kv_heads,
+                                                       int head_dim, int max_kv_len, float softmax_scale, void* out,
+                                                       void* workspace, size_t workspace_bytes, mllm_stream_t stream) {
+    MLLM_NVTX_RANGE("mllm_decode_attention_shared_paged_bf16");
+    if (batch < 0 || num_heads <= 0 || num_kv_heads <= 0 || max_kv_len <= 0)
+        return fail(MLLM_ERR_INVALID_ARGUMENT, "decode_attention_shared: bad sizes");
+    if (prefix_len < 0 || prefix_len > max_kv_len)
+        return fail(MLLM_ERR_INVALID_ARGUMENT, "decode_attention_shared: prefix_len must be in [0, max_kv_len]");
+    if (num_heads % num_kv_heads != 0)
+        return fail(MLLM_ERR_INVALID_ARGUMENT, "Attention: num_heads must be divisible by num_kv_heads.");
+    if (head_dim != 64 && head_dim != 128)
+        return fail(MLLM_ERR_UNSUPPORTED, "decode_attention_shared: head_dim must be 64 or 128");
+    const int n_rep = num_heads / num_kv_heads;
+    if (n_rep > kMaxGroup) return fail(MLLM_ERR_UNSUPPORTED, "decode_attention_shared: GQA group larger than 8");
+    if (batch > 65535 || num_kv_heads > 65535)
+        return fail(MLLM_ERR_UNSUPPORTED, "decode_attention_shared: more than 65535 sequences or kv heads");
+    if (!(softmax_scale > 0.f) || !std::isfinite(softmax_scale))
+        return fail(MLLM_ERR_INVALID_ARGUMENT, "decode_attention_shared: softmax_scale must be positive");
+    StreamArgs a = {};
+    if (int st = paged_layout(kv, max_kv_len, head_dim, "decode_attention_shared", &a.lay)) return st;
+    if (batch == 0) return ok();
+    if (!q || !out || !kv_lens) return fail(MLLM_ERR_INVALID_ARGUMENT, "decode_attention_shared: null pointer");
+    if (!aligned(q, 16) || !aligned(out, 4))
+        return fail(MLLM_ERR_INVALID_ARGUMENT, "decode_attention_shared: q/out misaligned");
+    const size_t need = mllm_decode_attention_shared_workspace_size(batch, num_heads, num_kv_heads, head_dim, prefix_len);
+    if (!workspace || !aligned(workspace, 256) || workspace_bytes < need)
+        return fail(MLLM_ERR_WORKSPACE, "decode_attention_shared: workspace missing, misaligned or smaller than "
+                                        "mllm_decode_attention_shared_workspace_size()");
+    int num_sms = 0;
+    if (int st = require_sm100(&num_sms)) return st;
+    num_sms = std::min(num_sms, kMaxSms);
+    const int64_t D = head_dim;
+    a.q = (const __nv_bfloat16*)q;
+    a.kv_lens = kv_lens;
+    a.out = (__nv_bfloat16*)out;
+    a.B = batch;
+    a.H = num_heads;
+    a.Hkv = num_kv_heads;
+    a.n_rep = n_rep;
+    a.max_len = max_kv_len;
+    a.scale_log2 = (float)((double)softmax_scale * 1.4426950408889634);
+    a.first_row = prefix_len;
+    a.part_o = static_cast<float*>(workspace);
+    a.part_lse = a.part_o + shared_part_rows(batch, num_heads, num_kv_heads, prefix_len) * D;
+    a.prefix_base = (int64_t)stream_part_rows(batch, num_kv_heads, true) * n_rep;
+    cudaStream_t s = (cudaStream_t)stream;
+    if (prefix_len > 0) {
+        const PrefixPlan p = plan_prefix(batch, num_kv_heads, n_rep, prefix_len, num_sms);
+        CUtensorMap tmQ, tmK, tmV, tmVend;
+        // Q [B, H, D]: heads as the map's rows, sequences as its third dimension
+        if (int st = encode_kv_map(&tmQ, q, D, num_heads, batch, 1, D, num_heads * D, (int64_t)batch * num_heads * D, 64,
+                                   n_rep, p.seqs))
+            return st;
+        if (int st = encode_kv_map(&tmK, kv->k_pool, D, kv->block_size, num_kv_heads, kv->num_blocks, kv->row_stride,
+                                   kv->head_stride, kv->block_stride, 64, kBN))
+            return st;
+        if (int st = encode_kv_map(&tmV, kv->v_pool, D, kv->block_size, num_kv_heads, kv->num_blocks, kv->row_stride,
+                                   kv->head_stride, kv->block_stride, 64, kBN))
+            return st;
+        const int tail = prefix_len % kv->block_size;   // rows of the prefix in its last block (0: all)
+        if (int st = encode_kv_map(&tmVend, kv->v_pool, D, tail ? tail : kv->block_size, num_kv_heads, kv->num_blocks,
+                                   kv->row_stride, kv->head_stride, kv->block_stride, 64, kBN))
+            return st;
+        PrefixArgs pa = {};
+        pa.part_o = a.part_o + a.prefix_base * D;
+        pa.part_lse = a.part_lse + a.prefix_base;
+        pa.B = batch;
+        pa.Hkv = num_kv_heads;
+        pa.n_rep = n_rep;
+        pa.seqs = p.seqs;
+        pa.prefix = prefix_len;
+        pa.n_tiles = (prefix_len + kBN - 1) / kBN;
+        pa.per = p.per;
+        pa.mblocks = p.mblocks;
+        pa.scale_log2 = a.scale_log2;
+        pa.lay = a.lay;
+        int st;
+        if (head_dim == 128)
+            st = p.pair ? launch_prefix_d<128, true>(pa, p, tmQ, tmK, tmV, tmVend, s)
+                        : launch_prefix_d<128, false>(pa, p, tmQ, tmK, tmV, tmVend, s);
+        else
+            st = p.pair ? launch_prefix_d<64, true>(pa, p, tmQ, tmK, tmV, tmVend, s)
+                        : launch_prefix_d<64, false>(pa, p, tmQ, tmK, tmV, tmVend, s);
+        if (st) return st;
+        a.prefix_parts = p.parts;
+        a.after_prefix = 1;
+    }
+    CUtensorMap tmK, tmV;
+    if (int st = encode_kv_map(&tmK, kv->k_pool, D, kv->block_size, num_kv_heads, kv->num_blocks, kv->row_stride,
+                               kv->head_stride, kv->block_stride, 64, 64))
+        return st;
+    if (int st = encode_kv_map(&tmV, kv->v_pool, D, kv->block_size, num_kv_heads, kv->num_blocks, kv->row_stride,
+                               kv->head_stride, kv->block_stride, 64, 64))
+        return st;
+    if (int st = launch_stream_bf16(a, head_dim, tmK, tmV, num_sms, s)) return st;
+    return ok();
+}

@@ -165,6 +165,7 @@ class PagedKVCache:
         self._blocks = [[] for _ in range(max_seqs)]
         self._host_lengths = [0] * max_seqs
         self._free = list(range(num_blocks - 1, -1, -1))   # pop() hands out block 0 first
+        self._owners = [0] * num_blocks                     # sequences whose table holds the block (fork)
 
     @property
     def capacity(self) -> int:
@@ -189,12 +190,48 @@ class PagedKVCache:
                 raise RuntimeError("PagedKVCache: out of blocks")
             start = len(blocks)
             while len(blocks) < need:
-                blocks.append(self._free.pop())
+                blocks.append(self._take_block())
             self.block_table[seq, start:need] = torch.tensor(blocks[start:need], dtype=torch.int32)
 
+    def _take_block(self) -> int:
+        blk = self._free.pop()
+        self._owners[blk] = 1
+        return blk
+
+    def fork(self, src: int, dst: int, rows: int) -> None:
+        """Give the empty row `dst` the first `rows` rows of sequence `src`: it shares src's full blocks
+        (a block is freed when its last owner is) and gets a copy of the rows in a block that ends
+        inside.  Shared rows must not be written again; appending to either sequence does not."""
+        if src == dst or self._blocks[dst] or self._host_lengths[dst]:
+            raise RuntimeError("PagedKVCache: fork target row is not empty")
+        full, part = divmod(rows, self.block_size)
+        if rows < 0 or len(self._blocks[src]) < full + (part > 0):
+            raise RuntimeError("PagedKVCache: fork of rows the source does not hold")
+        if part and not self._free:
+            raise RuntimeError("PagedKVCache: out of blocks")
+        blocks = self._blocks[src][:full]
+        for blk in blocks:
+            self._owners[blk] += 1
+        if part:
+            blocks.append(self._take_block())
+            self._copy_rows(self._blocks[src][full], blocks[-1], part)
+        self._blocks[dst] = blocks
+        self.block_table[dst, :len(blocks)] = torch.tensor(blocks, dtype=torch.int32)
+        self._host_lengths[dst] = rows
+        self.lengths[dst] = rows
+
+    def _copy_rows(self, src: int, dst: int, rows: int) -> None:
+        for pool in (self.k_pool, self.v_pool):
+            pool[dst, :, :rows] = pool[src, :, :rows]
+
     def release(self, seq: int) -> None:
-        """Return sequence `seq`'s blocks to the pool (zeroed) and reset its length."""
-        blocks = self._blocks[seq]
+        """Return sequence `seq`'s blocks to the pool (zeroed), those that no other sequence shares, and
+        reset its length."""
+        blocks = []
+        for blk in self._blocks[seq]:
+            self._owners[blk] -= 1
+            if self._owners[blk] == 0:
+                blocks.append(blk)
         if blocks:
             idx = torch.tensor(blocks, dtype=torch.long, device=self.k_pool.device)
             self._zero_blocks(idx)
@@ -301,6 +338,9 @@ class PagedSlot(PagedKVCache):
     def release(self, seq: int = 0) -> None:
         self._parent.release(self._row(seq))
 
+    def fork(self, src: int, dst: int, rows: int) -> None:
+        self._parent.fork(self._row(src), self._row(dst), rows)
+
     def move(self, src: int, dst: int) -> None:
         raise RuntimeError("PagedSlot: move rows on the parent cache")
 
@@ -345,6 +385,10 @@ class PagedKVCache8(PagedKVCache):
     def _zero_blocks(self, idx: torch.Tensor) -> None:
         for t in (self.k_pool.view(torch.uint8), self.v_pool.view(torch.uint8), self.k_exp, self.v_exp):
             t.index_fill_(0, idx, 0)
+
+    def _copy_rows(self, src: int, dst: int, rows: int) -> None:
+        for t in (self.k_pool.view(torch.uint8), self.v_pool.view(torch.uint8), self.k_exp, self.v_exp):
+            t[dst, :, :rows] = t[src, :, :rows]
 
     def slot(self, seq: int, count: int = 1) -> "PagedSlot8":
         return PagedSlot8(self, seq, count)
@@ -820,6 +864,36 @@ def decode_attention(q: torch.Tensor, kv_cache: KVCache, num_kv_heads: int,
     abi.call("mllm_decode_attention_bf16", _ptr(qq), _ptr(kv_cache.key_buf), _ptr(kv_cache.value_buf),
              csb, csh, cst, _ptr(kv_cache.lengths), B, H, num_kv_heads, D, L, 1.0 / math.sqrt(D),
              _ptr(out), _ptr(ws), ws.numel(), abi.stream_handle())
+    return out
+
+
+def decode_attention_shared(q: torch.Tensor, kv_cache: PagedKVCache, num_kv_heads: int, prefix_len: int,
+                            max_kv_len: int | None = None) -> torch.Tensor:
+    """decode_attention over a paged cache whose sequences 0 .. B-1 all begin with the same prefix_len
+    rows (PagedKVCache.fork): the prefix is read once, through row 0 of the block table, for the
+    whole batch, every sequence's further rows through its own -> [B, 1, H*D].  Lengths come from the
+    cache (each at least prefix_len, or 0)."""
+    _check_cuda_bf16("q", q)
+    if not isinstance(kv_cache, PagedKVCache) or isinstance(kv_cache, PagedKVCache8):
+        raise RuntimeError("decode_attention_shared: needs a bf16 PagedKVCache")
+    B, H, D = q.shape[0], q.shape[1], q.shape[-1]
+    qq = q.reshape(B, H, D)
+    if not qq.is_contiguous() or qq.data_ptr() % 16:
+        qq = qq.clone(memory_format=torch.contiguous_format)
+    if q.device != kv_cache.k_pool.device:
+        raise RuntimeError("Attention: q and the cache must be on one device")
+    if kv_cache.k_pool.shape[1] != num_kv_heads or kv_cache.k_pool.shape[3] != D or B > kv_cache.block_table.shape[0]:
+        raise RuntimeError("Attention: the cache has other kv heads, another head_dim or fewer sequences")
+    L = max_kv_len or max(kv_cache.host_lengths()[:B], default=0)
+    L = max(min(L, kv_cache.capacity), 1)
+    out = torch.empty((B, 1, H * D), dtype=BF16, device=q.device)
+    # a workspace of the call's own, from torch's stream-ordered allocator (a captured graph's from its pool)
+    nbytes = abi.load().mllm_decode_attention_shared_workspace_size(B, H, num_kv_heads, D, prefix_len)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    with _on_device(q):
+        abi.call("mllm_decode_attention_shared_paged_bf16", _ptr(qq), C.byref(kv_cache.descriptor()),
+                 _ptr(kv_cache.lengths), prefix_len, B, H, num_kv_heads, D, L, 1.0 / math.sqrt(D), _ptr(out), _ptr(ws),
+                 nbytes, abi.stream_handle())
     return out
 
 

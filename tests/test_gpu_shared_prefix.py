@@ -1,0 +1,165 @@
+"""Decode attention for a batch that shares a prefix, against 64-bit attention over each sequence's rows.  Needs a
+B200.
+
+Tolerance (from the formats): the output is rounded to bf16 (2^-8 of the value at most), P to bf16 (2^-8 of each
+weight, so 2^-8 of the weighted mean of |v|), fp32 score sums 2^-18 of sum |q k|, twice, as weight error."""
+import math
+import random
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+
+@pytest.fixture(scope="module")
+def rt(cuda_device):
+    from mllm_b200 import build
+    build.build()
+    from mllm_b200 import runtime
+    return runtime
+
+
+def _status_ok():
+    from mllm_b200 import abi
+    abi.call("mllm_attn_device_status", None)
+
+
+def _shared_cache(rt, prefix, suffix, Hkv, D, block, seed):
+    """A cache of len(suffix) sequences forked from one prefix, rows random, finite numbers behind the ends."""
+    B = len(suffix)
+    lens = [prefix + s for s in suffix]
+    per = -(-(prefix + max(suffix)) // block)
+    c = rt.PagedKVCache(num_blocks=per * B + 3, num_kv_heads=Hkv, head_dim=D, block_size=block, max_seqs=B,
+                        max_blocks_per_seq=per + 1)
+    random.Random(seed).shuffle(c._free)
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    c.k_pool.normal_(generator=g)
+    c.v_pool.normal_(generator=g)
+    c.reserve(0, prefix)
+    for b in range(1, B):
+        c.fork(0, b, prefix)
+    c.set_lengths(lens)
+    return c, lens
+
+
+def _check(c, q, got, lens, Hkv):
+    B, H, D = q.shape
+    for b, L in enumerate(lens):
+        o = got[b, 0].view(Hkv, H // Hkv, D).double()
+        if L == 0:
+            assert (o == 0).all()
+            continue
+        k, v = (x.double() for x in c.gather(b, L))
+        qq = q[b].view(Hkv, H // Hkv, D).double()
+        s = torch.einsum("grd,gtd->grt", qq, k) / math.sqrt(D)
+        w = torch.softmax(s, -1)
+        ref = torch.einsum("grt,gtd->grd", w, v)
+        mean_abs = torch.einsum("grt,gtd->grd", w, v.abs())
+        ds = 2.0 ** -18 * torch.einsum("grd,gtd->grt", qq.abs(), k.abs()).amax(-1, keepdim=True) / math.sqrt(D)
+        tol = 2.0 ** -8 * ref.abs() + (2.0 ** -8 + 2 * ds + 2.0 ** -18) * mean_abs
+        assert ((o - ref).abs() <= tol).all(), (b, L, ((o - ref).abs() / tol).max())
+
+
+CASES = [
+    # H, Hkv, D, prefix, rows behind it, block, factor on q
+    (8, 2, 128, 1, [1], 128, 1.0),
+    (32, 8, 128, 127, [1, 2, 3], 128, 1.5),
+    (32, 8, 128, 128, [0, 5, 64, 65], 128, 1.5),
+    (32, 8, 128, 129, [0, 0], 256, 1.5),
+    (32, 4, 64, 512, [1, 64, 17, 128, 0, 33, 2, 90], 128, 1.0),
+    (32, 8, 128, 2000, [s % 200 for s in range(32)], 256, 1.5),        # one tile of query rows, full
+    (32, 8, 128, 2000, [s % 7 for s in range(33)], 384, 1.5),          # a second tile with one sequence
+    (40, 8, 128, 5000, [s * 3 for s in range(64)], 256, 1.0),          # groups of 5: three tiles, the pair not full
+    (10, 2, 128, 700, [300] * 130, 128, 2.0),                          # two blocks of query rows
+    (4, 4, 64, 300, [s % 3 for s in range(300)], 128, 1.0),            # groups of one
+    (7, 1, 64, 40000, [9, 1], 128, 1.0),                               # many stretches
+    (8, 1, 128, 1000, [1] * 40, 128, 300.0),                           # one weight close to 1
+]
+
+
+@pytest.mark.parametrize("H,Hkv,D,prefix,suffix,block,qf", CASES)
+def test_against_64_bit_attention(rt, H, Hkv, D, prefix, suffix, block, qf):
+    c, lens = _shared_cache(rt, prefix, suffix, Hkv, D, block, seed=3)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    q = (qf * torch.randn(len(lens), H, D, device="cuda", generator=g)).bfloat16()
+    got = rt.decode_attention_shared(q, c, Hkv, prefix)
+    _status_ok()
+    _check(c, q, got, lens, Hkv)
+    assert torch.equal(got, rt.decode_attention_shared(q, c, Hkv, prefix, max_kv_len=c.capacity))
+
+
+def test_any_part_of_the_common_rows_gives_the_same_answer(rt):
+    """The prefix length is the caller's choice: 0 .. all rows in common, inside tiles and blocks."""
+    c, lens = _shared_cache(rt, 600, [1, 50, 200], 2, 128, 256, seed=7)
+    q = torch.randn(3, 8, 128, device="cuda").bfloat16()
+    for prefix in (0, 1, 63, 64, 65, 255, 256, 257, 511, 600):
+        got = rt.decode_attention_shared(q, c, 2, prefix)
+        _status_ok()
+        _check(c, q, got, lens, 2)
+
+
+def test_rows_behind_the_prefix_do_not_reach_other_sequences(rt):
+    """What lies behind the prefix in its last block, and behind each sequence's end, may be anything."""
+    c, lens = _shared_cache(rt, 200, [0, 30, 5], 2, 64, 128, seed=9)
+    q = torch.randn(3, 8, 64, device="cuda").bfloat16()
+    want = rt.decode_attention_shared(q, c, 2, 200)
+    for b, L in enumerate(lens):
+        blk = c.blocks_of(b)[L // 128]
+        c.k_pool[blk, :, L % 128:] = float("nan")
+        c.v_pool[blk, :, L % 128:] = float("inf")
+    got = rt.decode_attention_shared(q, c, 2, 200)
+    _status_ok()
+    assert torch.equal(want, got)
+
+
+def test_captured_and_replayed_with_other_lengths(rt):
+    c, lens = _shared_cache(rt, 300, [1, 100, 40], 2, 128, 128, seed=4)
+    for b in range(3):
+        c.reserve(b, 500)
+    q = torch.randn(3, 8, 128, device="cuda").bfloat16()
+    graphs = []
+    for _ in range(2):          # two graphs, replayed in turn, do not share their workspaces
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = rt.decode_attention_shared(q, c, 2, 300, max_kv_len=500)
+        graphs.append((graph, out))
+    for step in range(3):
+        c.set_lengths([300 + 10 * step, 350 + step, 301])
+        want = rt.decode_attention_shared(q, c, 2, 300)
+        for graph, out in graphs:
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
+    _status_ok()
+
+
+def test_lengths_shorter_than_the_prefix(rt):
+    from mllm_b200 import abi
+    c, lens = _shared_cache(rt, 300, [10, 20, 30], 2, 128, 128, seed=4)
+    q = torch.randn(3, 8, 128, device="cuda").bfloat16()
+    c.lengths[1] = 0            # an empty row of a padded batch: zeros, no error
+    got = rt.decode_attention_shared(q, c, 2, 300)
+    _status_ok()
+    _check(c, q, got, [310, 0, 330], 2)
+    for bad in (299, -4, 331):
+        c.lengths[1] = bad
+        rt.decode_attention_shared(q, c, 2, 300)
+        with pytest.raises(abi.MllmError) as e:
+            _status_ok()
+        assert e.value.status == 7
+
+
+def test_refusals(rt):
+    c, lens = _shared_cache(rt, 100, [1, 2], 2, 128, 128, seed=4)
+    q = torch.randn(2, 8, 128, device="cuda").bfloat16()
+    for bad in (-1, 103):
+        with pytest.raises(RuntimeError, match="prefix_len|workspace"):
+            rt.decode_attention_shared(q, c, 2, bad)
+    with pytest.raises(RuntimeError, match="kv heads"):
+        rt.decode_attention_shared(q, c, 4, 100)
+    with pytest.raises(RuntimeError, match="bf16"):
+        rt.decode_attention_shared(q, rt.PagedKVCache8(2, 2, 128, 128, 2), 2, 0)
+    with pytest.raises(RuntimeError, match="bfloat16"):
+        rt.decode_attention_shared(q.float(), c, 2, 100)
