@@ -14,6 +14,7 @@
  *                               lengths (several prompts in one launch each)
  *   mllm_decode_attention_shared_paged_bf16  decode for a batch that shares a prefix
  *   mllm_*_kv8                  epilogue, read-back and decode over an 8-bit paged KV cache
+ *   mllm_logit_rules            penalties, biases and a mask of allowed tokens, per row
  *   mllm_sample                 Sampler::Sample on the device (penalty, greedy / top-k / top-p)
  *
  * plus the RoPE table builder and RoPE apply that back the `mllm::RoPE` facade.
@@ -490,6 +491,35 @@ MLLM_API int mllm_sample(void* logits, int logits_bf16, int64_t row_stride, int 
                          float temperature, int top_k, float top_p, int use_greedy, float repetition_penalty,
                          uint64_t seed, uint64_t offset, int64_t* out_tokens, void* workspace,
                          size_t workspace_bytes, mllm_stream_t stream);
+
+/* ----------------------------------------------------------------------------------------
+ * Rules on logits, before mllm_sample (whose one penalty, the reference's, is the same for the
+ * whole batch).  Every row has its own; every rule may be NULL.  For a token v of a row:
+ *   seen = v occurs in the row's history, c = how often from position output_start[row] on
+ *   x = logit;  if seen: x = x < 0 ? x * repetition : x / repetition  (once, however often seen)
+ *   x -= c * frequency;  if c > 0: x -= presence;  x += the sum of v's biases, in list order
+ *   out = v allowed ? x : -inf               in fp32, rounded once to the logits' dtype
+ * A token that no rule touches keeps its bits; a forbidden one is -inf whatever its logit (NaN
+ * too); a row that allows nothing is all -inf.
+ *   logits / out: bf16 (logits_bf16 != 0) or fp32, row b at + b*row_stride / b*out_stride; out may
+ *       be the same memory as logits (with the same stride), else the two must not overlap.
+ *   history: int64 device, row b's history_lens[b] <= history_cols tokens at
+ *       history + b*history_stride; output_start: int32 device [batch] (NULL: 0) -- the tokens
+ *       before it are the prompt's, which only the repetition penalty counts.
+ *   repetition, presence, frequency: fp32 device [batch] (NULL: 1, 0, 0).
+ *   bias_ids / bias_values: int64 / fp32 device, row b's bias_lens[b] <= bias_cols <= 1024 pairs at
+ *       + b*bias_stride; a token listed more than once gets every one.
+ *   allowed: 32-bit words, bit v % 32 of word v / 32 of row b at allowed + b*allowed_stride says
+ *       whether token v may be picked (a grammar's mask); NULL: all may.
+ *   Ids outside the vocabulary are ignored.  A list length below 0 or above its columns records
+ *   MLLM_ERR_DEVICE_LENGTH and is cut to them. */
+MLLM_API int mllm_logit_rules(const void* logits, int logits_bf16, int64_t row_stride, int batch, int vocab,
+                              const int64_t* history, int64_t history_stride, int history_cols,
+                              const int32_t* history_lens, const int32_t* output_start, const float* repetition,
+                              const float* presence, const float* frequency, const int64_t* bias_ids,
+                              const float* bias_values, int64_t bias_stride, int bias_cols, const int32_t* bias_lens,
+                              const uint32_t* allowed, int64_t allowed_stride, void* out, int64_t out_stride,
+                              mllm_stream_t stream);
 
 /* ----------------------------------------------------------------------------------------
  * Projections for decode-sized token counts.  Replaces Linear::Forward (Linear.h:33-68,

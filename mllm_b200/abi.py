@@ -121,6 +121,8 @@ SIGNATURES = {
     "mllm_comm_in_flight": (_i, [_p]),
     "mllm_comm_abort": (_i, [_p]),
     "mllm_comm_destroy": (_i, [_p]),
+    "mllm_logit_rules": (_i, [_p, _i, _i64, _i, _i, _p, _i64, _i, _p, _p, _p, _p, _p, _p, _p, _i64, _i, _p, _p, _i64, _p,
+                              _i64, _p]),
     "mllm_sample_workspace_size": (_sz, [_i, _i]),
     "mllm_sample": (_i, [_p, _i, _i64, _i, _i, _p, _i64, _p, _f, _i, _f, _i, _f, C.c_uint64, C.c_uint64, _p, _p,
                          _sz, _p]),

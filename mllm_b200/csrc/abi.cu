@@ -174,12 +174,13 @@ extern "C" const char* mllm_attn_last_error(void) { return t_last_error.c_str();
 
 extern "C" int mllm_attn_device_status(mllm_stream_t stream) {
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    constexpr int kReaders = 8;
+    constexpr int kReaders = 9;
     unsigned v[kReaders] = {};
     int (*readers[kReaders])(cudaStream_t, unsigned*) = {read_clear_status_decode, read_clear_status_prefill,
                                                          read_clear_status_epilogue, read_clear_status_peer,
                                                          read_clear_status_linear, read_clear_status_kv8_rows,
-                                                         read_clear_status_decode_stream, read_clear_status_shared_prefix};
+                                                         read_clear_status_decode_stream, read_clear_status_shared_prefix,
+                                                         read_clear_status_logit_rules};
     for (int i = 0; i < kReaders; ++i) {
         const int e = readers[i](s, &v[i]);
         if (e != 0) return check_cuda((cudaError_t)e, "read device status");

@@ -63,6 +63,7 @@ int read_clear_status_linear(cudaStream_t s, unsigned* out);
 int read_clear_status_kv8_rows(cudaStream_t s, unsigned* out);
 int read_clear_status_decode_stream(cudaStream_t s, unsigned* out);
 int read_clear_status_shared_prefix(cudaStream_t s, unsigned* out);
+int read_clear_status_logit_rules(cudaStream_t s, unsigned* out);
 
 // Encodes a 4-D bf16 tensor map {d (inner), rows, heads, batch} with 128-byte swizzle and a
 // {box_d, box_rows, box_heads, 1} box.  Strides are in elements and need not be ordered (a

@@ -980,6 +980,88 @@ def decode_step(q, k, v, kv_cache: KVCache, positions: torch.Tensor, rope_theta:
     return out
 
 
+def _check_rows(name: str, t: torch.Tensor, B: int, dtype, device) -> None:
+    """A [B, n] device tensor whose rows are contiguous."""
+    if t.device != device or t.dtype != dtype or t.dim() != 2 or t.shape[0] != B or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise RuntimeError(f"{name}: expected a {dtype} [{B}, n] tensor with contiguous rows on {device}")
+
+
+def _rows_stride(t: torch.Tensor) -> int:
+    return max(t.stride(0), t.shape[1])     # the stride of a single row means nothing
+
+
+def _own_rows(t: torch.Tensor) -> torch.Tensor:
+    """The tensor, or a copy where its rows overlap (an expanded one)."""
+    return t if t.shape[0] < 2 or t.stride(0) >= t.shape[1] else t.contiguous()
+
+
+def apply_logit_rules(logits: torch.Tensor, history=None, history_lens=None, output_start=None, repetition=None,
+                      presence=None, frequency=None, bias_ids=None, bias_values=None, bias_lens=None, allowed=None,
+                      out: torch.Tensor | None = None) -> torch.Tensor:
+    """Penalties, biases and a mask of allowed tokens on logits [B, V] bf16 or fp32 (mllm_logit_rules),
+    each row with its own, before `sample`:
+      history int64 [B, n] with history_lens int32 [B]: the row's tokens, prompt first; those from
+        output_start int32 [B] (default 0) on are generated ones
+      repetition, presence, frequency fp32 [B]: a seen token's logit is divided by the first (multiplied
+        where negative), a generated token's lowered by the second, and by the third for each time
+      bias_ids int64 / bias_values fp32 [B, n <= 1024] with bias_lens int32 [B]: added to tokens
+      allowed int32 [B, ceil(V / 32)]: bit v % 32 of word v // 32 allows token v; others become -inf
+    All on the device.  Returns `out` (a new tensor by default; `logits` itself works in place)."""
+    if not logits.is_cuda:
+        raise RuntimeError("logit rules: logits must be a CUDA tensor (no CPU fallback)")
+    if logits.dtype not in (BF16, torch.float32):
+        raise RuntimeError("logit rules: logits must be bf16 or fp32")
+    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise RuntimeError("logit rules: logits must be [B, V] with contiguous rows")
+    B, V = logits.shape
+    dev = logits.device
+    if (history is None) != (history_lens is None):
+        raise RuntimeError("logit rules: give both history and history_lens or neither")
+    if history is not None:
+        _check_rows("history", history, B, torch.int64, dev)
+        _check_int("history_lens", history_lens, B, torch.int32, dev)
+    for name, t, dt in (("output_start", output_start, torch.int32), ("repetition", repetition, torch.float32),
+                        ("presence", presence, torch.float32), ("frequency", frequency, torch.float32)):
+        if t is not None:
+            if history is None:
+                raise RuntimeError("logit rules: penalties need a history")
+            _check_int(name, t, B, dt, dev)
+    if len({bias_ids is None, bias_values is None, bias_lens is None}) != 1:
+        raise RuntimeError("logit rules: give all of bias_ids, bias_values and bias_lens or none")
+    if bias_ids is not None:
+        _check_rows("bias_ids", bias_ids, B, torch.int64, dev)
+        _check_rows("bias_values", bias_values, B, torch.float32, dev)
+        _check_int("bias_lens", bias_lens, B, torch.int32, dev)
+        if bias_values.shape != bias_ids.shape or (B > 1 and bias_values.stride(0) != bias_ids.stride(0)):
+            raise RuntimeError("logit rules: bias_ids and bias_values must have the same layout")
+    if allowed is not None:
+        _check_rows("allowed", allowed, B, torch.int32, dev)
+        if allowed.shape[1] < (V + 31) // 32:
+            raise RuntimeError("logit rules: allowed needs ceil(V / 32) words a row")
+    if history is not None and history.shape[1] == 0:
+        history = history_lens = output_start = repetition = presence = frequency = None
+    if bias_ids is not None and bias_ids.shape[1] == 0:
+        bias_ids = bias_values = bias_lens = None
+    if out is not None and out.shape[0] > 1 and out.stride(0) < V:
+        raise RuntimeError("logit rules: out's rows overlap")
+    logits, history, bias_ids, bias_values, allowed = (
+        t if t is None else _own_rows(t) for t in (logits, history, bias_ids, bias_values, allowed))
+    if out is None:
+        out = torch.empty((B, V), dtype=logits.dtype, device=dev)
+    elif out.shape != logits.shape or out.dtype != logits.dtype or out.device != dev or (V > 1 and out.stride(1) != 1):
+        raise RuntimeError("logit rules: out must be like logits")
+    if B == 0 or V == 0:
+        return out
+    with _on_device(logits):
+        abi.call("mllm_logit_rules", _ptr(logits), int(logits.dtype == BF16), _rows_stride(logits), B, V, _ptr(history),
+                 _rows_stride(history) if history is not None else 0, history.shape[1] if history is not None else 0,
+                 _ptr(history_lens), _ptr(output_start), _ptr(repetition), _ptr(presence), _ptr(frequency),
+                 _ptr(bias_ids), _ptr(bias_values), _rows_stride(bias_ids) if bias_ids is not None else 0,
+                 bias_ids.shape[1] if bias_ids is not None else 0, _ptr(bias_lens), _ptr(allowed),
+                 _rows_stride(allowed) if allowed is not None else 0, _ptr(out), _rows_stride(out), abi.stream_handle())
+    return out
+
+
 _SAMPLE_WS = DecodeWorkspace()
 
 
