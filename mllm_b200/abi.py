@@ -177,6 +177,8 @@ def call(name: str, *args) -> int:
 
 def stream_handle(stream=None) -> int | None:
     """cudaStream_t of a torch stream (None -> torch's current stream)."""
+    if stream is not None:
+        return stream.cuda_stream or None
     import torch
-    s = stream if stream is not None else torch.cuda.current_stream()
-    return s.cuda_stream or None
+    # the raw handle: torch.cuda.current_stream() builds a Stream object, 3 us a call
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()) or None

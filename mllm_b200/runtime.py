@@ -191,7 +191,10 @@ class PagedKVCache:
             start = len(blocks)
             while len(blocks) < need:
                 blocks.append(self._take_block())
-            self.block_table[seq, start:need] = torch.tensor(blocks[start:need], dtype=torch.int32)
+            if need - start == 1:   # a growing sequence's next block: a fill, with no copy from the host to wait for
+                self.block_table[seq, start] = blocks[start]
+            else:
+                self.block_table[seq, start:need] = torch.tensor(blocks[start:need], dtype=torch.int32)
 
     def _take_block(self) -> int:
         blk = self._free.pop()
@@ -488,30 +491,20 @@ def _capturing() -> bool:
     return True
 
 
-def _check_int(name: str, t: torch.Tensor, n: int, dtype, device) -> None:
-    """A contiguous device vector of exactly n whole numbers."""
-    if t.device != device or t.dtype != dtype or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
-        raise RuntimeError(f"{name}: expected a contiguous {dtype} tensor of {n} elements on {device}")
+def _check_vec(name: str, t: torch.Tensor, n: int, dtype, dev: int) -> None:
+    """A contiguous vector of exactly n elements on CUDA device number `dev`."""
+    if t.get_device() != dev or t.dtype is not dtype or t.dim() != 1 or t.size(0) != n or not t.is_contiguous():
+        raise RuntimeError(f"{name}: expected a contiguous {dtype} tensor of {n} elements on cuda:{dev}")
 
 
-class _on_device:
-    """Makes a tensor's device the current one around a call, if it is not already: the library
-    launches on the current device, in torch's current stream of it."""
-
-    def __init__(self, t: torch.Tensor):
-        self.idx = t.device.index
-        self.prev = None
-
-    def __enter__(self):
-        cur = torch.cuda.current_device()
-        if cur != self.idx:
-            self.prev = cur
-            torch.cuda.set_device(self.idx)
-
-    def __exit__(self, *exc):
-        if self.prev is not None:
-            torch.cuda.set_device(self.prev)
-        return False
+def _launch(dev: int, name: str, *args) -> None:
+    """abi.call with torch's current stream of device number `dev` as the last argument; the library launches on
+    the current device, so `dev` is made that around the call if it is not."""
+    if dev == torch.cuda.current_device():
+        abi.call(name, *args, abi.stream_handle())
+    else:
+        with torch.cuda.device(dev):
+            abi.call(name, *args, abi.stream_handle())
 
 
 def qkv_epilogue_kv8(q, k, v, kv_cache: PagedKVCache8, cu_seqlens: torch.Tensor, start: torch.Tensor, positions=None,
@@ -531,47 +524,52 @@ def qkv_epilogue_kv8(q, k, v, kv_cache: PagedKVCache8, cu_seqlens: torch.Tensor,
             raise RuntimeError(f"Attention: {n} must be rank-3 [T, h, D] with D contiguous")
     if not isinstance(kv_cache, PagedKVCache8):
         raise RuntimeError("qkv_epilogue_kv8: needs a PagedKVCache8")
-    T, H, D = q.shape
-    Hkv = k.shape[1]
-    if k.shape != (T, Hkv, D) or v.shape != k.shape:
+    T, H, D = shape = q.shape
+    dev = q.get_device()
+    pool = kv_cache.k_pool
+    if k.shape != v.shape or k.size(0) != T or k.size(2) != D:
         raise RuntimeError("Attention: k and v must be [T, num_kv_heads, D] for q's T and D")
-    if kv_cache.k_pool.shape[1] != Hkv or kv_cache.k_pool.shape[3] != D:
+    Hkv = k.size(1)
+    if pool.size(1) != Hkv or pool.size(3) != D:
         raise RuntimeError("Attention: the cache has other kv heads or another head_dim")
-    dev = q.device
-    if k.device != dev or v.device != dev or kv_cache.k_pool.device != dev:
+    if k.get_device() != dev or v.get_device() != dev or pool.get_device() != dev:
         raise RuntimeError("Attention: q, k, v and the cache must be on one device")
     n = start.numel()
-    if n > kv_cache.block_table.shape[0]:
+    if n > kv_cache.block_table.size(0):
         raise RuntimeError("Attention: more sequences than the cache has rows for")
-    _check_int("cu_seqlens", cu_seqlens, n + 1, torch.int32, dev)
-    _check_int("start", start, n, torch.int32, dev)
-    cos = sin = None
+    _check_vec("cu_seqlens", cu_seqlens, n + 1, torch.int32, dev)
+    _check_vec("start", start, n, torch.int32, dev)
+    pos = cos = sin = None
     if rope_table is not None:
         cos, sin = rope_table
         for t in (cos, sin):
-            if t.device != dev or t.dtype != torch.float32 or t.shape != (T, D) or not t.is_contiguous():
+            if t.get_device() != dev or t.dtype is not torch.float32 or t.shape != (T, D) or not t.is_contiguous():
                 raise RuntimeError("RoPE: tables must be contiguous fp32 [T, D] on q's device")
+        cos, sin = cos.data_ptr(), sin.data_ptr()
     else:
         if positions is None:
             raise RuntimeError("RoPE: positions or rope_table required")
-        _check_int("positions", positions, T, torch.int64, dev)
+        _check_vec("positions", positions, T, torch.int64, dev)
+        pos = positions.data_ptr()
     if (q_norm_weight is None) != (k_norm_weight is None):
         raise RuntimeError("Attention: give both q/k norm weights or neither")
     qn = kn = None
     if q_norm_weight is not None:
-        qn, kn = (w if w.dtype == BF16 and w.is_contiguous() else w.to(BF16).contiguous()
+        qn, kn = (w if w.dtype is BF16 and w.is_contiguous() else w.to(BF16).contiguous()
                   for w in (q_norm_weight, k_norm_weight))
-        if qn.shape != (D,) or kn.shape != (D,) or qn.device != dev or kn.device != dev:
-            raise RuntimeError("Attention: norm weights must be [D] on q's device")
+        _check_vec("q_norm_weight", qn, D, BF16, dev)
+        _check_vec("k_norm_weight", kn, D, BF16, dev)
     if out is None:
-        out = torch.empty((T, H, D), dtype=BF16, device=dev)
-    elif out.shape != q.shape or out.dtype != BF16 or out.device != dev or out.stride(2) != 1:
+        out = torch.empty(shape, dtype=BF16, device=q.device)
+    elif out.shape != shape or out.dtype is not BF16 or out.get_device() != dev or out.stride(2) != 1:
         raise RuntimeError("Attention: out must be bf16 [T, H, D] with D contiguous on q's device")
-    with _on_device(q):
-        abi.call("mllm_qkv_epilogue_varlen_paged_kv8", _ptr(q), q.stride(0), q.stride(1), _ptr(k), k.stride(0),
-                 k.stride(1), _ptr(v), v.stride(0), v.stride(1), T, H, Hkv, D, None if cos is not None else _ptr(positions),
-                 float(rope_theta), _ptr(cos), _ptr(sin), _ptr(qn), _ptr(kn), float(eps), _ptr(out), out.stride(0),
-                 out.stride(1), C.byref(kv_cache.descriptor()), _ptr(cu_seqlens), n, _ptr(start), abi.stream_handle())
+    q_st, q_sh, _ = q.stride()
+    k_st, k_sh, _ = k.stride()
+    v_st, v_sh, _ = v.stride()
+    o_st, o_sh, _ = out.stride()
+    _launch(dev, "mllm_qkv_epilogue_varlen_paged_kv8", q.data_ptr(), q_st, q_sh, k.data_ptr(), k_st, k_sh, v.data_ptr(), v_st,
+            v_sh, T, H, Hkv, D, pos, float(rope_theta), cos, sin, _ptr(qn), _ptr(kn), float(eps), out.data_ptr(), o_st, o_sh,
+            C.byref(kv_cache.descriptor()), cu_seqlens.data_ptr(), n, start.data_ptr())
     return out
 
 
@@ -581,36 +579,46 @@ def kv8_read(kv_cache: PagedKVCache8, lens: torch.Tensor, rows: int, first: torc
     sequence are zero."""
     if not isinstance(kv_cache, PagedKVCache8):
         raise RuntimeError("kv8_read: needs a PagedKVCache8")
-    dev = kv_cache.k_pool.device
+    pool = kv_cache.k_pool
+    dev = pool.get_device()
     n = lens.numel()
-    if rows < 0 or n > kv_cache.block_table.shape[0]:
+    if rows < 0 or n > kv_cache.block_table.size(0):
         raise RuntimeError("kv8_read: negative rows, or more sequences than the cache has rows for")
-    _check_int("lens", lens, n, torch.int32, dev)
+    _check_vec("lens", lens, n, torch.int32, dev)
     if first is not None:
-        _check_int("first", first, n, torch.int32, dev)
-    _, Hkv, _, D = kv_cache.k_pool.shape
-    k = torch.empty((n, Hkv, rows, D), dtype=BF16, device=dev)
+        _check_vec("first", first, n, torch.int32, dev)
+    Hkv, D = pool.size(1), pool.size(3)
+    k = torch.empty((n, Hkv, rows, D), dtype=BF16, device=pool.device)
     v = torch.empty_like(k)
-    with _on_device(k):
-        abi.call("mllm_kv8_read_bf16", C.byref(kv_cache.descriptor()), _ptr(first), _ptr(lens), n, Hkv, D, rows, _ptr(k),
-                 _ptr(v), Hkv * rows * D, rows * D, D, abi.stream_handle())
+    _launch(dev, "mllm_kv8_read_bf16", C.byref(kv_cache.descriptor()), _ptr(first), lens.data_ptr(), n, Hkv, D, rows,
+            k.data_ptr(), v.data_ptr(), Hkv * rows * D, rows * D, D)
     return k, v
+
+
+def _check_decode(q: torch.Tensor, kv_cache: PagedKVCache, num_kv_heads: int) -> int:
+    """Checks decode queries [B, H, D] against a paged cache; returns the device number."""
+    pool = kv_cache.k_pool
+    dev = pool.get_device()
+    if q.get_device() != dev:
+        raise RuntimeError("Attention: q and the cache must be on one device")
+    if pool.size(1) != num_kv_heads or pool.size(3) != q.size(2) or q.size(0) > kv_cache.block_table.size(0):
+        raise RuntimeError("Attention: the cache has other kv heads, another head_dim or fewer sequences")
+    return dev
 
 
 def _decode_kv8(q: torch.Tensor, kv_cache: PagedKVCache8, num_kv_heads: int, max_kv_len: int) -> torch.Tensor:
     """decode_attention over an 8-bit cache: q [B, H, D] contiguous."""
     B, H, D = q.shape
-    if q.device != kv_cache.k_pool.device:
-        raise RuntimeError("Attention: q and the cache must be on one device")
-    if kv_cache.k_pool.shape[1] != num_kv_heads or kv_cache.k_pool.shape[3] != D or B > kv_cache.block_table.shape[0]:
-        raise RuntimeError("Attention: the cache has other kv heads, another head_dim or fewer sequences")
-    out = torch.empty((B, 1, H * D), dtype=BF16, device=q.device)
+    dev = _check_decode(q, kv_cache, num_kv_heads)
+    if q.data_ptr() % 8:
+        q = q.clone()
+    device = q.device
+    out = torch.empty((B, 1, H * D), dtype=BF16, device=device)
     # a workspace of the call's own, from torch's stream-ordered allocator (a captured graph's from its pool)
     nbytes = abi.load().mllm_decode_attention_kv8_workspace_size(H, num_kv_heads, D)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-    with _on_device(q):
-        abi.call("mllm_decode_attention_paged_kv8", _ptr(q), C.byref(kv_cache.descriptor()), _ptr(kv_cache.lengths), B, H,
-                 num_kv_heads, D, max_kv_len, 1.0 / math.sqrt(D), _ptr(out), _ptr(ws), nbytes, abi.stream_handle())
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    _launch(dev, "mllm_decode_attention_paged_kv8", q.data_ptr(), C.byref(kv_cache.descriptor()), kv_cache.lengths.data_ptr(),
+            B, H, num_kv_heads, D, max_kv_len, 1.0 / math.sqrt(D), out.data_ptr(), ws.data_ptr(), nbytes)
     return out
 
 
@@ -880,20 +888,16 @@ def decode_attention_shared(q: torch.Tensor, kv_cache: PagedKVCache, num_kv_head
     qq = q.reshape(B, H, D)
     if not qq.is_contiguous() or qq.data_ptr() % 16:
         qq = qq.clone(memory_format=torch.contiguous_format)
-    if q.device != kv_cache.k_pool.device:
-        raise RuntimeError("Attention: q and the cache must be on one device")
-    if kv_cache.k_pool.shape[1] != num_kv_heads or kv_cache.k_pool.shape[3] != D or B > kv_cache.block_table.shape[0]:
-        raise RuntimeError("Attention: the cache has other kv heads, another head_dim or fewer sequences")
+    dev = _check_decode(qq, kv_cache, num_kv_heads)
     L = max_kv_len or max(kv_cache.host_lengths()[:B], default=0)
     L = max(min(L, kv_cache.capacity), 1)
     out = torch.empty((B, 1, H * D), dtype=BF16, device=q.device)
     # a workspace of the call's own, from torch's stream-ordered allocator (a captured graph's from its pool)
     nbytes = abi.load().mllm_decode_attention_shared_workspace_size(B, H, num_kv_heads, D, prefix_len)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-    with _on_device(q):
-        abi.call("mllm_decode_attention_shared_paged_bf16", _ptr(qq), C.byref(kv_cache.descriptor()),
-                 _ptr(kv_cache.lengths), prefix_len, B, H, num_kv_heads, D, L, 1.0 / math.sqrt(D), _ptr(out), _ptr(ws),
-                 nbytes, abi.stream_handle())
+    _launch(dev, "mllm_decode_attention_shared_paged_bf16", qq.data_ptr(), C.byref(kv_cache.descriptor()),
+            kv_cache.lengths.data_ptr(), prefix_len, B, H, num_kv_heads, D, L, 1.0 / math.sqrt(D), out.data_ptr(),
+            ws.data_ptr(), nbytes)
     return out
 
 
@@ -980,19 +984,21 @@ def decode_step(q, k, v, kv_cache: KVCache, positions: torch.Tensor, rope_theta:
     return out
 
 
-def _check_rows(name: str, t: torch.Tensor, B: int, dtype, device) -> None:
-    """A [B, n] device tensor whose rows are contiguous."""
-    if t.device != device or t.dtype != dtype or t.dim() != 2 or t.shape[0] != B or (t.shape[1] > 1 and t.stride(1) != 1):
-        raise RuntimeError(f"{name}: expected a {dtype} [{B}, n] tensor with contiguous rows on {device}")
+def _rows(name: str, t: torch.Tensor, B: int, dtype, dev: int) -> torch.Tensor:
+    """A [B, n] tensor on device number `dev` whose rows are contiguous; a copy of it where the rows overlap (an
+    expanded one)."""
+    if t.get_device() != dev or t.dtype is not dtype or t.dim() != 2 or t.size(0) != B or \
+            (t.size(1) > 1 and t.stride(1) != 1):
+        raise RuntimeError(f"{name}: expected a {dtype} [{B}, n] tensor with contiguous rows on cuda:{dev}")
+    return t if B < 2 or t.stride(0) >= t.size(1) else t.contiguous()
 
 
-def _rows_stride(t: torch.Tensor) -> int:
-    return max(t.stride(0), t.shape[1])     # the stride of a single row means nothing
-
-
-def _own_rows(t: torch.Tensor) -> torch.Tensor:
-    """The tensor, or a copy where its rows overlap (an expanded one)."""
-    return t if t.shape[0] < 2 or t.stride(0) >= t.shape[1] else t.contiguous()
+def _rows_args(t: torch.Tensor | None):
+    """(pointer, row stride, columns); the stride of a single row means nothing."""
+    if t is None:
+        return None, 0, 0
+    n = t.size(1)
+    return t.data_ptr(), max(t.stride(0), n), n
 
 
 def apply_logit_rules(logits: torch.Tensor, history=None, history_lens=None, output_start=None, repetition=None,
@@ -1009,56 +1015,58 @@ def apply_logit_rules(logits: torch.Tensor, history=None, history_lens=None, out
     All on the device.  Returns `out` (a new tensor by default; `logits` itself works in place)."""
     if not logits.is_cuda:
         raise RuntimeError("logit rules: logits must be a CUDA tensor (no CPU fallback)")
-    if logits.dtype not in (BF16, torch.float32):
+    dtype = logits.dtype
+    if dtype is not BF16 and dtype is not torch.float32:
         raise RuntimeError("logit rules: logits must be bf16 or fp32")
-    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
-        raise RuntimeError("logit rules: logits must be [B, V] with contiguous rows")
-    B, V = logits.shape
-    dev = logits.device
+    if logits.dim() != 2:
+        raise RuntimeError("logit rules: logits must be [B, V]")
+    B, V = shape = logits.shape
+    dev = logits.get_device()
+    logits = _rows("logits", logits, B, dtype, dev)
     if (history is None) != (history_lens is None):
         raise RuntimeError("logit rules: give both history and history_lens or neither")
     if history is not None:
-        _check_rows("history", history, B, torch.int64, dev)
-        _check_int("history_lens", history_lens, B, torch.int32, dev)
-    for name, t, dt in (("output_start", output_start, torch.int32), ("repetition", repetition, torch.float32),
-                        ("presence", presence, torch.float32), ("frequency", frequency, torch.float32)):
-        if t is not None:
-            if history is None:
-                raise RuntimeError("logit rules: penalties need a history")
-            _check_int(name, t, B, dt, dev)
-    if len({bias_ids is None, bias_values is None, bias_lens is None}) != 1:
-        raise RuntimeError("logit rules: give all of bias_ids, bias_values and bias_lens or none")
-    if bias_ids is not None:
-        _check_rows("bias_ids", bias_ids, B, torch.int64, dev)
-        _check_rows("bias_values", bias_values, B, torch.float32, dev)
-        _check_int("bias_lens", bias_lens, B, torch.int32, dev)
-        if bias_values.shape != bias_ids.shape or (B > 1 and bias_values.stride(0) != bias_ids.stride(0)):
-            raise RuntimeError("logit rules: bias_ids and bias_values must have the same layout")
+        history = _rows("history", history, B, torch.int64, dev)
+        _check_vec("history_lens", history_lens, B, torch.int32, dev)
+    if output_start is not None:
+        _check_vec("output_start", output_start, B, torch.int32, dev)
+    if repetition is not None:
+        _check_vec("repetition", repetition, B, torch.float32, dev)
+    if presence is not None:
+        _check_vec("presence", presence, B, torch.float32, dev)
+    if frequency is not None:
+        _check_vec("frequency", frequency, B, torch.float32, dev)
+    if bias_ids is not None and bias_values is not None and bias_lens is not None:
+        bias_ids = _rows("bias_ids", bias_ids, B, torch.int64, dev)
+        bias_values = _rows("bias_values", bias_values, B, torch.float32, dev)
+        _check_vec("bias_lens", bias_lens, B, torch.int32, dev)
+        if bias_values.shape != bias_ids.shape:
+            raise RuntimeError("logit rules: bias_ids and bias_values must have the same shape")
+        if B > 1 and bias_values.stride(0) != bias_ids.stride(0):
+            bias_ids, bias_values = bias_ids.contiguous(), bias_values.contiguous()
     if allowed is not None:
-        _check_rows("allowed", allowed, B, torch.int32, dev)
-        if allowed.shape[1] < (V + 31) // 32:
+        allowed = _rows("allowed", allowed, B, torch.int32, dev)
+        if allowed.size(1) < (V + 31) // 32:
             raise RuntimeError("logit rules: allowed needs ceil(V / 32) words a row")
-    if history is not None and history.shape[1] == 0:
+    if history is not None and history.size(1) == 0:
         history = history_lens = output_start = repetition = presence = frequency = None
-    if bias_ids is not None and bias_ids.shape[1] == 0:
+    if bias_ids is not None and bias_ids.size(1) == 0:
         bias_ids = bias_values = bias_lens = None
-    if out is not None and out.shape[0] > 1 and out.stride(0) < V:
-        raise RuntimeError("logit rules: out's rows overlap")
-    logits, history, bias_ids, bias_values, allowed = (
-        t if t is None else _own_rows(t) for t in (logits, history, bias_ids, bias_values, allowed))
     if out is None:
-        out = torch.empty((B, V), dtype=logits.dtype, device=dev)
-    elif out.shape != logits.shape or out.dtype != logits.dtype or out.device != dev or (V > 1 and out.stride(1) != 1):
-        raise RuntimeError("logit rules: out must be like logits")
+        out = torch.empty(shape, dtype=dtype, device=logits.device)
+    elif out.shape != shape or out.dtype is not dtype or out.get_device() != dev or (V > 1 and out.stride(1) != 1) or \
+            (B > 1 and out.stride(0) < V):
+        raise RuntimeError("logit rules: out must be like logits, its rows apart")
     if B == 0 or V == 0:
         return out
-    with _on_device(logits):
-        abi.call("mllm_logit_rules", _ptr(logits), int(logits.dtype == BF16), _rows_stride(logits), B, V, _ptr(history),
-                 _rows_stride(history) if history is not None else 0, history.shape[1] if history is not None else 0,
-                 _ptr(history_lens), _ptr(output_start), _ptr(repetition), _ptr(presence), _ptr(frequency),
-                 _ptr(bias_ids), _ptr(bias_values), _rows_stride(bias_ids) if bias_ids is not None else 0,
-                 bias_ids.shape[1] if bias_ids is not None else 0, _ptr(bias_lens), _ptr(allowed),
-                 _rows_stride(allowed) if allowed is not None else 0, _ptr(out), _rows_stride(out), abi.stream_handle())
+    x, x_stride, _ = _rows_args(logits)
+    hist, hist_stride, hist_cols = _rows_args(history)
+    ids, bias_stride, bias_cols = _rows_args(bias_ids)
+    words, words_stride, _ = _rows_args(allowed)
+    y, y_stride, _ = _rows_args(out)
+    _launch(dev, "mllm_logit_rules", x, int(dtype is BF16), x_stride, B, V, hist, hist_stride, hist_cols, _ptr(history_lens),
+            _ptr(output_start), _ptr(repetition), _ptr(presence), _ptr(frequency), ids, _ptr(bias_values), bias_stride,
+            bias_cols, _ptr(bias_lens), words, words_stride, y, y_stride)
     return out
 
 
