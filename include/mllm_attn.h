@@ -385,8 +385,8 @@ MLLM_API int mllm_prefill_attention_varlen_paged_bf16(const void* q, const mllm_
  *   does).  Arguments as that call's, but:
  *   rope_cos / rope_sin: fp32 [total_tokens, head_dim], one row per token, or both NULL: the angles
  *       are computed from positions (int64 [total_tokens]) and rope_theta.
- *   q_out: token t's head h at q_out + t*q_out_st + h*q_out_sh (multiples of 4 elements), so
- *       that it can be written as [heads, tokens, d] for prefill or [tokens, heads, d] for decode.
+ *   q_out: token t's head h at q_out + t*q_out_st + h*q_out_sh (multiples of 8 elements, 16-byte
+ *       aligned), so that it can be written as [heads, tokens, d] for prefill or [tokens, heads, d] for decode.
  *   cache_start: int32 device [batch], required.
  *   A token outside the ranges cu_seqlens describes is left out: none of its rows is written.  A
  *   cache row past the block table, or a table entry outside the pool, records

@@ -166,6 +166,13 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
     return d;
 }
 
+// max(|a|, |b|, c) in one instruction, NaN if any is.
+__device__ __forceinline__ float fmax3_abs_nan(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(fabsf(a)), "f"(fabsf(b)), "f"(c));
+    return d;
+}
+
 // Packed fp32 pair arithmetic (sm_100 f32x2): two IEEE round-to-nearest results per instruction.
 __device__ __forceinline__ void fma2(float& d0, float& d1, float a0, float a1, float b0, float b1, float c0,
                                      float c1) {
@@ -182,6 +189,14 @@ __device__ __forceinline__ void add2(float& d0, float& d1, float a0, float a1) {
     asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(d0), "f"(d1));
     asm("mov.b64 %0, {%1, %2};" : "=l"(a) : "f"(a0), "f"(a1));
     asm("add.rn.f32x2 %0, %0, %1;" : "+l"(d) : "l"(a));
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(d0), "=f"(d1) : "l"(d));
+}
+
+__device__ __forceinline__ void mul2(float& d0, float& d1, float a0, float a1, float b0, float b1) {
+    unsigned long long a, b, d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(a) : "f"(a0), "f"(a1));
+    asm("mov.b64 %0, {%1, %2};" : "=l"(b) : "f"(b0), "f"(b1));
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     asm("mov.b64 {%0, %1}, %2;" : "=f"(d0), "=f"(d1) : "l"(d));
 }
 

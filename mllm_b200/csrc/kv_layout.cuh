@@ -29,8 +29,13 @@ __device__ __forceinline__ bool kv_locate(const KvLayout& lay, int b, int64_t t,
         row = (int)t;
         return true;
     }
-    const int64_t i = t / lay.block_size;
-    row = (int)(t - i * lay.block_size);
+    if (t > 0x7fffffffLL) {   // no cache addresses so many rows; below, 32-bit division
+        record_error(kErrBadLength);
+        blk = row = 0;
+        return false;
+    }
+    const int i = (int)t / lay.block_size;
+    row = (int)t - i * lay.block_size;
     const int e = (i < lay.max_blocks) ? lay.table[(int64_t)b * lay.table_stride + i] : -1;
     if (e < 0 || e >= lay.num_blocks) {
         record_error(kErrBadLength);

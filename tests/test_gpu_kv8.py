@@ -74,6 +74,10 @@ EPILOGUE = [
     (4, 4, 64, [1, 1, 0, 2], [10, 300, 7, 0], 0, False, 4),
     (5, 1, 128, [33], [95], 2, True, 1),             # rows that start on no 8-byte boundary
     (40, 8, 128, [2] * 40, list(range(40)), 0, True, 0),   # more sequences than one ballot
+    # enough tokens for the form that streams them (some SMs' warps get one more than others)
+    (8, 2, 128, [3000, 1, 0, 777, 1500], [0, 130, 9, 5, 100], 5, True, 0),
+    (5, 1, 64, [1] * 50 + [4999], [3] * 51, 0, False, 0),
+    (10, 2, 64, [2500, 2499], [0, 1], 700, True, 8),
 ]
 
 
