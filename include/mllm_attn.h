@@ -434,7 +434,7 @@ MLLM_API int mllm_kv8_read_bf16(const mllm_paged_kv8* kv, const int32_t* first_r
                                 int num_kv_heads, int head_dim, int rows, void* k_out, void* v_out, int64_t out_sb,
                                 int64_t out_sh, int64_t out_st, mllm_stream_t stream);
 
-MLLM_API size_t mllm_decode_attention_kv8_workspace_size(int num_heads, int num_kv_heads, int head_dim);
+MLLM_API size_t mllm_decode_attention_kv8_workspace_size(int batch, int num_heads, int num_kv_heads, int head_dim);
 
 MLLM_API int mllm_decode_attention_paged_kv8(const void* q, const mllm_paged_kv8* kv, const int32_t* kv_lens, int batch,
                                              int num_heads, int num_kv_heads, int head_dim, int max_kv_len,

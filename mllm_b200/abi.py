@@ -94,7 +94,7 @@ SIGNATURES = {
     "mllm_qkv_epilogue_varlen_paged_kv8": (_i, [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _i, _i, _i, _i, _p, _d,
                                                 _p, _p, _p, _p, _d, _p, _i64, _i64, _kv8, _p, _i, _p, _p]),
     "mllm_kv8_read_bf16": (_i, [_kv8, _p, _p, _i, _i, _i, _i, _p, _p, _i64, _i64, _i64, _p]),
-    "mllm_decode_attention_kv8_workspace_size": (_sz, [_i, _i, _i]),
+    "mllm_decode_attention_kv8_workspace_size": (_sz, [_i, _i, _i, _i]),
     "mllm_decode_attention_paged_kv8": (_i, [_p, _kv8, _p, _i, _i, _i, _i, _i, _f, _p, _p, _sz, _p]),
     "mllm_decode_attention_shared_workspace_size": (_sz, [_i, _i, _i, _i, _i]),
     "mllm_decode_attention_shared_paged_bf16": (_i, [_p, _kv, _p, _i, _i, _i, _i, _i, _i, _f, _p, _p, _sz, _p]),

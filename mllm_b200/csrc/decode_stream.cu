@@ -95,6 +95,9 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
         : "memory");
 }
 
+// The slots of whole pairs (joined with a prefix) follow two for every CTA there may be.
+__device__ __forceinline__ int64_t whole_slots(const StreamArgs& a) { return 2 * (int64_t)kSharedWaves * a.ctas; }
+
 // A pair's stretch of this CTA's tiles.
 struct Walk {
     int b, g;
@@ -155,13 +158,13 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
         mbar_fence_init();
     }
-    // Behind a prefix kernel (after_prefix) nothing here depends on that kernel, which has itself waited for
+    // Behind a prefix kernel (shared) nothing here depends on that kernel, which has itself waited for
     // everything before it and then let this grid start: the wait moves to the end of the kernel.
-    if (!a.after_prefix) pdl_wait();
+    if (!a.shared) pdl_wait();
     pdl_trigger();
     if (warp == 0) {
         const int total = total_tiles<TILE>(a, lane);
-        const int per = tiles_per_cta(total, gridDim.x, a.min_tiles);
+        const int per = tiles_per_cta(a, total);
         const int p0 = min(total, (int)blockIdx.x * per);
         const int n = min(per, total - p0);
         int before = 0;   // tiles of the sequences before this batch of 32
@@ -191,6 +194,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         if (lane == 0) {
             s_plan[0] = n;
             s_plan[1] = p0;
+            if (blockIdx.x == 0) a.plan[kPlanPer] = per;
         }
     }
     __syncthreads();
@@ -254,51 +258,65 @@ __global__ void __launch_bounds__(kThreads, 2)
         int stage = 0;
         uint32_t phase = 0;
         bool alive = true;
+        // Raw q of a pair as the B operand needs it: column n = head grp, along head_dim four neighbours (8-bit) or two
+        // pairs eight apart per k-step.  The next pair's is loaded while the present one is worked on.
+        uint2 raw[KS];
+        auto load_q = [&](const Walk& at) {
+            const bool ok = grp < a.n_rep;
+            const __nv_bfloat16* qrow = a.q + ((int64_t)at.b * a.H + (int64_t)at.g * a.n_rep + (ok ? grp : 0)) * D;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                if constexpr (k8) {
+                    raw[ks] = *reinterpret_cast<const uint2*>(qrow + ks * 16 + tig * 4);
+                } else {
+                    raw[ks].x = *reinterpret_cast<const uint32_t*>(qrow + ks * 16 + tig * 2);
+                    raw[ks].y = *reinterpret_cast<const uint32_t*>(qrow + ks * 16 + tig * 2 + 8);
+                }
+                if (!ok) raw[ks] = make_uint2(0u, 0u);
+            }
+        };
+        load_q(w);
+        bool more;
+        Walk next = w;
         do {
-            // Q as the B operand: column n = head grp; two values per register along head_dim
             uint32_t qb[KS][2];
             float sc0, sc1;          // log2-domain scales of heads 2 tig and 2 tig + 1
-            {
-                const bool ok = grp < a.n_rep;
-                const __nv_bfloat16* qrow = a.q + ((int64_t)w.b * a.H + (int64_t)w.g * a.n_rep + (ok ? grp : 0)) * D;
-                if constexpr (k8) {
-                    float x[KS][4];
-                    float amax = 0.f;
+            if constexpr (k8) {
+                float x[KS][4];
+                float amax = 0.f;
 #pragma unroll
-                    for (int ks = 0; ks < KS; ++ks) {
-                        const uint2 raw = *reinterpret_cast<const uint2*>(qrow + ks * 16 + tig * 4);
-                        const float2 lo = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.x));
-                        const float2 hi = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.y));
-                        x[ks][0] = ok ? lo.x : 0.f;
-                        x[ks][1] = ok ? lo.y : 0.f;
-                        x[ks][2] = ok ? hi.x : 0.f;
-                        x[ks][3] = ok ? hi.y : 0.f;
+                for (int ks = 0; ks < KS; ++ks) {
+                    const float2 lo = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[ks].x));
+                    const float2 hi = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[ks].y));
+                    x[ks][0] = lo.x;
+                    x[ks][1] = lo.y;
+                    x[ks][2] = hi.x;
+                    x[ks][3] = hi.y;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) amax = fmaxf(amax, fabsf(x[ks][e]));
-                    }
-                    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-                    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-                    const int eq = max((int)(__float_as_uint(amax) >> 23) - 127 - 13, kExpMin);
-                    const float inv = pow2i(-eq);
-#pragma unroll
-                    for (int ks = 0; ks < KS; ++ks) {
-                        qb[ks][0] = pack_f16x2(x[ks][0] * inv, x[ks][1] * inv);
-                        qb[ks][1] = pack_f16x2(x[ks][2] * inv, x[ks][3] * inv);
-                    }
-                    const float qs = pow2i(eq) * a.scale_log2;
-                    sc0 = __shfl_sync(0xffffffffu, qs, 8 * tig);
-                    sc1 = __shfl_sync(0xffffffffu, qs, 8 * tig + 4);
-                } else {
-#pragma unroll
-                    for (int ks = 0; ks < KS; ++ks) {
-                        const uint32_t lo = *reinterpret_cast<const uint32_t*>(qrow + ks * 16 + tig * 2);
-                        const uint32_t hi = *reinterpret_cast<const uint32_t*>(qrow + ks * 16 + tig * 2 + 8);
-                        qb[ks][0] = ok ? lo : 0u;
-                        qb[ks][1] = ok ? hi : 0u;
-                    }
-                    sc0 = sc1 = a.scale_log2;
+                    for (int e = 0; e < 4; ++e) amax = fmaxf(amax, fabsf(x[ks][e]));
                 }
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+                const int eq = max((int)(__float_as_uint(amax) >> 23) - 127 - 13, kExpMin);
+                const float inv = pow2i(-eq);
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    qb[ks][0] = pack_f16x2(x[ks][0] * inv, x[ks][1] * inv);
+                    qb[ks][1] = pack_f16x2(x[ks][2] * inv, x[ks][3] * inv);
+                }
+                const float qs = pow2i(eq) * a.scale_log2;
+                sc0 = __shfl_sync(0xffffffffu, qs, 8 * tig);
+                sc1 = __shfl_sync(0xffffffffu, qs, 8 * tig + 4);
+            } else {
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    qb[ks][0] = raw[ks].x;
+                    qb[ks][1] = raw[ks].y;
+                }
+                sc0 = sc1 = a.scale_log2;
             }
+            more = walk_next<TILE>(a, next);
+            if (more) load_q(next);
             float o[KS][4];
 #pragma unroll
             for (int i = 0; i < KS; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
@@ -527,7 +545,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             }
             asm volatile("bar.sync 1, %0;" ::"n"(kConsumerWarps * 32) : "memory");
             // ---- write the stretch's rows: final, or a partial ----
-            if (w.whole() && !a.prefix_parts) {
+            if (w.whole() && !a.shared) {
                 __nv_bfloat16* orow = a.out + ((int64_t)w.b * a.H + (int64_t)w.g * a.n_rep) * D;
                 for (int i = threadIdx.x; i < a.n_rep * (D / 2); i += kConsumerWarps * 32) {
                     const int h = i / (D / 2), d = 2 * (i % (D / 2));
@@ -537,7 +555,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             } else {
                 // a whole pair's row (joined with the prefix) has a slot of its own; a cut pair takes the
                 // CTA's first slot if the CTA begins in it, else the second
-                const int64_t slot = w.whole() ? 2 * (int64_t)gridDim.x + (int64_t)w.b * a.Hkv + w.g
+                const int64_t slot = w.whole() ? whole_slots(a) + (int64_t)w.b * a.Hkv + w.g
                                                : 2 * (int64_t)blockIdx.x + (w.pos == s_plan[1] ? 0 : 1);
                 float* po = a.part_o + slot * a.n_rep * D;
                 for (int i = threadIdx.x; i < a.n_rep * (D / 4); i += kConsumerWarps * 32) {
@@ -547,107 +565,120 @@ __global__ void __launch_bounds__(kThreads, 2)
                 }
                 if (threadIdx.x < a.n_rep) a.part_lse[slot * a.n_rep + threadIdx.x] = red_l[threadIdx.x];
             }
+            if (w.t0 == 0 && threadIdx.x == 0) a.plan[kPlanHead + w.b * a.Hkv + w.g] = w.pos;   // where the pair begins
             asm volatile("bar.sync 1, %0;" ::"n"(kConsumerWarps * 32) : "memory");
-        } while (walk_next<TILE>(a, w));
+            w = next;
+        } while (more);
     }
-    if (a.after_prefix) pdl_wait();   // so that this grid ends after the prefix kernel's
+    // One CTA waits, so that this grid ends after the prefix kernel's; were it all of them, those that are done would
+    // hold their SMs until then.
+    if (a.shared && blockIdx.x == gridDim.x - 1) pdl_wait();
 }
 
 // Joins the parts of every (sequence, query head): the stretches of the cut pairs and, with a shared prefix, the
-// prefix's parts.  A part is a normalised row and log2 of its weight: out = sum_i 2^(e_i - M) row_i / sum_i 2^(e_i - M).
-// One CTA a (query head, sequence), thread d column d, parts in a fixed order.
+// prefix's parts.  A part is a normalised row and log2 of its weight: out = sum_i 2^(e_i - M) row_i / sum_i 2^(e_i - M),
+// parts in a fixed order.  A warp takes one query head, so nothing waits at a barrier: the time of this kernel is that
+// of its chain of dependent loads (the pair's place, the weights, the rows), and its launch.
+constexpr int kCombineWarps = 4;
+
 template <int D, int TILE>
-__global__ void __launch_bounds__(D) stream_combine_kernel(StreamArgs a, int grid) {
-    __shared__ float s_red[D / 32];
-    __shared__ int s_tiles[2][D / 32];
+__global__ void __launch_bounds__(kCombineWarps * 32) stream_combine_kernel(StreamArgs a) {
+    constexpr int E = D / 32;        // columns per lane
+    constexpr int U = 8;             // rows in flight
+    const int lane = threadIdx.x & 31;
+    const int bh = blockIdx.x * kCombineWarps + (threadIdx.x >> 5);
+    if (bh >= a.B * a.H) return;
+    const int b = bh / a.H, h = bh - b * a.H, g = h / a.n_rep, r = h - g * a.n_rep;
     pdl_wait();
-    const int h = blockIdx.x, b = blockIdx.y, g = h / a.n_rep, r = h - g * a.n_rep;
-    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-    // tiles of all sequences, and of those before b
-    int all = 0, before = 0;
-    for (int i = t; i < a.B; i += D) {
-        const int n = seq_tiles<TILE>(a, i).tiles;
-        all += n;
-        if (i < b) before += n;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        all += __shfl_xor_sync(0xffffffffu, all, o);
-        before += __shfl_xor_sync(0xffffffffu, before, o);
-    }
-    if (lane == 0) {
-        s_tiles[0][warp] = all;
-        s_tiles[1][warp] = before;
-    }
-    __syncthreads();
-    all = before = 0;
-#pragma unroll
-    for (int w = 0; w < D / 32; ++w) {
-        all += s_tiles[0][w];
-        before += s_tiles[1][w];
-    }
+    const int per = a.plan[kPlanPer], p0 = a.plan[kPlanHead + b * a.Hkv + g];   // p0 means nothing without tiles
     const SeqTiles s = seq_tiles<TILE>(a, b);
-    __nv_bfloat16* orow = a.out + ((int64_t)b * a.H + h) * D;
-    const int n_pre = s.short_len ? 0 : a.prefix_parts;
-    if (s.tiles == 0 && n_pre == 0) {   // nothing to attend to
-        orow[t] = __float2bfloat16_rn(0.f);
-        return;
+    const int n_pre = !a.shared || s.short_len ? 0 : a.plan[b < a.pair_seqs ? kPlanPair : kPlanSingle];
+    int c0 = s.tiles ? p0 / per : 0;
+    int own = s.tiles ? (p0 + s.tiles - 1) / per - c0 + 1 : 0;
+    if (s.tiles && (p0 < 0 || c0 + own > kSharedWaves * a.ctas)) {   // the pair's place was never written: its CTA
+                                                                      // gave up a wait
+        record_error(kErrTimeout);
+        c0 = own = 0;
     }
-    const int per = tiles_per_cta(all * a.Hkv, grid, a.min_tiles);
-    const int p0 = before * a.Hkv + g * s.tiles, p1 = p0 + s.tiles;
-    const int c0 = p0 / per, c1 = s.tiles ? (p1 - 1) / per : c0 - 1;
-    const int own = c1 - c0 + 1;
     if (own == 1 && n_pre == 0) return;   // written directly
-    const int n = own + n_pre;
+    const int n = own + n_pre;            // 0: nothing to attend to
     auto part = [&](int i) -> int64_t {   // index of part i's row in part_o and part_lse
         if (i >= own) return a.prefix_base + (((int64_t)(i - own) * a.Hkv + g) * a.B + b) * a.n_rep + r;
         const int c = c0 + i;
-        const int64_t slot = own == 1 ? 2 * (int64_t)grid + (int64_t)b * a.Hkv + g : 2 * (int64_t)c + (c * per >= p0 ? 0 : 1);
+        const int64_t slot = own == 1 ? whole_slots(a) + (int64_t)b * a.Hkv + g
+                                      : 2 * (int64_t)c + (c * per >= p0 ? 0 : 1);
         return slot * a.n_rep + r;
     };
-    float mx = -INFINITY;
-    for (int i = t; i < n; i += D) mx = fmaxf(mx, a.part_lse[part(i)]);
+    float acc[E], sum = 0.f, M = -INFINITY;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    if (lane == 0) s_red[warp] = mx;
-    __syncthreads();
-    float M = s_red[0];
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+    for (int i0 = 0; i0 < n; i0 += 32) {
+        const int m = min(32, n - i0);
+        const int64_t mine = part(min(i0 + lane, n - 1));
+        const float w = lane < m ? a.part_lse[mine] : -INFINITY;
+        auto load = [&](int i, float (&v)[E]) {
+            const float* src = a.part_o + __shfl_sync(0xffffffffu, mine, i & 31) * D + lane * E;
+            if constexpr (E == 4) {
+                const float4 x = *reinterpret_cast<const float4*>(src);
+                v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+            } else {
+                const float2 x = *reinterpret_cast<const float2*>(src);
+                v[0] = x.x, v[1] = x.y;
+            }
+        };
+        float v[U][E];
 #pragma unroll
-    for (int w = 1; w < D / 32; ++w) M = fmaxf(M, s_red[w]);
-    if (M == -INFINITY) M = 0.f;
-    float acc = 0.f, sum = 0.f;
-    constexpr int U = 8;   // parts whose loads are in flight together
-    for (int i0 = 0; i0 < n; i0 += U) {
-        float v[U], e[U];
+        for (int u = 0; u < U; ++u) load(min(u, m - 1), v[u]);   // on their way while the weights are
+        float top = w;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const bool in = i0 + u < n;
-            const int64_t p = in ? part(i0 + u) : 0;
-            v[u] = in ? a.part_o[p * D + t] : 0.f;
-            e[u] = in ? a.part_lse[p] : -INFINITY;
-        }
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        top = fmaxf(top, M);
+        const float Mu = top == -INFINITY ? 0.f : top;
+        const float scale = ex2_approx(M - Mu);
+        M = top;
+        sum *= scale;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const float wgt = ex2_approx(e[u] - M);
-            acc += wgt * v[u];
-            sum += wgt;
+        for (int e = 0; e < E; ++e) acc[e] *= scale;
+        const float wgt = ex2_approx(w - Mu);
+        for (int j = 0; j < m; j += U) {
+            if (j > 0) {
+#pragma unroll
+                for (int u = 0; u < U; ++u) load(min(j + u, m - 1), v[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const float f = __shfl_sync(0xffffffffu, wgt, (j + u) & 31);
+                if (j + u < m) {
+                    sum += f;
+#pragma unroll
+                    for (int e = 0; e < E; ++e) acc[e] += f * v[u][e];
+                }
+            }
         }
     }
-    orow[t] = __float2bfloat16_rn(sum > 0.f || sum != sum ? acc / sum : 0.f);
+    const bool any = sum > 0.f || sum != sum;
+    __nv_bfloat16* out = a.out + (int64_t)bh * D + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; e += 2)
+        *reinterpret_cast<uint32_t*>(out + e) = pack_bf16x2(any ? acc[e] / sum : 0.f, any ? acc[e + 1] / sum : 0.f);
 }
 
-constexpr int kMaxGrid = 2 * 160;
-
-int stream_grid(int num_sms) { return std::min(2 * num_sms, kMaxGrid); }
+constexpr int kMaxCtas = 2 * 160;
 
 }  // namespace
 
-size_t stream_part_rows(int batch, int num_kv_heads, bool shared) {
-    return 2 * (size_t)kMaxGrid + (shared ? (size_t)batch * num_kv_heads : 0);
+size_t stream_part_rows(int n_rep, int batch, int num_kv_heads, bool shared) {
+    return (2 * (size_t)kMaxCtas * (shared ? kSharedWaves : 1) + (shared ? (size_t)batch * num_kv_heads : 0)) * n_rep;
 }
 
-size_t stream_workspace_bytes(int n_rep, int D, size_t part_rows) {
-    return (part_rows * n_rep * (size_t)(D + 1) * 4 + 255) & ~size_t(255);
+size_t stream_workspace_bytes(int D, size_t part_rows, int batch, int num_kv_heads) {
+    return (part_rows * (size_t)(D + 1) * 4 + (kPlanHead + (size_t)batch * num_kv_heads) * 4 + 255) & ~size_t(255);
+}
+
+void stream_place(StreamArgs& a, void* workspace, int D, size_t part_rows) {
+    a.part_o = static_cast<float*>(workspace);
+    a.part_lse = a.part_o + part_rows * D;
+    a.plan = reinterpret_cast<int*>(a.part_lse + part_rows);
 }
 
 namespace {
@@ -656,11 +687,11 @@ template <int D, bool k8>
 int launch_stream_d(StreamArgs& a, const Kv8View& kv, const CUtensorMap& tmK, const CUtensorMap& tmV, int num_sms,
                     cudaStream_t s) {
     using C = Cfg<D, k8>;
-    a.min_tiles = k8 ? 1 : 2;
     // no more CTAs than tiles there can be
-    const int64_t most = (int64_t)a.B * a.Hkv * ((a.max_len + C::kTile - 1) / C::kTile);
+    const int64_t most = (int64_t)a.B * a.Hkv * ((a.max_len + C::kTile - 1) / C::kTile - a.first_row / C::kTile);
     if (most > 0x7fffffffLL - 65536) return fail(MLLM_ERR_UNSUPPORTED, "decode_attention: batch too large for one call");
-    const int grid = (int)std::min<int64_t>(stream_grid(num_sms), std::max<int64_t>(most, 1));
+    a.ctas = std::min(2 * num_sms, kMaxCtas);
+    const int grid = stream_ctas(most, a.ctas, a.shared);
     auto kern = stream_decode_kernel<D, k8>;
     if (int st = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes),
                             "stream_decode smem attribute"))
@@ -668,7 +699,9 @@ int launch_stream_d(StreamArgs& a, const Kv8View& kv, const CUtensorMap& tmK, co
     if (int st = check_cuda(launch_pdl(kern, dim3(grid), dim3(kThreads), C::kSmemBytes, s, tmK, tmV, a, kv),
                             "stream_decode_kernel launch"))
         return st;
-    return check_cuda(launch_pdl(stream_combine_kernel<D, C::kTile>, dim3(a.H, a.B), dim3(D), 0, s, a, grid),
+    return check_cuda(launch_pdl(stream_combine_kernel<D, C::kTile>,
+                                 dim3((unsigned)(((int64_t)a.B * a.H + kCombineWarps - 1) / kCombineWarps)),
+                                 dim3(kCombineWarps * 32), 0, s, a),
                       "stream_combine_kernel launch");
 }
 
@@ -686,9 +719,10 @@ MLLM_DEFINE_STATUS_READER(decode_stream)
 
 using namespace mllm_b200;
 
-extern "C" size_t mllm_decode_attention_kv8_workspace_size(int num_heads, int num_kv_heads, int head_dim) {
-    if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads || head_dim <= 0) return 0;
-    return stream_workspace_bytes(num_heads / num_kv_heads, head_dim, stream_part_rows(0, num_kv_heads, false));
+extern "C" size_t mllm_decode_attention_kv8_workspace_size(int batch, int num_heads, int num_kv_heads, int head_dim) {
+    if (batch <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads || head_dim <= 0) return 0;
+    const size_t rows = stream_part_rows(num_heads / num_kv_heads, batch, num_kv_heads, false);
+    return stream_workspace_bytes(head_dim, rows, batch, num_kv_heads);
 }
 
 extern "C" int mllm_decode_attention_paged_kv8(const void* q, const mllm_paged_kv8* kv, const int32_t* kv_lens, int batch,
@@ -715,7 +749,7 @@ extern "C" int mllm_decode_attention_paged_kv8(const void* q, const mllm_paged_k
     if (!aligned(q, 8) || !aligned(out, 4))
         return fail(MLLM_ERR_INVALID_ARGUMENT, "decode_attention_kv8: q/out misaligned");
     if (!workspace || !aligned(workspace, 256) ||
-        workspace_bytes < mllm_decode_attention_kv8_workspace_size(num_heads, num_kv_heads, head_dim))
+        workspace_bytes < mllm_decode_attention_kv8_workspace_size(batch, num_heads, num_kv_heads, head_dim))
         return fail(MLLM_ERR_WORKSPACE, "decode_attention_kv8: workspace missing, misaligned or smaller than "
                                         "mllm_decode_attention_kv8_workspace_size()");
     int num_sms = 0;
@@ -736,8 +770,7 @@ extern "C" int mllm_decode_attention_paged_kv8(const void* q, const mllm_paged_k
     a.n_rep = n_rep;
     a.max_len = max_kv_len;
     a.scale_log2 = (float)((double)softmax_scale * 1.4426950408889634);
-    a.part_o = static_cast<float*>(workspace);
-    a.part_lse = a.part_o + stream_part_rows(0, num_kv_heads, false) * n_rep * head_dim;
+    stream_place(a, workspace, head_dim, stream_part_rows(n_rep, batch, num_kv_heads, false));
     if (int st = head_dim == 128 ? launch_stream_d<128, true>(a, view, tmK, tmV, num_sms, (cudaStream_t)stream)
                                  : launch_stream_d<64, true>(a, view, tmK, tmV, num_sms, (cudaStream_t)stream))
         return st;

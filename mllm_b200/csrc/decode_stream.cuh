@@ -10,22 +10,27 @@ namespace mllm_b200 {
 
 constexpr int kMaxGroup = 8;       // query heads per kv head (the N side of the MMAs)
 
+constexpr int kPlanPer = 0, kPlanPair = 1, kPlanSingle = 2, kPlanHead = 3;
+
 struct StreamArgs {
     const __nv_bfloat16* q;        // [B, H, D]
     const int32_t* kv_lens;        // [B]
     __nv_bfloat16* out;            // [B, H * D]
     float* part_o;                 // parts: rows of D floats ...
     float* part_lse;               // ... and log2 of their weights
+    int* plan;                     // [kPlanHead + B * Hkv]: what the kernels work out for one another (kPlan*), then
+                                   // the first tile of every pair that has any
     int B, H, Hkv, n_rep, max_len;
-    int min_tiles;                 // tiles a CTA takes at least
+    int ctas;                      // two per SM
     float scale_log2;
     KvLayout lay;
-    // shared prefix: rows before first_row are the prefix kernel's, which leaves prefix_parts parts a query row at
-    // row prefix_base of the parts: [part][kv head][sequence][head of the group]
+    // shared prefix: rows before first_row are the prefix kernel's, which leaves plan[kPlanPair] parts of every query
+    // row of the first pair_seqs sequences, plan[kPlanSingle] of the others', at row prefix_base of the parts:
+    // [part][kv head][sequence][head of the group]
     int first_row;
-    int prefix_parts;
+    int shared;                    // there is a prefix, and its kernel let this grid in
+    int pair_seqs;
     int64_t prefix_base;
-    int after_prefix;              // the grid was let in by the prefix kernel
 };
 
 // Rows [first_row, len) of a sequence in tiles of TILE cache rows.  A length outside [0, max_len] is recorded and
@@ -61,13 +66,34 @@ __device__ __forceinline__ int total_tiles(const StreamArgs& a, int lane) {
     return n * a.Hkv;
 }
 
-__device__ __forceinline__ int tiles_per_cta(int total, int grid, int min_tiles) {
-    return max((total + grid - 1) / grid, min_tiles);
+// CTAs the tiles are dealt to: two per SM, which stay; behind a prefix kernel up to four times as many, so that the SMs
+// that become free first take more of them (with two per SM, the ones that had to wait for a prefix CTA's SM ended
+// last), but only where each has a few tiles.  It follows from the tiles there are, not from a bound on them: a graph
+// captured for longer sequences gives the same bits.
+constexpr int kSharedWaves = 4;
+constexpr int kWaveTiles = 4;
+
+__host__ __device__ __forceinline__ int stream_ctas(int64_t tiles, int ctas, int shared) {
+    int64_t n = ctas;
+    if (shared) {
+        const int64_t waves = tiles / kWaveTiles < (int64_t)kSharedWaves * ctas ? tiles / kWaveTiles
+                                                                                : (int64_t)kSharedWaves * ctas;
+        if (waves > n) n = waves;
+    }
+    if (n > tiles) n = tiles;
+    return n < 1 ? 1 : (int)n;
 }
 
+__device__ __forceinline__ int tiles_per_cta(const StreamArgs& a, int total) {
+    const int n = stream_ctas(total, a.ctas, a.shared);
+    return max((total + n - 1) / n, 1);
+}
+
+// The workspace: `part_rows` rows of D floats, their weights, the plan.
 // Rows of parts the even-split decode writes: two slots a CTA, and with a shared prefix one per pair.
-size_t stream_part_rows(int batch, int num_kv_heads, bool shared);
-size_t stream_workspace_bytes(int n_rep, int D, size_t part_rows);
+size_t stream_part_rows(int n_rep, int batch, int num_kv_heads, bool shared);
+size_t stream_workspace_bytes(int D, size_t part_rows, int batch, int num_kv_heads);
+void stream_place(StreamArgs& a, void* workspace, int D, size_t part_rows);
 
 // Runs the split and the combine kernel over a bf16 paged cache.
 int launch_stream_bf16(StreamArgs& a, int head_dim, const CUtensorMap& tmK, const CUtensorMap& tmV, int num_sms,

@@ -7,15 +7,18 @@
 //
 // prefix_kernel: one CTA per (kv head, block of query rows, stretch of the prefix); the machinery is that of the
 // prefill kernel (tcgen05.mma M = 128, scores and O in tensor memory, one softmax thread per row, TMA ring with
-// separate K and V barriers), without a causal bound and with two forms:
-//   two query tiles (kPair): 256 query rows share every K/V tile.  For batches of more than 128 rows, where the
-//       tensor and exponential work per K/V byte is what bounds.
-//   one query tile: 128 rows, and the two softmax groups take alternate K/V tiles, each with its own running
-//       maximum, sum and O.  With so few rows the kernel is bound by the K/V bytes; alternating keeps one tile's
-//       products running under the other's softmax, and the Q tile not needed makes room for a third stage.
+// separate K and V barriers), without a causal bound and in two forms:
+//   a pair of query tiles: 256 query rows share every K/V tile.  For batches of more than 128 rows, where the tensor
+//       and exponential work per K/V byte is what bounds.
+//   a single query tile (a small batch, or the odd tile of a large one): the two softmax groups take alternate K/V
+//       tiles, each with its own running maximum, sum and O, and are joined at the end.  With few rows the kernel is
+//       bound by the K/V bytes; alternating keeps one tile's products running under the other's softmax.
 // A query tile holds floor(128 / n_rep) sequences with their n_rep heads, fetched by one TMA box
 // {64 columns, n_rep heads, sequences}; rows behind them are never looked at.  Warps without a valid row skip
-// their softmax.  The stretches leave normalised fp32 rows and log2 weights.
+// their softmax.  The stretches are dealt out by what a K/V tile costs each form.
+// A stretch leaves one normalised fp32 row and log2 weight per query row.  The rows of a tile are contiguous in the
+// parts; they go through shared memory (the tiles are done with by then), because a thread holds a whole row in tensor
+// memory and 32 threads storing 16 bytes of 32 rows at a time took 4 us of a 16 us kernel.
 // The rows of the last K/V tile behind the prefix are other rows of the block: K's are masked, V's read as zero
 // through a tensor map that ends with the prefix, so that their contents cannot matter.
 //
@@ -34,6 +37,7 @@ namespace {
 
 constexpr int kBM = 128;            // query rows per tile
 constexpr int kBN = 128;            // cache rows per K/V tile
+constexpr int kOwnTile = 64;        // cache rows per tile of the bf16 even-split decode
 constexpr int kThreads = 384;       // {producer, MMA, 2 idle warps}, softmax group 0, softmax group 1
 // The register split of the prefill kernel: 128 x 72 + 256 x 216 = 384 x 168.
 constexpr uint32_t kLaunchRegs = 168;
@@ -44,80 +48,200 @@ constexpr int kBox = kBN * 128;     // one 128-row x 64-column bf16 box (16 KB)
 constexpr uint32_t kTmemCols = 512; // S_0, S_1, O_0, O_1 of 128 columns
 constexpr float kRescaleThreshold = 8.0f;  // log2 units: O is rescaled only when the maximum grows by more
 
-template <int D, bool kPair>
+// kPairs: the launch has pairs of query tiles; without, a third stage takes the place of the second Q tile.
+template <int D, bool kPairs>
 struct PrefixCfg {
     static constexpr int kBoxes = D / 64;
     static constexpr int kTileBytes = kBoxes * kBox;                 // one Q, K or V tile
-    static constexpr int kQTiles = kPair ? 2 : 1;
-    static constexpr int kStages = D == 128 ? (kPair ? 2 : 3) : 4;
+    static constexpr int kQTiles = kPairs ? 2 : 1;
+    static constexpr int kStages = D == 128 ? (kPairs ? 2 : 3) : 4;
+    static constexpr int kRowFloats = D + 4;                         // of a result row in shared memory (bank spread)
     static constexpr int kSmemBytes = (kQTiles + 2 * kStages) * kTileBytes + 256 + 1024;
     static_assert((1 + 4 * kStages + 6) * 8 + 4 <= 256, "barrier area too small");
     static_assert(kSmemBytes <= 232448, "more shared memory than a CTA has");
+    static_assert(2 * kBM * (kRowFloats + 2) * 4 <= (kQTiles + 2 * kStages) * kTileBytes, "results do not fit");
 };
 
 struct PrefixArgs {
     float* part_o;       // [parts][Hkv][B][n_rep][D]
     float* part_lse;     // [parts][Hkv][B][n_rep]
     int B, Hkv, n_rep, seqs;   // seqs: sequences per query tile
-    int prefix, n_tiles, per;  // K/V tiles of the prefix; tiles per stretch
-    int mblocks;
+    int prefix, n_tiles;       // K/V tiles of the prefix
+    int pairs, single;         // blocks of two query tiles; whether one more block follows with the tile left
+    int num_sms;
     float scale_log2;
     KvLayout lay;
 };
 
+// How the prefix is cut: stretches and K/V tiles in each, for a pair's block and for the single tile's.
+struct PrefixCut {
+    int splits, per, splits_single, per_single;
+};
+
+// Blocks get stretches by their cost per K/V tile, 3 for a pair and 2 for a single tile, so that the CTAs of `sms` SMs
+// per kv head end together.  More SMs never give fewer stretches.
+__host__ __device__ inline PrefixCut cut_prefix(int n_tiles, int sms, int pairs, int single) {
+    PrefixCut c = {};
+    int want_single = 0;
+    if (single) {
+        want_single = 2 * sms / (3 * pairs + 2);
+        if (want_single < 1) want_single = 1;
+        c.per_single = (n_tiles + want_single - 1) / want_single;
+        c.splits_single = (n_tiles + c.per_single - 1) / c.per_single;
+    }
+    if (pairs) {
+        int want = (sms - want_single) / pairs;
+        if (want < 1) want = 1;
+        c.per = (n_tiles + want - 1) / want;
+        c.splits = (n_tiles + c.per - 1) / c.per;
+    }
+    return c;
+}
+
+// SMs per kv head for the prefix, so that it ends with the decode of the sequences' own rows on the other SMs: with P
+// and S the SM-microseconds of the two, F the fixed time of a prefix CTA and N SMs, X SMs take F + P / X, and all is
+// done after (P + S + F X) / N.  Fitted (D = 128): 1.8 us a tile for a pair, 0.9 for a single tile, 4 us for the CTA; 0.5 us
+// for a 64-row tile of the other kernel and 2 us of an SM for each of its CTAs.  D = 64 moves half.
+__device__ __forceinline__ int prefix_sms(const PrefixArgs& a, float own_tiles, float dim_scale) {
+    const float N = (float)a.num_sms, F = 4.f;
+    const float P = (float)a.Hkv * a.n_tiles * (1.8f * a.pairs + 0.9f * a.single) * dim_scale;
+    const float S = 0.5f * own_tiles * dim_scale + 2.f * fminf(own_tiles, 2.f * N);
+    const float b = P + S - N * F;
+    const float X = (sqrtf(b * b + 4.f * F * N * P) - b) / (2.f * F);
+    return max(1, min(a.num_sms / a.Hkv, (int)(X / a.Hkv + 0.5f)));
+}
+
 __device__ __forceinline__ uint32_t col_s(int i) { return (uint32_t)(i * kBN); }
 __device__ __forceinline__ uint32_t col_o(int i) { return (uint32_t)(2 * kBN + i * 128); }
 
-template <int D, bool kPair>
+// The barriers of a CTA, in shared memory behind the tiles.
+template <int ST>
+struct Bars {
+    uint64_t *q_full, *k_full, *k_empty, *v_full, *v_empty;   // [1], then [ST] each
+    uint64_t *s_full, *p_full, *o_done;                       // [2] per softmax group
+    __device__ __forceinline__ explicit Bars(uint64_t* p)
+        : q_full(p), k_full(p + 1), k_empty(k_full + ST), v_full(k_empty + ST), v_empty(v_full + ST),
+          s_full(v_empty + ST), p_full(s_full + 2), o_done(p_full + 2) {}
+};
+
+// The tensor pipe's thread: for every step and group O += P V, then the group's next S = Q K^T, so that one group's
+// softmax runs under the other's products.  Step k of group i works on tile k (kPair) or 2 k + i.
+template <int D, bool kPairs, bool kPair>
+__device__ __forceinline__ void issue_products(uint8_t* sQ, uint8_t* sKV, uint64_t* bars, uint32_t tmem, int n) {
+    using C = PrefixCfg<D, kPairs>;
+    constexpr int ST = C::kStages;
+    const Bars<ST> bar(bars);
+    constexpr uint32_t idesc_s = idesc_bf16_f32(kBM, kBN, false);
+    constexpr uint32_t idesc_o = idesc_bf16_f32(kBM, D, true);
+    constexpr uint32_t desc_hi = smem_desc_hi_sw128(1024);
+    const int steps[2] = {kPair ? n : (n + 1) / 2, kPair ? n : n / 2};
+    auto tile_of = [&](int i, int k) { return kPair ? k : 2 * k + i; };
+    auto issue_s = [&](int i, int j) {
+        const uint32_t qd = smem_desc_lo(smem_u32(sQ + (kPair ? i : 0) * C::kTileBytes), 16);
+        const uint32_t kd = smem_desc_lo(smem_u32(sKV + (j % ST) * 2 * C::kTileBytes), 16);
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+            const uint32_t off = (uint32_t)(((ks >> 2) * kBox + (ks & 3) * 32) >> 4);
+            tc_mma_ss_w(tmem + col_s(i), qd + off, kd + off, desc_hi, idesc_s, ks > 0 ? 1u : 0u);
+        }
+        tc_commit(&bar.s_full[i]);
+    };
+    // K tile j has been read by every product that needs it: free it if it will be refilled
+    auto free_k = [&](int j) { if (j + ST < n) tc_commit(&bar.k_empty[j % ST]); };
+    bool alive = mbar_wait(bar.q_full, 0);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        if (!alive || steps[i] == 0) continue;
+        const int j = tile_of(i, 0);
+        if ((i == 0 || !kPair) && !mbar_wait(&bar.k_full[j % ST], (j / ST) & 1)) { alive = false; continue; }
+        tc_fence_after();
+        issue_s(i, j);
+        if (!kPair || i == 1) free_k(j);
+    }
+    for (int k = 0; k < steps[0] && alive; ++k) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            if (!alive || k >= steps[i]) continue;
+            const int j = tile_of(i, k);
+            if (!mbar_wait(&bar.p_full[i], k & 1)) { alive = false; continue; }
+            if ((!kPair || i == 0) && !mbar_wait(&bar.v_full[j % ST], (j / ST) & 1)) { alive = false; continue; }
+            tc_fence_after();
+            const uint32_t vd = smem_desc_lo(smem_u32(sKV + (j % ST) * 2 * C::kTileBytes + C::kTileBytes), kBox);
+#pragma unroll
+            for (int ks = 0; ks < kBN / 16; ++ks)
+                tc_mma_ts_w(tmem + col_o(i), tmem + col_s(i) + ks * 8, vd + (uint32_t)((ks * 16 * 128) >> 4), desc_hi,
+                            idesc_o, (k > 0 || ks > 0) ? 1u : 0u);
+            const bool last_use = !kPair || i == 1;
+            if (last_use && j + ST < n) tc_commit(&bar.v_empty[j % ST]);
+            if (k + 1 < steps[i]) {
+                const int jn = tile_of(i, k + 1);
+                if ((!kPair || i == 0) && !mbar_wait(&bar.k_full[jn % ST], (jn / ST) & 1)) { alive = false; continue; }
+                tc_fence_after();
+                issue_s(i, jn);   // overwrites P_i(k) only after the product above read it
+                if (last_use) free_k(jn);
+            } else {
+                tc_commit(&bar.o_done[i]);
+            }
+        }
+    }
+}
+
+template <int D, bool kPairs>
 __global__ void __launch_bounds__(kThreads, 1)
     prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                  const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmVend, PrefixArgs a) {
-    using C = PrefixCfg<D, kPair>;
+                  const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmVend, PrefixArgs a,
+                  StreamArgs st) {
+    using C = PrefixCfg<D, kPairs>;
     constexpr int ST = C::kStages;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* sQ = smem;
     uint8_t* sKV = sQ + C::kQTiles * C::kTileBytes;      // [ST][K | V]
     uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + ST * 2 * C::kTileBytes);
-    uint64_t* q_full = bars;
-    uint64_t* k_full = bars + 1;
-    uint64_t* k_empty = k_full + ST;
-    uint64_t* v_full = k_empty + ST;
-    uint64_t* v_empty = v_full + ST;
-    uint64_t* s_full = v_empty + ST;    // [2]
-    uint64_t* p_full = s_full + 2;      // [2] 128 arrivals
-    uint64_t* o_done = p_full + 2;      // [2]
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_done + 2);
+    const Bars<ST> bar(bars);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar.o_done + 2);
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
-    const int g = blockIdx.x % a.Hkv;
-    const int mb = blockIdx.x / a.Hkv;
-    const int split = blockIdx.y;
-    const int first = split * a.per;                     // K/V tiles first .. first + n - 1
-    const int n = min(a.per, a.n_tiles - first);
-    // Step k of softmax group i works on tile k (pair form) or 2 k + i (alternating); group i has steps[i] steps.
-    int steps[2];
-    if (kPair) {
-        steps[0] = n;
-        steps[1] = (2 * mb + 1) * a.seqs < a.B ? n : 0;   // a last block may hold one query tile
-    } else {
-        steps[0] = (n + 1) / 2;
-        steps[1] = n / 2;
+    pdl_wait();
+    // ---- the plan, the same in every CTA: from the tiles that the other kernel will find ----
+    __shared__ PrefixCut s_cut;
+    if (warp == 2) {
+        const int own = total_tiles<kOwnTile>(st, lane);
+        if (lane == 0) {
+            s_cut = cut_prefix(a.n_tiles, prefix_sms(a, (float)own, D == 128 ? 1.f : 0.6f), a.pairs, a.single);
+            if (blockIdx.x == 0 && blockIdx.y == 0) {
+                st.plan[kPlanPair] = s_cut.splits;
+                st.plan[kPlanSingle] = s_cut.splits_single;
+            }
+        }
     }
+    __syncthreads();
+    const PrefixCut cut = s_cut;
+    const int g = blockIdx.x;
+    const int y = blockIdx.y;
+    if (y >= a.pairs * cut.splits + cut.splits_single) return;            // fewer stretches than the most there may be
+    const int mb = y < a.pairs * cut.splits ? y / cut.splits : a.pairs;   // a.pairs: the single tile's block
+    const bool pair = kPairs && mb < a.pairs;
+    const int split = y - mb * cut.splits;
+    const int per = pair ? cut.per : cut.per_single;
+    const int first = split * per;                       // K/V tiles first .. first + n - 1
+    const int n = min(per, a.n_tiles - first);
+    // Step k of softmax group i works on tile k (pair) or 2 k + i (alternating); group i has steps[i] steps.
+    const int steps[2] = {pair ? n : (n + 1) / 2, pair ? n : n / 2};
 
     if (threadIdx.x == 0) {
-        mbar_init(q_full, 1);
+        mbar_init(bar.q_full, 1);
         for (int s = 0; s < ST; ++s) {
-            mbar_init(&k_full[s], 1);
-            mbar_init(&k_empty[s], 1);
-            mbar_init(&v_full[s], 1);
-            mbar_init(&v_empty[s], 1);
+            mbar_init(&bar.k_full[s], 1);
+            mbar_init(&bar.k_empty[s], 1);
+            mbar_init(&bar.v_full[s], 1);
+            mbar_init(&bar.v_empty[s], 1);
         }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], 128);
-            mbar_init(&o_done[i], 1);
+            mbar_init(&bar.s_full[i], 1);
+            mbar_init(&bar.p_full[i], 128);
+            mbar_init(&bar.o_done[i], 1);
         }
         mbar_fence_init();
     }
@@ -129,7 +253,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    pdl_wait();
     pdl_trigger();   // the decode of the sequences' own rows may fill SMs as these CTAs leave them
 
     if (warp < 4) {
@@ -140,13 +263,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                 tma_prefetch_desc(&tmQ);
                 tma_prefetch_desc(&tmK);
                 tma_prefetch_desc(&tmV);
-                const int q_tiles = kPair && steps[1] > 0 ? 2 : 1;
+                const int q_tiles = pair ? 2 : 1;
                 const uint32_t q_box = 128u * (uint32_t)(a.n_rep * a.seqs);   // bytes of one 64-column box
-                mbar_arrive_expect_tx(q_full, (uint32_t)q_tiles * C::kBoxes * q_box);
+                mbar_arrive_expect_tx(bar.q_full, (uint32_t)q_tiles * C::kBoxes * q_box);
                 for (int i = 0; i < q_tiles; ++i)
                     for (int bx = 0; bx < C::kBoxes; ++bx)
-                        tma_load_4d(sQ + i * C::kTileBytes + bx * kBox, &tmQ, q_full, bx * 64, g * a.n_rep,
-                                    ((kPair ? 2 * mb : mb) + i) * a.seqs, 0);
+                        tma_load_4d(sQ + i * C::kTileBytes + bx * kBox, &tmQ, bar.q_full, bx * 64, g * a.n_rep,
+                                    (2 * mb + i) * a.seqs, 0);
                 for (int j = 0; j < n; ++j) {
                     const int stage = j % ST;
                     const uint32_t phase = ((j / ST) & 1) ^ 1;
@@ -155,78 +278,24 @@ __global__ void __launch_bounds__(kThreads, 1)
                     int blk, row;
                     kv_locate(a.lay, 0, (int64_t)(first + j) * kBN, blk, row);   // a bad entry reads block 0
                     const CUtensorMap* mv = first + j == a.n_tiles - 1 ? &tmVend : &tmV;
-                    if (!mbar_wait(&k_empty[stage], phase)) break;
-                    mbar_arrive_expect_tx(&k_full[stage], C::kTileBytes);
+                    if (!mbar_wait(&bar.k_empty[stage], phase)) break;
+                    mbar_arrive_expect_tx(&bar.k_full[stage], C::kTileBytes);
 #pragma unroll
                     for (int bx = 0; bx < C::kBoxes; ++bx)
-                        tma_load_4d(sk + bx * kBox, &tmK, &k_full[stage], bx * 64, row, g, blk);
-                    if (!mbar_wait(&v_empty[stage], phase)) break;
-                    mbar_arrive_expect_tx(&v_full[stage], C::kTileBytes);
+                        tma_load_4d(sk + bx * kBox, &tmK, &bar.k_full[stage], bx * 64, row, g, blk);
+                    if (!mbar_wait(&bar.v_empty[stage], phase)) break;
+                    mbar_arrive_expect_tx(&bar.v_full[stage], C::kTileBytes);
 #pragma unroll
                     for (int bx = 0; bx < C::kBoxes; ++bx)
-                        tma_load_4d(sv + bx * kBox, mv, &v_full[stage], bx * 64, row, g, blk);
+                        tma_load_4d(sv + bx * kBox, mv, &bar.v_full[stage], bx * 64, row, g, blk);
                 }
             }
-        } else if (warp == 1) {
-            // ------------------------------- MMA issuer -------------------------------
-            if (lane == 0) {
-                constexpr uint32_t idesc_s = idesc_bf16_f32(kBM, kBN, false);
-                constexpr uint32_t idesc_o = idesc_bf16_f32(kBM, D, true);
-                constexpr uint32_t desc_hi = smem_desc_hi_sw128(1024);
-                auto tile_of = [&](int i, int k) { return kPair ? k : 2 * k + i; };
-                auto issue_s = [&](int i, int j) {
-                    const uint32_t qd = smem_desc_lo(smem_u32(sQ + (kPair ? i : 0) * C::kTileBytes), 16);
-                    const uint32_t kd = smem_desc_lo(smem_u32(sKV + (j % ST) * 2 * C::kTileBytes), 16);
-#pragma unroll
-                    for (int ks = 0; ks < D / 16; ++ks) {
-                        const uint32_t off = (uint32_t)(((ks >> 2) * kBox + (ks & 3) * 32) >> 4);
-                        tc_mma_ss_w(tmem + col_s(i), qd + off, kd + off, desc_hi, idesc_s, ks > 0 ? 1u : 0u);
-                    }
-                    tc_commit(&s_full[i]);
-                };
-                // K tile j has been read by every product that needs it: free it if it will be refilled
-                auto free_k = [&](int j) { if (j + ST < n) tc_commit(&k_empty[j % ST]); };
-                bool alive = mbar_wait(q_full, 0);
-                for (int i = 0; i < 2 && alive; ++i) {
-                    if (steps[i] == 0) continue;
-                    const int j = tile_of(i, 0);
-                    if ((i == 0 || !kPair) && !mbar_wait(&k_full[j % ST], (j / ST) & 1)) { alive = false; break; }
-                    tc_fence_after();
-                    issue_s(i, j);
-                    if (!kPair || i == 1 || steps[1] == 0) free_k(j);
-                }
-                for (int k = 0; k < steps[0] && alive; ++k) {
-                    bool v_ready = false, k_ready = false;
-                    for (int i = 0; i < 2 && alive; ++i) {
-                        if (k >= steps[i]) continue;
-                        const int j = tile_of(i, k);
-                        if (!mbar_wait(&p_full[i], k & 1)) { alive = false; break; }
-                        if (!kPair || !v_ready) {
-                            if (!mbar_wait(&v_full[j % ST], (j / ST) & 1)) { alive = false; break; }
-                            v_ready = true;
-                        }
-                        tc_fence_after();
-                        const uint32_t vd = smem_desc_lo(smem_u32(sKV + (j % ST) * 2 * C::kTileBytes + C::kTileBytes), kBox);
-#pragma unroll
-                        for (int ks = 0; ks < kBN / 16; ++ks)
-                            tc_mma_ts_w(tmem + col_o(i), tmem + col_s(i) + ks * 8, vd + (uint32_t)((ks * 16 * 128) >> 4),
-                                        desc_hi, idesc_o, (k > 0 || ks > 0) ? 1u : 0u);
-                        const bool last_use = !kPair || i == 1 || steps[1] == 0;
-                        if (last_use && j + ST < n) tc_commit(&v_empty[j % ST]);
-                        if (k + 1 < steps[i]) {
-                            const int jn = tile_of(i, k + 1);
-                            if (!kPair || !k_ready) {
-                                if (!mbar_wait(&k_full[jn % ST], (jn / ST) & 1)) { alive = false; break; }
-                                tc_fence_after();
-                                k_ready = true;
-                            }
-                            issue_s(i, jn);   // overwrites P_i(k) only after the product above read it
-                            if (last_use) free_k(jn);
-                        } else {
-                            tc_commit(&o_done[i]);
-                        }
-                    }
-                }
+        } else if (warp == 1 && lane == 0) {
+            if constexpr (kPairs) {
+                if (pair) issue_products<D, kPairs, true>(sQ, sKV, bars, tmem, n);
+                else issue_products<D, kPairs, false>(sQ, sKV, bars, tmem, n);
+            } else {
+                issue_products<D, kPairs, false>(sQ, sKV, bars, tmem, n);
             }
         }
     } else {
@@ -235,7 +304,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int grp = (warp - 4) >> 2;
         const int quad = warp & 3;               // TMEM lane quadrant of this warp
         const int row = quad * 32 + lane;
-        const int qt = kPair ? 2 * mb + grp : mb;
+        const int qt = 2 * mb + (pair ? grp : 0);
         const int b = qt * a.seqs + row / a.n_rep;
         const bool valid = row < a.seqs * a.n_rep && b < a.B;
         const bool work = __any_sync(0xffffffffu, valid);   // a warp without a valid row only keeps the barriers going
@@ -247,10 +316,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         bool alive = true;
         const int ns = grp == 0 ? steps[0] : steps[1];
         for (int k = 0; k < ns; ++k) {
-            if (!mbar_wait(&s_full[grp], k & 1)) { alive = false; break; }
+            if (!mbar_wait(&bar.s_full[grp], k & 1)) { alive = false; break; }
             tc_fence_after();
             if (work) {
-                const int j = first + (kPair ? k : 2 * k + grp);
+                const int j = first + (pair ? k : 2 * k + grp);
                 float sv[kBN];
 #pragma unroll
                 for (int c = 0; c < kBN / 32; ++c)
@@ -313,32 +382,74 @@ __global__ void __launch_bounds__(kThreads, 1)
                 m_run = m_use;
             }
             tc_fence_before();
-            mbar_arrive(&p_full[grp]);
+            mbar_arrive(&bar.p_full[grp]);
         }
-        if (ns > 0 && alive && mbar_wait(&o_done[grp], 0) && work) {
+        alive = ns > 0 && alive && mbar_wait(&bar.o_done[grp], 0);
+        // Once both groups' products are complete, the tiles' memory is free for the result rows: scaled to their final
+        // weight when they are written there, so that joining two groups' rows is an addition.
+        float* s_rows = reinterpret_cast<float*>(smem);                       // [2][128][kRowFloats]
+        float* s_stat = s_rows + 2 * kBM * C::kRowFloats;                     // [2][128][2]: maximum and sum
+        float* my_stat = s_stat + (grp * kBM + row) * 2;
+        const int64_t base = (((int64_t)split * a.Hkv + g) * a.B + (int64_t)qt * a.seqs) * a.n_rep;   // row 0's part
+        const int rows = min(a.seqs, a.B - qt * a.seqs) * a.n_rep;            // valid rows of this query tile
+        if (!alive) l_run = 0.f;
+        my_stat[0] = l_run != 0.f ? m_run : -INFINITY;
+        my_stat[1] = l_run;
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (work) {
+            float f = l_run != 0.f ? 1.f / l_run : 0.f, lse = l_run != 0.f ? m_run + log2f(l_run) : -INFINITY;
+            if (!pair) {
+                const float2 other = *reinterpret_cast<const float2*>(s_stat + ((grp ^ 1) * kBM + row) * 2);
+                const float M = fmaxf(my_stat[0], other.x);
+                const float mine = l_run != 0.f ? ex2_approx(m_run - M) : 0.f;
+                const float L = l_run * mine + (other.y != 0.f ? other.y * ex2_approx(other.x - M) : 0.f);
+                f = mine != 0.f ? mine / L : 0.f;
+                lse = L != 0.f ? M + log2f(L) : -INFINITY;
+            }
+            if (valid && (pair || grp == 0)) a.part_lse[base + row] = lse;
+            float* dst = s_rows + (grp * kBM + row) * C::kRowFloats;
             tc_fence_after();
-            const float inv_l = l_run != 0.f ? 1.f / l_run : 0.f;
-            const int part = kPair ? split : 2 * split + grp;
-            const int64_t prow = (((int64_t)part * a.Hkv + g) * a.B + b) * a.n_rep + row % a.n_rep;
-            float* dst = a.part_o + prow * D;
 #pragma unroll
             for (int c = 0; c < D / 32; ++c) {
                 float o[32];
-                tmem_ld32(t_o + c * 32, o);
-                tmem_wait_ld();
-                if (valid) {
+                if (alive) {   // a group without a step has no O
+                    tmem_ld32(t_o + c * 32, o);
+                    tmem_wait_ld();
+                }
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4)
-                        *reinterpret_cast<float4*>(dst + c * 32 + i) =
-                            make_float4(o[i] * inv_l, o[i + 1] * inv_l, o[i + 2] * inv_l, o[i + 3] * inv_l);
+                for (int i = 0; i < 32; i += 4) {
+                    const bool any = f != 0.f;
+                    *reinterpret_cast<float4*>(dst + c * 32 + i) =
+                        any ? make_float4(o[i] * f, o[i + 1] * f, o[i + 2] * f, o[i + 3] * f) : make_float4(0.f, 0.f, 0.f, 0.f);
                 }
             }
-            if (valid) a.part_lse[prow] = l_run != 0.f ? m_run + log2f(l_run) : -INFINITY;
-        } else if (!kPair && ns == 0 && valid) {
-            // a stretch of one tile has no tile for the second group: an empty part
-            const int64_t prow = (((int64_t)(2 * split + grp) * a.Hkv + g) * a.B + b) * a.n_rep + row % a.n_rep;
-            for (int i = 0; i < D; i += 4) *reinterpret_cast<float4*>(a.part_o + prow * D + i) = make_float4(0.f, 0.f, 0.f, 0.f);
-            a.part_lse[prow] = -INFINITY;
+        }
+        constexpr int kLanes = D / 4;                 // lanes that move one row, 16 bytes each
+        constexpr int kRows = 32 / kLanes;            // rows a warp moves at a time
+        const int lr = lane / kLanes, d = lane % kLanes * 4;
+        float* part = a.part_o + base * D + d;
+        if (pair) {
+            __syncwarp();                             // a warp writes out the rows that it holds
+            const float* src = s_rows + grp * kBM * C::kRowFloats + d;
+#pragma unroll 8
+            for (int i = 0; i < 32; i += kRows) {
+                const int r = quad * 32 + i + lr;
+                if (r < rows)
+                    *reinterpret_cast<float4*>(part + (int64_t)r * D) =
+                        *reinterpret_cast<const float4*>(src + r * C::kRowFloats);
+            }
+        } else {
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            const float* src = s_rows + d;
+#pragma unroll 8
+            for (int i = 0; i < kBM; i += 8 * kRows) {
+                const int r = i + (warp - 4) * kRows + lr;
+                if (r < rows) {
+                    const float4 x = *reinterpret_cast<const float4*>(src + r * C::kRowFloats);
+                    const float4 y = *reinterpret_cast<const float4*>(src + (kBM + r) * C::kRowFloats);
+                    *reinterpret_cast<float4*>(part + (int64_t)r * D) = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
+                }
+            }
         }
     }
 
@@ -350,45 +461,35 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 }
 
-// The split of the prefix: query tiles of `seqs` sequences, pairs of them when one does not hold the batch, and as
-// many stretches as fill the SMs once.
+// Query tiles of `seqs` sequences, taken in pairs, and the most stretches they may be cut into.
 struct PrefixPlan {
-    int seqs, mblocks, splits, per, parts;
-    bool pair;
+    int seqs, pairs, single;
+    PrefixCut most;
 };
 
 PrefixPlan plan_prefix(int B, int Hkv, int n_rep, int prefix, int num_sms) {
-    PrefixPlan p;
+    PrefixPlan p = {};
     p.seqs = kBM / n_rep;
     const int q_tiles = (B + p.seqs - 1) / p.seqs;
-    p.pair = q_tiles > 1;
-    p.mblocks = p.pair ? (q_tiles + 1) / 2 : 1;
-    const int n_tiles = (prefix + kBN - 1) / kBN;
-    const int most = std::max(1, num_sms / (Hkv * p.mblocks));
-    p.per = (n_tiles + most - 1) / most;
-    p.splits = p.per ? (n_tiles + p.per - 1) / p.per : 0;
-    p.parts = p.pair ? p.splits : 2 * p.splits;
+    p.pairs = q_tiles / 2;
+    p.single = q_tiles % 2;
+    p.most = cut_prefix((prefix + kBN - 1) / kBN, std::max(1, num_sms / Hkv), p.pairs, p.single);
     return p;
 }
 
 constexpr int kMaxSms = 160;
 
 size_t shared_part_rows(int B, int H, int Hkv, int prefix) {
-    // parts of the prefix for the most SMs a GPU may have: more SMs never give fewer parts
+    // parts of the prefix: a block has no more stretches than SMs per kv head on the largest GPU, and than tiles
     const int n_rep = H / Hkv;
-    size_t parts = 0;
-    if (prefix > 0) {
-        const PrefixPlan p = plan_prefix(B, Hkv, n_rep, prefix, kMaxSms);
-        const int most = std::max(1, kMaxSms / (Hkv * p.mblocks));
-        parts = (size_t)(p.pair ? 1 : 2) * std::min(most, (prefix + kBN - 1) / kBN);
-    }
-    return (stream_part_rows(B, Hkv, true) + parts * Hkv * B) * n_rep;
+    const size_t parts = prefix > 0 ? std::min(std::max(1, kMaxSms / Hkv), (prefix + kBN - 1) / kBN) : 0;
+    return stream_part_rows(n_rep, B, Hkv, true) + parts * Hkv * B * n_rep;
 }
 
-template <int D, bool kPair>
-int launch_prefix_d(const PrefixArgs& a, const PrefixPlan& p, const CUtensorMap& tmQ, const CUtensorMap& tmK,
+template <int D, bool kPairs>
+int launch_prefix_d(const PrefixArgs& a, const StreamArgs& sa, const PrefixPlan& p, const CUtensorMap& tmQ, const CUtensorMap& tmK,
                     const CUtensorMap& tmV, const CUtensorMap& tmVend, cudaStream_t s) {
-    auto kern = prefix_kernel<D, kPair>;
+    auto kern = prefix_kernel<D, kPairs>;
     // setmaxnreg is only safe if the compiled kernel launches with the registers the split was sized for
     static int regs_ok = -1;
     if (regs_ok < 0) {
@@ -397,11 +498,12 @@ int launch_prefix_d(const PrefixArgs& a, const PrefixPlan& p, const CUtensorMap&
         regs_ok = (uint32_t)attr.numRegs >= kLaunchRegs ? MLLM_OK : MLLM_ERR_UNSUPPORTED;
     }
     if (regs_ok != MLLM_OK) return fail(regs_ok, "prefix_kernel: compiled with fewer registers than its split needs");
-    const int smem = PrefixCfg<D, kPair>::kSmemBytes;
+    const int smem = PrefixCfg<D, kPairs>::kSmemBytes;
     if (int st = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
                             "prefix_kernel smem attribute"))
         return st;
-    return check_cuda(launch_pdl(kern, dim3(a.Hkv * p.mblocks, p.splits), dim3(kThreads), smem, s, tmQ, tmK, tmV, tmVend, a),
+    return check_cuda(launch_pdl(kern, dim3(a.Hkv, p.pairs * p.most.splits + p.most.splits_single), dim3(kThreads), smem, s,
+                                 tmQ, tmK, tmV, tmVend, a, sa),
                       "prefix_kernel launch");
 }
 
@@ -418,7 +520,7 @@ extern "C" size_t mllm_decode_attention_shared_workspace_size(int batch, int num
     if (batch <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads || head_dim <= 0 ||
         prefix_len < 0 || num_heads / num_kv_heads > kMaxGroup)
         return 0;
-    return (shared_part_rows(batch, num_heads, num_kv_heads, prefix_len) * (size_t)(head_dim + 1) * 4 + 255) & ~size_t(255);
+    return stream_workspace_bytes(head_dim, shared_part_rows(batch, num_heads, num_kv_heads, prefix_len), batch, num_kv_heads);
 }
 
 extern "C" int mllm_decode_attention_shared_paged_bf16(const void* q, const mllm_paged_kv* kv, const int32_t* kv_lens,
@@ -464,9 +566,8 @@ extern "C" int mllm_decode_attention_shared_paged_bf16(const void* q, const mllm
     a.max_len = max_kv_len;
     a.scale_log2 = (float)((double)softmax_scale * 1.4426950408889634);
     a.first_row = prefix_len;
-    a.part_o = static_cast<float*>(workspace);
-    a.part_lse = a.part_o + shared_part_rows(batch, num_heads, num_kv_heads, prefix_len) * D;
-    a.prefix_base = (int64_t)stream_part_rows(batch, num_kv_heads, true) * n_rep;
+    stream_place(a, workspace, head_dim, shared_part_rows(batch, num_heads, num_kv_heads, prefix_len));
+    a.prefix_base = (int64_t)stream_part_rows(n_rep, batch, num_kv_heads, true);
     cudaStream_t s = (cudaStream_t)stream;
     if (prefix_len > 0) {
         const PrefixPlan p = plan_prefix(batch, num_kv_heads, n_rep, prefix_len, num_sms);
@@ -494,20 +595,21 @@ extern "C" int mllm_decode_attention_shared_paged_bf16(const void* q, const mllm
         pa.seqs = p.seqs;
         pa.prefix = prefix_len;
         pa.n_tiles = (prefix_len + kBN - 1) / kBN;
-        pa.per = p.per;
-        pa.mblocks = p.mblocks;
+        pa.pairs = p.pairs;
+        pa.single = p.single;
+        pa.num_sms = num_sms;
         pa.scale_log2 = a.scale_log2;
         pa.lay = a.lay;
+        a.pair_seqs = 2 * p.pairs * p.seqs;
+        a.shared = 1;
         int st;
         if (head_dim == 128)
-            st = p.pair ? launch_prefix_d<128, true>(pa, p, tmQ, tmK, tmV, tmVend, s)
-                        : launch_prefix_d<128, false>(pa, p, tmQ, tmK, tmV, tmVend, s);
+            st = p.pairs ? launch_prefix_d<128, true>(pa, a, p, tmQ, tmK, tmV, tmVend, s)
+                        : launch_prefix_d<128, false>(pa, a, p, tmQ, tmK, tmV, tmVend, s);
         else
-            st = p.pair ? launch_prefix_d<64, true>(pa, p, tmQ, tmK, tmV, tmVend, s)
-                        : launch_prefix_d<64, false>(pa, p, tmQ, tmK, tmV, tmVend, s);
+            st = p.pairs ? launch_prefix_d<64, true>(pa, a, p, tmQ, tmK, tmV, tmVend, s)
+                        : launch_prefix_d<64, false>(pa, a, p, tmQ, tmK, tmV, tmVend, s);
         if (st) return st;
-        a.prefix_parts = p.parts;
-        a.after_prefix = 1;
     }
     CUtensorMap tmK, tmV;
     if (int st = encode_kv_map(&tmK, kv->k_pool, D, kv->block_size, num_kv_heads, kv->num_blocks, kv->row_stride,

@@ -615,7 +615,7 @@ def _decode_kv8(q: torch.Tensor, kv_cache: PagedKVCache8, num_kv_heads: int, max
     device = q.device
     out = torch.empty((B, 1, H * D), dtype=BF16, device=device)
     # a workspace of the call's own, from torch's stream-ordered allocator (a captured graph's from its pool)
-    nbytes = abi.load().mllm_decode_attention_kv8_workspace_size(H, num_kv_heads, D)
+    nbytes = abi.load().mllm_decode_attention_kv8_workspace_size(B, H, num_kv_heads, D) if B else 256
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
     _launch(dev, "mllm_decode_attention_paged_kv8", q.data_ptr(), C.byref(kv_cache.descriptor()), kv_cache.lengths.data_ptr(),
             B, H, num_kv_heads, D, max_kv_len, 1.0 / math.sqrt(D), out.data_ptr(), ws.data_ptr(), nbytes)

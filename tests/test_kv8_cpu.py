@@ -112,8 +112,8 @@ def test_bad_arguments_are_refused(lib):
 
 def test_workspace_does_not_depend_on_lengths(lib):
     size = lib.mllm_decode_attention_kv8_workspace_size
-    assert size(32, 8, 128) >= 2 * 2 * 148 * 4 * (128 + 1) * 4 and size(32, 8, 128) % 256 == 0
-    assert size(8, 3, 128) == 0 and size(0, 8, 128) == 0
+    assert size(1, 32, 8, 128) >= 2 * 2 * 148 * 4 * (128 + 1) * 4 and size(64, 32, 8, 128) % 256 == 0
+    assert size(4, 8, 3, 128) == 0 and size(4, 0, 8, 128) == 0 and size(0, 32, 8, 128) == 0
 
 
 def test_python_checks():
