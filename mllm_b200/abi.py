@@ -168,10 +168,9 @@ def header_functions() -> list[str]:
 
 def call(name: str, *args) -> int:
     """Call an entry point and raise MllmError on a nonzero status."""
-    lib = load()
-    st = getattr(lib, name)(*args)
+    st = getattr(_lib or load(), name)(*args)
     if st != MLLM_OK:
-        raise MllmError(st, name, lib.mllm_attn_last_error().decode())
+        raise MllmError(st, name, _lib.mllm_attn_last_error().decode())
     return st
 
 

@@ -8,12 +8,16 @@ Cases (Qwen3-8B attention geometry: 32 q heads, 8 kv heads, head_dim 128, hidden
   decode     one query row per sequence over L cache rows, B sequences (decode_split_kernel)
   ragged     Qwen3-14B decode over 64 sequences of seeded lengths U[256, 32768], --kv-heads kv heads
              (5 q heads each): 8 is one GPU's share at 1 GPU, 1 at 8 GPUs
+  decode8    decode over an 8-bit cache (stream_decode_kernel)
+  shared     decode over --kv-len rows that B sequences share and --own rows of each (prefix_kernel, stream_decode_kernel)
+  epilogue8  QK-RMSNorm + RoPE + quantising append of B x S tokens (kv8_epilogue_stream_kernel)
+  logits     penalties, biases and a mask on B rows of Qwen3 logits (logit_rules_kernel)
   linear     q|k|v projection of T tokens, bf16 weights (linear_kernel)
   linear_fp8 the same with e4m3 weights and 128 x 128 block scales (linear_fp8_kernel)
 
 Prints one line: the case, its sizes and the mean milliseconds per launch over --iters launches
 (after --warmup).  Inputs are seeded random data; every launch goes through the C-ABI.  With --graph
-(the default for the projections, whose launches last about as long as a host call) the --iters
+(the default for the projections and the shorter calls, whose launches last about as long as a host call) the --iters
 launches are recorded once in a CUDA graph and the graph is timed."""
 import argparse
 import json
@@ -77,6 +81,74 @@ def _decode(args, dev, g):
     return launch, {"batch": B, "kv_len": L, "bytes": 2 * B * HKV * L * D * 2}
 
 
+def _cache8(B, rows, dev, g):
+    cache = rt.PagedKVCache8(B * -(-rows // 256), HKV, D, max_seqs=B, device=dev)
+    for pool in (cache.k_pool, cache.v_pool):
+        pool.view(torch.uint8).random_(0, 127, generator=g)       # positive finite e4m3 values
+    cache.k_exp.fill_(120)
+    cache.v_exp.fill_(120)
+    return cache
+
+
+def _decode8(args, dev, g):
+    B, L = args.batch, args.kv_len
+    cache = _cache8(B, L, dev, g)
+    cache.set_lengths([L] * B)
+    q = torch.randn(B, H, D, device=dev, generator=g).bfloat16()
+
+    def launch():
+        rt.decode_attention(q, cache, HKV, max_kv_len=L)
+    return launch, {"batch": B, "kv_len": L, "bytes": 2 * B * HKV * L * (D + 1)}
+
+
+def _shared(args, dev, g):
+    B, P, own = args.batch, args.kv_len, args.own
+    bs = 256
+    cache = rt.PagedKVCache(P // bs + B * (own // bs + 2) + 1, HKV, D, bs, max_seqs=B, device=dev)
+    cache.k_pool.normal_(generator=g)
+    cache.v_pool.normal_(generator=g)
+    cache.reserve(0, P)
+    for b in range(1, B):
+        cache.fork(0, b, P)
+    cache.set_lengths([P + own] * B)
+    q = torch.randn(B, H, D, device=dev, generator=g).bfloat16()
+
+    def launch():
+        rt.decode_attention_shared(q, cache, HKV, P)
+    return launch, {"batch": B, "prefix": P, "own": own, "bytes": 4 * HKV * D * (P + B * own),
+                    "flop": 4 * B * H * D * (P + own)}
+
+
+def _epilogue8(args, dev, g):
+    B, S = args.batch, args.seq
+    T, row = B * S, (H + 2 * HKV) * D
+    qkv = (torch.randn(T, row, device=dev, generator=g) * 0.5).bfloat16()
+    q, k, v = (qkv[:, a:b].view(T, -1, D) for a, b in ((0, H * D), (H * D, (H + HKV) * D), ((H + HKV) * D, row)))
+    gamma = (1 + 0.1 * torch.randn(D, device=dev, generator=g)).bfloat16()
+    cache = _cache8(B, S, dev, g)
+    cache.set_lengths([S] * B)
+    cu = torch.arange(0, T + 1, S, dtype=torch.int32, device=dev)
+    start = torch.zeros(B, dtype=torch.int32, device=dev)
+    pos = torch.arange(S, dtype=torch.int64, device=dev).repeat(B)
+
+    def launch():
+        rt.qkv_epilogue_kv8(q, k, v, cache, cu, start, pos, 1e6, q_norm_weight=gamma, k_norm_weight=gamma)
+    return launch, {"batch": B, "seq": S, "bytes": T * (row * 2 + H * D * 2 + 2 * HKV * (D + 1))}
+
+
+def _logits(args, dev, g):
+    B, V, n = args.batch, 151936, 2000
+    x = torch.randn(B, V, device=dev, generator=g)
+    hist = torch.randint(0, V, (B, n), device=dev, generator=g)
+    lens = torch.full((B,), n, dtype=torch.int32, device=dev)
+    one = torch.full((B,), 1.1, device=dev)
+    mask = torch.randint(-2**31, 2**31, (B, V // 32), device=dev, generator=g).int()
+
+    def launch():
+        rt.apply_logit_rules(x, history=hist, history_lens=lens, repetition=one, presence=one, frequency=one, allowed=mask)
+    return launch, {"rows": B, "bytes": 8 * B * V + B * V // 8 + 8 * B * n}
+
+
 def _ragged(args, dev, g):
     import numpy as np
     B, rep = 64, 5
@@ -119,12 +191,16 @@ def _linear(args, dev, g, fp8):
     return launch, {"tokens": T, "bytes": nbytes, "ring": len(ring)}
 
 
+_OPERATORS = {"decode8": _decode8, "shared": _shared, "epilogue8": _epilogue8, "logits": _logits}
+
+
 def main(argv=None):
     ap = argparse.ArgumentParser(description=__doc__.split("\n")[0])
-    ap.add_argument("case", choices=["epilogue", "prefill", "decode", "ragged", "linear", "linear_fp8"])
+    ap.add_argument("case", choices=["epilogue", "prefill", "decode", "ragged", "linear", "linear_fp8", *_OPERATORS])
     ap.add_argument("--batch", type=int, default=None)
     ap.add_argument("--seq", type=int, default=8192)
     ap.add_argument("--kv-len", type=int, default=4096)
+    ap.add_argument("--own", type=int, default=256, help="shared: rows of each sequence behind the prefix")
     ap.add_argument("--tokens", type=int, default=32)
     ap.add_argument("--kv-heads", type=int, default=1,
                     help="ragged: kv heads (Qwen3-14B has 8); epilogue: kv heads with --heads")
@@ -137,9 +213,9 @@ def main(argv=None):
                     help="time the launches as one CUDA graph (default: on for linear and linear_fp8)")
     args = ap.parse_args(argv)
     if args.graph is None:
-        args.graph = args.case in ("linear", "linear_fp8", "ragged")
+        args.graph = args.case in ("linear", "linear_fp8", "ragged", *_OPERATORS)
     if args.batch is None:
-        args.batch = 32 if args.case == "decode" else 4
+        args.batch = 32 if args.case in ("decode", "decode8", "shared", "logits") else 4
     if not torch.cuda.is_available():
         raise SystemExit("kernel_cases: needs a CUDA device")
     dev = torch.device("cuda", 0)
@@ -153,6 +229,8 @@ def main(argv=None):
         launch, info = _decode(args, dev, g)
     elif args.case == "ragged":
         launch, info = _ragged(args, dev, g)
+    elif args.case in _OPERATORS:
+        launch, info = _OPERATORS[args.case](args, dev, g)
     else:
         launch, info = _linear(args, dev, g, args.case == "linear_fp8")
     for _ in range(args.warmup):

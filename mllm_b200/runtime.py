@@ -20,6 +20,7 @@ tensors are required and anything else raises RuntimeError, like the reference's
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 
 import torch
@@ -150,6 +151,7 @@ class PagedKVCache:
     this is the serving-format step beyond it."""
 
     capture_max_len = None   # set while a CUDA graph of decode steps is captured (decode_step)
+    shared_prefix = 0        # rows that all the sequences of a decode step begin with (decode_step)
 
     def __init__(self, num_blocks: int, num_kv_heads: int, head_dim: int, block_size: int = 256,
                  max_seqs: int = 64, max_blocks_per_seq: int | None = None, device="cuda"):
@@ -493,18 +495,24 @@ def _capturing() -> bool:
 
 def _check_vec(name: str, t: torch.Tensor, n: int, dtype, dev: int) -> None:
     """A contiguous vector of exactly n elements on CUDA device number `dev`."""
-    if t.get_device() != dev or t.dtype is not dtype or t.dim() != 1 or t.size(0) != n or not t.is_contiguous():
+    if t.get_device() != dev or t.dtype is not dtype or t.shape != (n,) or not t.is_contiguous():
         raise RuntimeError(f"{name}: expected a contiguous {dtype} tensor of {n} elements on cuda:{dev}")
 
 
 def _launch(dev: int, name: str, *args) -> None:
     """abi.call with torch's current stream of device number `dev` as the last argument; the library launches on
     the current device, so `dev` is made that around the call if it is not."""
-    if dev == torch.cuda.current_device():
-        abi.call(name, *args, abi.stream_handle())
+    if dev == torch._C._cuda_getDevice():   # the callers hold CUDA tensors: CUDA is initialised
+        abi.call(name, *args, torch._C._cuda_getCurrentRawStream(dev) or None)
     else:
         with torch.cuda.device(dev):
             abi.call(name, *args, abi.stream_handle())
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_size(name: str, *sizes: int) -> int:
+    """Bytes a *_workspace_size entry point asks for (it depends on its arguments alone)."""
+    return getattr(abi.load(), name)(*sizes)
 
 
 def qkv_epilogue_kv8(q, k, v, kv_cache: PagedKVCache8, cu_seqlens: torch.Tensor, start: torch.Tensor, positions=None,
@@ -518,24 +526,28 @@ def qkv_epilogue_kv8(q, k, v, kv_cache: PagedKVCache8, cu_seqlens: torch.Tensor,
     (cos, sin) fp32 [T, D], or positions int64 [T] and rope_theta.  Returns Q [T, H, D] (rotated);
     `out` takes it in another layout.  The cache's lengths are the caller's to advance; the
     functions below do both."""
-    for n, t in (("q", q), ("k", k), ("v", v)):
-        _check_cuda_bf16(n, t)
-        if t.dim() != 3 or t.stride(2) != 1:
-            raise RuntimeError(f"Attention: {n} must be rank-3 [T, h, D] with D contiguous")
+    _check_cuda_bf16("q", q)
+    _check_cuda_bf16("k", k)
+    _check_cuda_bf16("v", v)
     if not isinstance(kv_cache, PagedKVCache8):
         raise RuntimeError("qkv_epilogue_kv8: needs a PagedKVCache8")
-    T, H, D = shape = q.shape
+    shape, kv_shape, pool = q.shape, k.shape, kv_cache.k_pool
+    q_stride, k_stride, v_stride = q.stride(), k.stride(), v.stride()
+    if len(shape) != 3 or len(kv_shape) != 3 or v.shape != kv_shape or \
+            q_stride[2] != 1 or k_stride[2] != 1 or v_stride[2] != 1:
+        raise RuntimeError("Attention: q, k and v must be rank-3 [T, h, D] with D contiguous")
+    T, H, D = shape
     dev = q.get_device()
-    pool = kv_cache.k_pool
-    if k.shape != v.shape or k.size(0) != T or k.size(2) != D:
+    Hkv = kv_shape[1]
+    if kv_shape[0] != T or kv_shape[2] != D:
         raise RuntimeError("Attention: k and v must be [T, num_kv_heads, D] for q's T and D")
-    Hkv = k.size(1)
-    if pool.size(1) != Hkv or pool.size(3) != D:
+    pool_shape = pool.shape
+    if pool_shape[1] != Hkv or pool_shape[3] != D:
         raise RuntimeError("Attention: the cache has other kv heads or another head_dim")
     if k.get_device() != dev or v.get_device() != dev or pool.get_device() != dev:
         raise RuntimeError("Attention: q, k, v and the cache must be on one device")
     n = start.numel()
-    if n > kv_cache.block_table.size(0):
+    if n > kv_cache.block_table.shape[0]:
         raise RuntimeError("Attention: more sequences than the cache has rows for")
     _check_vec("cu_seqlens", cu_seqlens, n + 1, torch.int32, dev)
     _check_vec("start", start, n, torch.int32, dev)
@@ -555,21 +567,19 @@ def qkv_epilogue_kv8(q, k, v, kv_cache: PagedKVCache8, cu_seqlens: torch.Tensor,
         raise RuntimeError("Attention: give both q/k norm weights or neither")
     qn = kn = None
     if q_norm_weight is not None:
-        qn, kn = (w if w.dtype is BF16 and w.is_contiguous() else w.to(BF16).contiguous()
-                  for w in (q_norm_weight, k_norm_weight))
+        qn, kn = q_norm_weight, k_norm_weight
+        if qn.dtype is not BF16 or kn.dtype is not BF16 or not qn.is_contiguous() or not kn.is_contiguous():
+            qn, kn = qn.to(BF16).contiguous(), kn.to(BF16).contiguous()
         _check_vec("q_norm_weight", qn, D, BF16, dev)
         _check_vec("k_norm_weight", kn, D, BF16, dev)
     if out is None:
         out = torch.empty(shape, dtype=BF16, device=q.device)
     elif out.shape != shape or out.dtype is not BF16 or out.get_device() != dev or out.stride(2) != 1:
         raise RuntimeError("Attention: out must be bf16 [T, H, D] with D contiguous on q's device")
-    q_st, q_sh, _ = q.stride()
-    k_st, k_sh, _ = k.stride()
-    v_st, v_sh, _ = v.stride()
-    o_st, o_sh, _ = out.stride()
-    _launch(dev, "mllm_qkv_epilogue_varlen_paged_kv8", q.data_ptr(), q_st, q_sh, k.data_ptr(), k_st, k_sh, v.data_ptr(), v_st,
-            v_sh, T, H, Hkv, D, pos, float(rope_theta), cos, sin, _ptr(qn), _ptr(kn), float(eps), out.data_ptr(), o_st, o_sh,
-            C.byref(kv_cache.descriptor()), cu_seqlens.data_ptr(), n, start.data_ptr())
+    out_stride = out.stride()
+    _launch(dev, "mllm_qkv_epilogue_varlen_paged_kv8", q.data_ptr(), q_stride[0], q_stride[1], k.data_ptr(), k_stride[0],
+            k_stride[1], v.data_ptr(), v_stride[0], v_stride[1], T, H, Hkv, D, pos, rope_theta, cos, sin, _ptr(qn), _ptr(kn),
+            eps, out.data_ptr(), out_stride[0], out_stride[1], C.byref(kv_cache.descriptor()), cu_seqlens.data_ptr(), n, start.data_ptr())
     return out
 
 
@@ -615,7 +625,7 @@ def _decode_kv8(q: torch.Tensor, kv_cache: PagedKVCache8, num_kv_heads: int, max
     device = q.device
     out = torch.empty((B, 1, H * D), dtype=BF16, device=device)
     # a workspace of the call's own, from torch's stream-ordered allocator (a captured graph's from its pool)
-    nbytes = abi.load().mllm_decode_attention_kv8_workspace_size(B, H, num_kv_heads, D) if B else 256
+    nbytes = _workspace_size("mllm_decode_attention_kv8_workspace_size", B, H, num_kv_heads, D)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
     _launch(dev, "mllm_decode_attention_paged_kv8", q.data_ptr(), C.byref(kv_cache.descriptor()), kv_cache.lengths.data_ptr(),
             B, H, num_kv_heads, D, max_kv_len, 1.0 / math.sqrt(D), out.data_ptr(), ws.data_ptr(), nbytes)
@@ -893,7 +903,7 @@ def decode_attention_shared(q: torch.Tensor, kv_cache: PagedKVCache, num_kv_head
     L = max(min(L, kv_cache.capacity), 1)
     out = torch.empty((B, 1, H * D), dtype=BF16, device=q.device)
     # a workspace of the call's own, from torch's stream-ordered allocator (a captured graph's from its pool)
-    nbytes = abi.load().mllm_decode_attention_shared_workspace_size(B, H, num_kv_heads, D, prefix_len)
+    nbytes = _workspace_size("mllm_decode_attention_shared_workspace_size", B, H, num_kv_heads, D, prefix_len)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
     _launch(dev, "mllm_decode_attention_shared_paged_bf16", qq.data_ptr(), C.byref(kv_cache.descriptor()),
             kv_cache.lengths.data_ptr(), prefix_len, B, H, num_kv_heads, D, L, 1.0 / math.sqrt(D), out.data_ptr(),
@@ -921,12 +931,47 @@ def _decode_step_kv8(q, k, v, cache: PagedKVCache8, positions, rope_theta, num_k
     return _decode_kv8(q_rot, cache, num_kv_heads, min(L, cache.capacity))
 
 
+def _decode_step_shared(q, k, v, cache: PagedKVCache, positions, rope_theta, num_kv_heads, qn, kn, eps, rope_table):
+    """decode_step over a cache whose sequences share their first rows: the epilogue appends at the device lengths,
+    which then advance, and the attention reads the prefix once."""
+    B, H, _, D = q.shape
+    capturing = _capturing()
+    if capturing and cache.capture_max_len is None:
+        raise RuntimeError("decode_step: set the cache's capture_max_len before capturing a graph")
+    if not capturing:   # raises before any launch if the pool is full
+        for b in range(B):
+            cache.reserve(b, cache.host_lengths()[b] + 1)
+    pos = positions.to(torch.int64).reshape(-1)
+    cos = sin = None
+    rsb = 0
+    if rope_table is not None:
+        cos, sin = (t.to(torch.float32).contiguous() for t in rope_table)
+        rsb = 0 if cos.shape[0] == 1 else 1
+    if qn is not None:
+        qn, kn = qn.to(BF16).contiguous(), kn.to(BF16).contiguous()
+    q_rot = torch.empty((B, H, D), dtype=BF16, device=q.device)
+    kv = cache.descriptor()
+    abi.call("mllm_qkv_epilogue_paged_bf16", _ptr(q), q.stride(0), q.stride(2), q.stride(1), _ptr(k), k.stride(0),
+             k.stride(2), k.stride(1), _ptr(v), v.stride(0), v.stride(2), v.stride(1), B, 1, H, num_kv_heads, D, _ptr(pos),
+             0 if pos.numel() == 1 else pos.stride(0), 0, float(rope_theta), _ptr(cos), _ptr(sin), rsb, 0, _ptr(qn),
+             _ptr(kn), float(eps), _ptr(q_rot), C.byref(kv), _ptr(cache.lengths), 0, abi.stream_handle())
+    if capturing:
+        cache.lengths[:B] += 1
+        L = cache.capture_max_len
+    else:
+        cache.advance(1, batch=B)
+        L = max(cache.host_lengths()[:B])
+    return decode_attention_shared(q_rot, cache, num_kv_heads, cache.shared_prefix, min(L, cache.capacity))
+
+
 def decode_step(q, k, v, kv_cache: KVCache, positions: torch.Tensor, rope_theta: float, num_kv_heads: int,
                 q_norm_weight=None, k_norm_weight=None, eps: float = 1e-6, rope_table=None) -> torch.Tensor:
     """One new token per sequence through the fused step: QK-RMSNorm (optional) + RoPE + KV
     append + decode attention in one launch.  q [B,H,1,D], k/v [B,Hkv,1,D] (strided views of the
     projections); positions int64 [1] (shared) or [B] / [B, 1].  The new rows go to slot
-    lengths[b] of each sequence and the lengths advance by one.  Returns [B, 1, H*D]."""
+    lengths[b] of each sequence and the lengths advance by one.  Returns [B, 1, H*D].  A paged cache
+    whose shared_prefix is set (every sequence begins with that many equal rows) is read by
+    decode_attention_shared, after an epilogue launch of its own."""
     for n, t in (("q", q), ("k", k), ("v", v)):
         _check_cuda_bf16(n, t)
         if t.dim() != 4 or t.size(2) != 1 or t.stride(3) != 1:
@@ -937,6 +982,9 @@ def decode_step(q, k, v, kv_cache: KVCache, positions: torch.Tensor, rope_theta:
     if isinstance(kv_cache, PagedKVCache8):
         return _decode_step_kv8(q, k, v, kv_cache, positions, rope_theta, num_kv_heads, q_norm_weight, k_norm_weight,
                                 eps, rope_table)
+    if isinstance(kv_cache, PagedKVCache) and kv_cache.shared_prefix > 0:
+        return _decode_step_shared(q, k, v, kv_cache, positions, rope_theta, num_kv_heads, q_norm_weight, k_norm_weight,
+                                   eps, rope_table)
     pos = positions.to(torch.int64).reshape(-1)
     pos_sb = 0 if pos.numel() == 1 else pos.stride(0)
     cos = sin = None
@@ -999,6 +1047,9 @@ def _rows_args(t: torch.Tensor | None):
         return None, 0, 0
     n = t.size(1)
     return t.data_ptr(), max(t.stride(0), n), n
+
+
+MAX_LOGIT_BIASES = 1024
 
 
 def apply_logit_rules(logits: torch.Tensor, history=None, history_lens=None, output_start=None, repetition=None,

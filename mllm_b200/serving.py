@@ -16,7 +16,13 @@ a time (Scheduler.cpp:45-77).  Here requests of any length share the GPU:
   * the next tokens of all live rows come from one device sampler call (`mllm_sample`) and one
     device-to-host read per step;
   * while the batch keeps its size, the decode step replays a CUDA graph recorded for that size
-    (`DecodeGraph`): one launch per step instead of several hundred.
+    (`DecodeGraph`): one launch per step instead of several hundred;
+  * a prefix that every request begins with (a system prompt) is prefilled once; the requests share
+    its blocks (`PagedKVCache.fork`) and the decode step reads it once for the whole batch
+    (`mllm_decode_attention_shared_paged_bf16`);
+  * a request may carry `LogitRules`: penalties, biases and a mask of allowed tokens, applied to its
+    row of logits on the device (`mllm_logit_rules`) before the token is picked;
+  * with kv8 the caches hold 8-bit rows (`runtime.PagedKVCache8`).
 
 `DecoderModel` is the layer stack of TransformerBlock::Forward (TransformerBlock.h:51-195) with
 the reference's RMSNorm (RMSNorm.h:27-64) and SwiGLU MLP (MLP.h:31-43) as LibTorch ops, the
@@ -25,8 +31,11 @@ and lm_head (QwenRunner.cpp:285-418).  Its weights are random (there is no check
 """
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass, field
+from typing import Callable
 
+import numpy as np
 import torch
 
 from . import runtime as rt
@@ -64,10 +73,12 @@ class DecoderShape:
 class DecoderModel:
     """Random-init decoder (Qwen3 or Llama layout) whose attention step runs on the B200 path."""
 
-    def __init__(self, shape: DecoderShape, seed: int = 0, device="cuda", fp8: bool = False):
+    def __init__(self, shape: DecoderShape, seed: int = 0, device="cuda", fp8: bool = False, kv8: bool = False):
         """fp8: every projection (q/k/v/o and the MLP) held as e4m3 with 128 x 128 block scales,
-        the layout of FP8 checkpoints, and multiplied as stored (runtime.linear_fp8)."""
+        the layout of FP8 checkpoints, and multiplied as stored (runtime.linear_fp8).  kv8: the
+        caches it makes hold 8-bit rows."""
         self.s = shape
+        self.kv8 = kv8
         g = torch.Generator(device=device).manual_seed(seed)
         E, H, Hkv, D, I = shape.hidden, shape.heads, shape.kv_heads, shape.head_dim, shape.intermediate
 
@@ -103,8 +114,9 @@ class DecoderModel:
 
     def new_caches(self, num_blocks: int, block_size: int = 256, max_seqs: int = 64,
                    max_blocks_per_seq: int | None = None):
-        return [rt.PagedKVCache(num_blocks, self.s.kv_heads, self.s.head_dim, block_size, max_seqs,
-                                max_blocks_per_seq, device=self.embed.device) for _ in self.layers]
+        cls = rt.PagedKVCache8 if self.kv8 else rt.PagedKVCache
+        return [cls(num_blocks, self.s.kv_heads, self.s.head_dim, block_size, max_seqs, max_blocks_per_seq,
+                    device=self.embed.device) for _ in self.layers]
 
     def forward(self, ids: torch.Tensor, positions: torch.Tensor, caches) -> torch.Tensor:
         """ids int64 [B, S]; positions int64 [S] (shared) or [B] (one new token per sequence);
@@ -175,28 +187,90 @@ class DecodeGraph:
 
 
 @dataclass
+class LogitRules:
+    """What restricts a request's next token (runtime.apply_logit_rules): the repetition penalty counts
+    prefix, prompt and generated tokens, presence and frequency the generated ones; `bias` adds to
+    tokens; `allowed(tokens)` gives, for the tokens generated so far, a truth value per token of the
+    vocabulary (a grammar's next tokens), or None for no restriction."""
+    repetition: float = 1.0
+    presence: float = 0.0
+    frequency: float = 0.0
+    bias: dict[int, float] = field(default_factory=dict)
+    allowed: Callable | None = None
+
+    def __post_init__(self):
+        if not (self.repetition > 0 and all(math.isfinite(x) for x in (self.repetition, self.presence, self.frequency))):
+            raise ValueError("LogitRules: penalties must be finite and repetition positive")
+        if len(self.bias) > rt.MAX_LOGIT_BIASES:
+            raise ValueError(f"LogitRules: at most {rt.MAX_LOGIT_BIASES} biases")
+
+
+def _pack_mask(allow, vocab: int) -> np.ndarray:
+    """A truth value per token as the 32-bit words apply_logit_rules reads."""
+    allow = np.asarray(allow, dtype=bool)
+    if allow.shape != (vocab,):
+        raise ValueError("LogitRules: allowed must give one truth value per token of the vocabulary")
+    return np.packbits(np.pad(allow, (0, -vocab % 32)), bitorder="little").view(np.int32)
+
+
+def apply_rules(logits: torch.Tensor, rules: list, prompts: list[list[int]], generated: list[list[int]]) -> torch.Tensor:
+    """`logits` [B, vocab] with every row's rules (None: none) applied; the row's history is its prompt
+    and generated tokens."""
+    B, V = logits.shape
+    if len(rules) != B or len(prompts) != B or len(generated) != B:
+        raise ValueError("apply_rules: one entry per row of logits")
+    dev = logits.device
+    given = [r or LogitRules() for r in rules]
+    hist = [list(p) + list(t) if r else [] for r, p, t in zip(rules, prompts, generated)]
+    up = lambda x, dt: torch.tensor(x, dtype=dt).to(dev, non_blocking=True)
+    kw = {}
+    n = max((len(h) for h in hist), default=0)
+    if n:
+        kw.update(history=up([h + [-1] * (n - len(h)) for h in hist], torch.int64),
+                  history_lens=up([len(h) for h in hist], torch.int32),
+                  output_start=up([len(p) for p in prompts], torch.int32),
+                  repetition=up([r.repetition for r in given], torch.float32),
+                  presence=up([r.presence for r in given], torch.float32),
+                  frequency=up([r.frequency for r in given], torch.float32))
+    m = max((len(r.bias) for r in given), default=0)
+    if m:
+        kw.update(bias_ids=up([list(r.bias) + [-1] * (m - len(r.bias)) for r in given], torch.int64),
+                  bias_values=up([list(r.bias.values()) + [0.0] * (m - len(r.bias)) for r in given], torch.float32),
+                  bias_lens=up([len(r.bias) for r in given], torch.int32))
+    masks = [r.allowed(list(t)) if r.allowed else None for r, t in zip(given, generated)]
+    if any(k is not None for k in masks):
+        words = np.stack([np.full((V + 31) // 32, -1, np.int32) if k is None else _pack_mask(k, V) for k in masks])
+        kw["allowed"] = torch.from_numpy(words).to(dev, non_blocking=True)
+    return rt.apply_logit_rules(logits, **kw)
+
+
+@dataclass
 class Request:
     rid: int
-    prompt: list[int]
+    prompt: list[int]                 # behind the batcher's prefix, if it has one
     max_new_tokens: int
     eos: int | None = None
+    rules: LogitRules | None = None
     tokens: list[int] = field(default_factory=list)
     logits: list[torch.Tensor] = field(default_factory=list)   # kept when record_logits is set
 
     @property
     def rows(self) -> int:
-        """Cache rows the request can need: prompt plus generated tokens (the last one is never fed)."""
+        """Cache rows the request can need behind the prefix: prompt plus generated tokens (the last
+        one is never fed)."""
         return len(self.prompt) + self.max_new_tokens
 
 
 class ContinuousBatcher:
     """Greedy batched generation with requests joining and leaving between steps (see the module
     docstring).  `model` provides forward(ids, positions, caches) -> [B, vocab] logits and
-    new_caches(num_blocks, block_size, max_seqs, max_blocks_per_seq)."""
+    new_caches(num_blocks, block_size, max_seqs, max_blocks_per_seq).  `prefix`: tokens that every
+    request begins with; they are prefilled once, into a row of their own, whose blocks the requests
+    share."""
 
     def __init__(self, model, max_batch: int, num_blocks: int, block_size: int = 256,
                  max_blocks_per_seq: int | None = None, record_logits: bool = False, graphs: bool = True,
-                 max_graphs: int = 8):
+                 max_graphs: int = 8, prefix: list[int] | None = None):
         self.model = model
         # CUDA graphs of the decode step, one per batch size, recorded when a size repeats
         emb = getattr(model, "embed", None)
@@ -206,7 +280,8 @@ class ContinuousBatcher:
         self._last_n = 0
         self.graph_steps = 0   # decode steps that replayed a recorded graph
         self.max_batch = max_batch
-        self.caches = model.new_caches(num_blocks, block_size, max_batch, max_blocks_per_seq)
+        self.prefix = list(prefix or [])
+        self.caches = model.new_caches(num_blocks, block_size, max_batch + (1 if self.prefix else 0), max_blocks_per_seq)
         self.block_size = block_size
         self.record_logits = record_logits
         self.waiting: list[Request] = []
@@ -214,19 +289,40 @@ class ContinuousBatcher:
         self.done: dict[int, Request] = {}
         self._next_id = 0
         self.steps = 0
+        if self.prefix:
+            row = max_batch                    # behind the live rows, for as long as the batcher lives
+            views = [c.slot(row) for c in self.caches]
+            ids = torch.tensor(self.prefix, dtype=torch.int64, device=self._device())
+            if hasattr(model, "forward_packed"):
+                model.forward_packed(ids, [len(self.prefix)], views)
+            else:
+                model.forward(ids.view(1, -1), torch.arange(len(self.prefix), device=ids.device), views)
+            for c in self.caches:
+                c.shared_prefix = len(self.prefix)
 
-    def submit(self, prompt, max_new_tokens: int, eos: int | None = None) -> int:
+    def _device(self):
+        return self.model.embed.device if hasattr(self.model, "embed") else "cpu"
+
+    def _blocks_needed(self, r: Request) -> int:
+        """Blocks a request takes from the pool: those of its rows, but for the prefix's full ones."""
+        return -(-(len(self.prefix) + r.rows) // self.block_size) - len(self.prefix) // self.block_size
+
+    def submit(self, prompt, max_new_tokens: int, eos: int | None = None, rules: LogitRules | None = None) -> int:
         if len(prompt) == 0 or max_new_tokens < 1:
             raise ValueError("a request needs a prompt and at least one new token")
-        r = Request(self._next_id, list(prompt), max_new_tokens, eos)
-        need = -(-r.rows // self.block_size)
-        if need > self.caches[0].max_blocks_per_seq or need > self.caches[0].num_blocks:
+        r = Request(self._next_id, list(prompt), max_new_tokens, eos, rules)
+        held = -(-len(self.prefix) // self.block_size)
+        if -(-(len(self.prefix) + r.rows) // self.block_size) > self.caches[0].max_blocks_per_seq or \
+                self._blocks_needed(r) + held > self.caches[0].num_blocks:
             raise ValueError("request longer than one sequence's cache can hold")
         self._next_id += 1
         self.waiting.append(r)
         return r.rid
 
-    def _pick(self, logits: torch.Tensor) -> list[int]:
+    def _pick(self, logits: torch.Tensor, requests: list[Request]) -> list[int]:
+        if any(r.rules for r in requests):
+            logits = apply_rules(logits, [r.rules for r in requests], [self.prefix + r.prompt for r in requests],
+                                 [r.tokens for r in requests])
         if logits.is_cuda:
             return rt.sample(logits, use_greedy=True).tolist()
         return logits.argmax(-1).tolist()
@@ -240,18 +336,20 @@ class ContinuousBatcher:
         return len(r.tokens) >= r.max_new_tokens or (r.eos is not None and r.tokens and r.tokens[-1] == r.eos)
 
     def _admit(self) -> None:
-        dev = self.model.embed.device if hasattr(self.model, "embed") else "cpu"
+        dev = self._device()
         first = len(self.live)
         joined: list[Request] = []
         while self.waiting and first + len(joined) < self.max_batch:
             r = self.waiting[0]
-            need = -(-r.rows // self.block_size)
+            need = self._blocks_needed(r)
             if any(c.free_blocks < need for c in self.caches):
                 break                        # first come, first served: wait for blocks
             self.waiting.pop(0)
             row = first + len(joined)
             for c in self.caches:
-                c.reserve(row, r.rows)       # the whole request's blocks, up front
+                if self.prefix:
+                    c.fork(self.max_batch, row, len(self.prefix))
+                c.reserve(row, len(self.prefix) + r.rows)       # the whole request's blocks, up front
             joined.append(r)
         if not joined:
             return
@@ -265,10 +363,10 @@ class ContinuousBatcher:
             for i, r in enumerate(joined):
                 views = [c.slot(first + i) for c in self.caches]
                 ids = torch.tensor([r.prompt], dtype=torch.int64, device=dev)
-                pos = torch.arange(len(r.prompt), dtype=torch.int64, device=dev)
+                pos = torch.arange(len(r.prompt), dtype=torch.int64, device=dev) + len(self.prefix)
                 rows.append(self.model.forward(ids, pos, views))
             logits = torch.cat(rows)
-        for r, t, row in zip(joined, self._pick(logits), logits):
+        for r, t, row in zip(joined, self._pick(logits, joined), logits):
             self._emit(r, t, row)
             self.live.append(r)
 
@@ -296,7 +394,7 @@ class ContinuousBatcher:
         self._retire()                       # a request may finish with its first token
         if not self.live:
             return
-        dev = self.model.embed.device if hasattr(self.model, "embed") else "cpu"
+        dev = self._device()
         n = len(self.live)
         ids = torch.tensor([[r.tokens[-1]] for r in self.live], dtype=torch.int64, device=dev)
         lens = self.caches[0].host_lengths()[:n]
@@ -309,7 +407,7 @@ class ContinuousBatcher:
             self.graph_steps += 1
         else:
             logits = self.model.forward(ids, pos, self.caches)
-        for r, t, row in zip(self.live, self._pick(logits), logits):
+        for r, t, row in zip(self.live, self._pick(logits, self.live), logits):
             self._emit(r, t, row)
         self.steps += 1
 
@@ -320,7 +418,7 @@ class ContinuousBatcher:
             return None
         repeat, self._last_n = self._last_n == n, n
         # every live row stays below its request's rows; round up so that one graph serves a while
-        need = max(r.rows for r in self.live)
+        need = len(self.prefix) + max(r.rows for r in self.live)
         bound = min(-(-need // 256) * 256, self.caches[0].capacity)
         g = self._graphs.get(n)
         if g is not None and g.max_len >= need:

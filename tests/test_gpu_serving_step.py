@@ -1,0 +1,115 @@
+"""The serving step with its newer parts in place: a prefix that the batch shares, 8-bit caches and per-request
+rules, alone and together, through the continuous batcher.  Needs a B200."""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+if not torch.cuda.is_available():
+    pytest.skip("needs a GPU", allow_module_level=True)
+
+from mllm_b200 import abi  # noqa: E402
+from mllm_b200.serving import ContinuousBatcher, DecoderModel, DecoderShape, LogitRules, apply_rules  # noqa: E402
+from tests.test_gpu_serving import _solo_logits  # noqa: E402
+
+SHAPE = DecoderShape(vocab=2048, hidden=1024, layers=3, heads=8, kv_heads=2, head_dim=128, intermediate=2048)
+
+
+def _run(model, prompts, news, **kw):
+    bat = ContinuousBatcher(model, max_batch=3, num_blocks=24, block_size=128, record_logits=True, **kw)
+    free = bat.caches[0].free_blocks
+    ids = [bat.submit(p, n) for p, n in zip(prompts, news)]
+    out = bat.run()
+    assert all(c.free_blocks == free for c in bat.caches)
+    abi.call("mllm_attn_device_status", None)
+    return [out[i] for i in ids], [torch.stack(bat.done[i].logits) for i in ids], bat
+
+
+@pytest.mark.parametrize("graphs", [False, True])
+@pytest.mark.parametrize("plen", [1, 128, 300])
+def test_shared_prefix_matches_solo_runs(plen, graphs):
+    """As the batcher without a prefix is tested: against each request alone, prefix and prompt in one contiguous cache,
+    within 0.03 of the largest logit (bf16 through three layers), and the greedy token where the margin is clear."""
+    model = DecoderModel(SHAPE, seed=3)
+    rng = np.random.default_rng(plen)
+    prefix = rng.integers(0, SHAPE.vocab, plen).tolist()
+    prompts = [rng.integers(0, SHAPE.vocab, n).tolist() for n in (5, 130, 37, 1, 64)]
+    toks, logits, bat = _run(model, prompts, [12, 5, 20, 16, 10], prefix=prefix, graphs=graphs)
+    assert (bat.graph_steps > 5) == graphs
+    agree = total = 0
+    for p, t, got in zip(prompts, toks, logits):
+        ref = _solo_logits(model, prefix + p, t)
+        scale = ref.abs().max().item()
+        np.testing.assert_allclose(got.numpy(), ref.numpy(), atol=0.03 * scale, rtol=0)
+        top2 = ref.topk(2, dim=-1).values
+        clear = (top2[:, 0] - top2[:, 1]) > 0.02 * scale
+        agree += int((ref.argmax(-1) == torch.tensor(t))[clear].sum())
+        total += int(clear.sum())
+    assert total > 0 and agree == total
+
+
+@pytest.mark.parametrize("prefix_len", [0, 200])
+def test_8bit_caches_batched_and_alone(prefix_len):
+    """8-bit caches: requests side by side (steps from graphs) against one at a time, eager.  Another order of additions in
+    the projections can move a cached element by one e4m3 step, so up to the first token that differs (a near-tie)
+    the logits agree to the same 0.03 of the largest."""
+    model = DecoderModel(SHAPE, seed=4, kv8=True)
+    rng = np.random.default_rng(1)
+    prefix = rng.integers(0, SHAPE.vocab, prefix_len).tolist()
+    prompts = [rng.integers(0, SHAPE.vocab, n).tolist() for n in (20, 200, 3, 129, 64)]
+    news = [20, 15, 25, 12, 18]
+    toks, logits, bat = _run(model, prompts, news, prefix=prefix)
+    assert bat.graph_steps > 5
+    compared = 0
+    for p, n, t, got in zip(prompts, news, toks, logits):
+        solo_t, solo_l, _ = _run(model, [p], [n], prefix=prefix, graphs=False)
+        scale = solo_l[0].abs().max().item()
+        for k in range(n):
+            np.testing.assert_allclose(got[k].numpy(), solo_l[0][k].numpy(), atol=0.03 * scale, rtol=0)
+            compared += 1
+            if t[k] != solo_t[0][k]:
+                top2 = solo_l[0][k].topk(2).values
+                assert float(top2[0] - top2[1]) < 0.03 * scale
+                break
+    assert compared > 50
+
+
+@pytest.mark.parametrize("kv8,prefix_len", [(False, 0), (True, 150), (False, 150)])
+def test_rules_hold_for_their_request_only(kv8, prefix_len):
+    """A grammar, penalties and biases on some of the requests: the picked tokens are the greedy ones of the recorded
+    logits under the rules computed in 64 bits; requests without rules pick the plain greedy token."""
+    model = DecoderModel(SHAPE, seed=6, kv8=kv8)
+    rng = np.random.default_rng(2)
+    prefix = rng.integers(0, SHAPE.vocab, prefix_len).tolist()
+
+    def even_then_odd(tokens):
+        return (np.arange(SHAPE.vocab) + len(tokens)) % 2 == 0
+    rules = [None, LogitRules(allowed=even_then_odd), LogitRules(repetition=1.7, presence=0.5, frequency=0.25),
+             LogitRules(bias={7: 50.0, 8: -5.0}), LogitRules(repetition=1.2, frequency=1.0, bias={9: 1.0}, allowed=even_then_odd)]
+    bat = ContinuousBatcher(model, max_batch=3, num_blocks=24, block_size=128, record_logits=True, prefix=prefix)
+    prompts = [rng.integers(0, SHAPE.vocab, n).tolist() for n in (20, 100, 3, 64, 7)]
+    ids = [bat.submit(p, 14, rules=r) for p, r in zip(prompts, rules)]
+    bat.run()
+    abi.call("mllm_attn_device_status", None)
+    for i, p, r in zip(ids, prompts, rules):
+        req = bat.done[i]
+        for k, (t, row) in enumerate(zip(req.tokens, req.logits)):
+            x = row.double().numpy().copy()
+            if r is not None:
+                made = req.tokens[:k]
+                for v in set(prefix + p + made):
+                    x[v] = x[v] * r.repetition if x[v] < 0 else x[v] / r.repetition
+                    x[v] -= made.count(v) * r.frequency + (v in made) * r.presence
+                for v, b in r.bias.items():
+                    x[v] += b
+                if r.allowed:
+                    x[~r.allowed(made)] = -np.inf
+            # fp32 arithmetic on numbers below 100: six steps of 2^-24
+            assert x[t] >= x.max() - 6 * 2.0 ** -24 * 100, (i, k)
+    assert bat.done[ids[3]].tokens == [7] * 14
+
+
+def test_apply_rules_on_rows_without_any():
+    x = torch.randn(2, 100, device="cuda")
+    assert torch.equal(apply_rules(x, [None, LogitRules()], [[], [1]], [[], []]), x)
