@@ -39,7 +39,7 @@ namespace {
 constexpr int kBoxRows = 64;
 constexpr int kConsumerWarps = 4;
 constexpr int kThreads = (kConsumerWarps + 1) * 32;
-constexpr int kPad = 8;            // floats between the merge rows of two heads (bank spread)
+constexpr int kPad = 4;            // floats between the merge rows of two heads (bank spread)
 
 template <int D, bool k8>
 struct Cfg {
@@ -54,9 +54,10 @@ struct Cfg {
     static constexpr int kStageBytes = 2 * kTileBytes;
     static constexpr int kStages = kStageBytes >= 32768 ? 3 : 6;
     static constexpr int kExpBytes = k8 ? 2 * kTile : 0;        // K and V exponents of a stage
-    static constexpr int kRedFloats = (kConsumerWarps - 1) * kMaxGroup * (D + kPad);
-    static constexpr int kSmemBytes = kStages * (kStageBytes + kExpBytes) + kRedFloats * 4 +
-                                      3 * kConsumerWarps * kMaxGroup * 4 + 2 * kStages * 8 + 1024;
+    static constexpr int kRedFloats = kConsumerWarps * kMaxGroup * (D + kPad);   // the warps' rows, in a stage
+    static constexpr int kSmemBytes =
+        kStages * (kStageBytes + kExpBytes) + 3 * kConsumerWarps * kMaxGroup * 4 + 2 * kStages * 8 + 1024;
+    static_assert(kRedFloats * 4 <= kStageBytes, "a stage holds the warps' rows");
     static_assert(2 * (kSmemBytes + 1024) <= 233472, "two CTAs per SM no longer fit");
 };
 
@@ -141,8 +142,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* s_exp = smem + NS * C::kStageBytes;                       // [NS][K exps | V exps]
-    float* red_o = reinterpret_cast<float*>(s_exp + NS * C::kExpBytes);
-    float* red_m = red_o + C::kRedFloats;                              // [4][8]
+    float* red_m = reinterpret_cast<float*>(s_exp + NS * C::kExpBytes);   // [4][8]
     float* red_l = red_m + kConsumerWarps * kMaxGroup;
     float* red_mo = red_l + kConsumerWarps * kMaxGroup;
     uint64_t* full = reinterpret_cast<uint64_t*>(red_mo + kConsumerWarps * kMaxGroup);
@@ -476,13 +476,17 @@ __global__ void __launch_bounds__(kThreads, 2)
                         }
                     }
                 }
+                if (t + 1 == w.t1) break;            // the stretch's last stage is kept for the merge
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&empty[stage]);
                 if (++stage == NS) { stage = 0; phase ^= 1; }
             }
             if (!alive) break;
 
-            // ---- merge the four warps ----
+            // ---- merge the four warps, in the memory of the stretch's last stage (the next tiles are on their way) ----
+            float* red_o = reinterpret_cast<float*>(smem + stage * C::kStageBytes);   // [4][8][D + kPad]
+            asm volatile("bar.sync 1, %0;" ::"n"(kConsumerWarps * 32) : "memory");    // all have read that stage, and
+                                                                                       // the last stretch's statistics
 #pragma unroll
             for (int off = 4; off < 32; off <<= 1) {
                 l[0] += __shfl_xor_sync(0xffffffffu, l[0], off);
@@ -498,75 +502,59 @@ __global__ void __launch_bounds__(kThreads, 2)
             }
             // column of o[i][2h + .]: 8-bit rows 16 i + 2 grp + h, bf16 rows 16 i + 8 h + grp
             auto o_col = [&](int i, int h) -> int { return k8 ? 16 * i + 2 * grp + h : 16 * i + 8 * h + grp; };
-            if (warp > 0) {
-                float* dst = red_o + (warp - 1) * kMaxGroup * (D + kPad);
+            float* dst = red_o + warp * kMaxGroup * (D + kPad);
 #pragma unroll
-                for (int i = 0; i < KS; ++i) {
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        dst[(2 * tig + e) * (D + kPad) + o_col(i, 0)] = o[i][e];
-                        dst[(2 * tig + e) * (D + kPad) + o_col(i, 1)] = o[i][2 + e];
-                    }
-                }
-            }
-            asm volatile("bar.sync 1, %0;" ::"n"(kConsumerWarps * 32) : "memory");
-            if (warp == 0) {
+            for (int i = 0; i < KS; ++i) {
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const int h = 2 * tig + e;
-                    float M = red_m[h], MO = red_mo[h];
-#pragma unroll
-                    for (int v = 1; v < kConsumerWarps; ++v) {
-                        M = fmaxf(M, red_m[v * kMaxGroup + h]);
-                        MO = fmaxf(MO, red_mo[v * kMaxGroup + h]);
-                    }
-                    const float Mu = M == -INFINITY ? 0.f : M, MOu = MO == -INFINITY ? 0.f : MO;
-                    float L = 0.f, ow[kConsumerWarps];
-#pragma unroll
-                    for (int v = 0; v < kConsumerWarps; ++v) {
-                        L += red_l[v * kMaxGroup + h] * ex2_approx(red_m[v * kMaxGroup + h] - Mu);
-                        ow[v] = ex2_approx(red_mo[v * kMaxGroup + h] - MOu);
-                    }
-                    // the stretch's own attention row (normalised), and log2 of its weight
-                    const float f = L != 0.f ? ex2_approx(MOu - Mu) / L : 0.f;
-#pragma unroll
-                    for (int i = 0; i < KS; ++i) {
-#pragma unroll
-                        for (int hh = 0; hh < 2; ++hh) {
-                            float* at = red_o + h * (D + kPad) + o_col(i, hh);
-                            float x = o[i][2 * hh + e] * ow[0];
-#pragma unroll
-                            for (int v = 1; v < kConsumerWarps; ++v) x += at[(v - 1) * kMaxGroup * (D + kPad)] * ow[v];
-                            *at = x * f;
-                        }
-                    }
-                    if (grp == 0) red_l[h] = L != 0.f ? Mu + log2f(L) : -INFINITY;
+                    dst[(2 * tig + e) * (D + kPad) + o_col(i, 0)] = o[i][e];
+                    dst[(2 * tig + e) * (D + kPad) + o_col(i, 1)] = o[i][2 + e];
                 }
             }
             asm volatile("bar.sync 1, %0;" ::"n"(kConsumerWarps * 32) : "memory");
-            // ---- write the stretch's rows: final, or a partial ----
-            if (w.whole() && !a.shared) {
-                __nv_bfloat16* orow = a.out + ((int64_t)w.b * a.H + (int64_t)w.g * a.n_rep) * D;
-                for (int i = threadIdx.x; i < a.n_rep * (D / 2); i += kConsumerWarps * 32) {
-                    const int h = i / (D / 2), d = 2 * (i % (D / 2));
-                    *reinterpret_cast<uint32_t*>(orow + h * D + d) =
-                        pack_bf16x2(red_o[h * (D + kPad) + d], red_o[h * (D + kPad) + d + 1]);
+            // A thread joins four columns of a head: the final row, or the stretch's own attention row (normalised) and
+            // log2 of its weight as a part.  A whole pair's part (to be joined with the prefix) has a slot of its own; a
+            // cut pair's takes the CTA's first slot if the CTA begins in it, else the second.
+            const bool final_row = w.whole() && !a.shared;
+            const int64_t slot = w.whole() ? whole_slots(a) + (int64_t)w.b * a.Hkv + w.g
+                                           : 2 * (int64_t)blockIdx.x + (w.pos == s_plan[1] ? 0 : 1);
+            for (int i = threadIdx.x; i < a.n_rep * (D / 4); i += kConsumerWarps * 32) {
+                const int h = i / (D / 4), d = 4 * (i % (D / 4));
+                float M = red_m[h], MO = red_mo[h];
+#pragma unroll
+                for (int v = 1; v < kConsumerWarps; ++v) {
+                    M = fmaxf(M, red_m[v * kMaxGroup + h]);
+                    MO = fmaxf(MO, red_mo[v * kMaxGroup + h]);
                 }
-            } else {
-                // a whole pair's row (joined with the prefix) has a slot of its own; a cut pair takes the
-                // CTA's first slot if the CTA begins in it, else the second
-                const int64_t slot = w.whole() ? whole_slots(a) + (int64_t)w.b * a.Hkv + w.g
-                                               : 2 * (int64_t)blockIdx.x + (w.pos == s_plan[1] ? 0 : 1);
-                float* po = a.part_o + slot * a.n_rep * D;
-                for (int i = threadIdx.x; i < a.n_rep * (D / 4); i += kConsumerWarps * 32) {
-                    const int h = i / (D / 4), d = 4 * (i % (D / 4));
-                    *reinterpret_cast<float4*>(po + h * D + d) =
-                        *reinterpret_cast<const float4*>(red_o + h * (D + kPad) + d);
+                const float Mu = M == -INFINITY ? 0.f : M, MOu = MO == -INFINITY ? 0.f : MO;
+                float L = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int v = 0; v < kConsumerWarps; ++v) {
+                    L += red_l[v * kMaxGroup + h] * ex2_approx(red_m[v * kMaxGroup + h] - Mu);
+                    const float ow = ex2_approx(red_mo[v * kMaxGroup + h] - MOu);
+                    const float4 r = *reinterpret_cast<const float4*>(red_o + (v * kMaxGroup + h) * (D + kPad) + d);
+                    x[0] = fmaf(r.x, ow, x[0]);
+                    x[1] = fmaf(r.y, ow, x[1]);
+                    x[2] = fmaf(r.z, ow, x[2]);
+                    x[3] = fmaf(r.w, ow, x[3]);
                 }
-                if (threadIdx.x < a.n_rep) a.part_lse[slot * a.n_rep + threadIdx.x] = red_l[threadIdx.x];
+                const float f = L != 0.f ? ex2_approx(MOu - Mu) / L : 0.f;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] *= f;
+                if (final_row) {
+                    uint32_t* orow = reinterpret_cast<uint32_t*>(a.out + ((int64_t)w.b * a.H + w.g * a.n_rep + h) * D + d);
+                    orow[0] = pack_bf16x2(x[0], x[1]);
+                    orow[1] = pack_bf16x2(x[2], x[3]);
+                } else {
+                    *reinterpret_cast<float4*>(a.part_o + (slot * a.n_rep + h) * D + d) = make_float4(x[0], x[1], x[2], x[3]);
+                    if (d == 0) a.part_lse[slot * a.n_rep + h] = L != 0.f ? Mu + log2f(L) : -INFINITY;
+                }
             }
             if (w.t0 == 0 && threadIdx.x == 0) a.plan[kPlanHead + w.b * a.Hkv + w.g] = w.pos;   // where the pair begins
-            asm volatile("bar.sync 1, %0;" ::"n"(kConsumerWarps * 32) : "memory");
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // before TMA writes the stage again
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty[stage]);
+            if (++stage == NS) { stage = 0; phase ^= 1; }
             w = next;
         } while (more);
     }
