@@ -444,7 +444,7 @@ MLLM_API int mllm_decode_attention_paged_kv8(const void* q, const mllm_paged_kv8
 /* ----------------------------------------------------------------------------------------
  * Decode attention over a paged cache for a batch that shares a prefix: cache rows 0 ..
  * prefix_len - 1 are the same for every sequence of the call (a system prompt, a document) and are
- * read through block-table row 0, once for the whole batch; rows prefix_len .. kv_lens[b] - 1 are
+ * read once for the whole batch, through the block-table row of the first sequence that is not empty; rows prefix_len .. kv_lens[b] - 1 are
  * each sequence's own, through its own table row.  The result is that of
  * mllm_decode_attention_paged_bf16 over caches that hold equal rows there; whether the tables share
  * the blocks or hold copies makes no difference.  prefix_len 0 is the plain decode.

@@ -206,9 +206,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     pdl_wait();
     // ---- the plan, the same in every CTA: from the tiles that the other kernel will find ----
     __shared__ PrefixCut s_cut;
+    __shared__ int s_holder;
     if (warp == 2) {
+        // the first sequence that has the prefix: its table row is the one to read (others may be empty)
+        int holder = -1;
+        for (int base = 0; base < a.B && holder < 0; base += 32) {
+            const bool has = base + lane < a.B && !seq_tiles<kOwnTile>(st, base + lane).short_len;
+            const unsigned m = __ballot_sync(0xffffffffu, has);
+            if (m != 0u) holder = base + __ffs(m) - 1;
+        }
         const int own = total_tiles<kOwnTile>(st, lane);
         if (lane == 0) {
+            s_holder = holder;
             s_cut = cut_prefix(a.n_tiles, prefix_sms(a, (float)own, D == 128 ? 1.f : 0.6f), a.pairs, a.single);
             if (blockIdx.x == 0 && blockIdx.y == 0) {
                 st.plan[kPlanPair] = s_cut.splits;
@@ -217,6 +226,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     }
     __syncthreads();
+    const int holder = s_holder;
+    if (holder < 0) return;                                               // nobody has it
     const PrefixCut cut = s_cut;
     const int g = blockIdx.x;
     const int y = blockIdx.y;
@@ -276,7 +287,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     uint8_t* sk = sKV + stage * 2 * C::kTileBytes;
                     uint8_t* sv = sk + C::kTileBytes;
                     int blk, row;
-                    kv_locate(a.lay, 0, (int64_t)(first + j) * kBN, blk, row);   // a bad entry reads block 0
+                    kv_locate(a.lay, holder, (int64_t)(first + j) * kBN, blk, row);   // a bad entry reads block 0
                     const CUtensorMap* mv = first + j == a.n_tiles - 1 ? &tmVend : &tmV;
                     if (!mbar_wait(&bar.k_empty[stage], phase)) break;
                     mbar_arrive_expect_tx(&bar.k_full[stage], C::kTileBytes);

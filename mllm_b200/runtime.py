@@ -669,9 +669,8 @@ def _prefill_kv8(q: torch.Tensor, cache: PagedKVCache8, cu_dev: torch.Tensor, B:
     lens = cache.lengths[:B]
     rows = max(cache.host_lengths()[:B])
     kst, vst = kv8_read(cache, lens, rows)
-    abi.call("mllm_prefill_attention_varlen_bf16", _ptr(q), _ptr(kst), _ptr(vst), num_kv_heads * rows * D, rows * D, D,
-             rows, _ptr(cu_dev), _ptr(lens), B, H, num_kv_heads, D, T, max_q, 1.0 / math.sqrt(D), _ptr(out),
-             abi.stream_handle())
+    _launch(q.get_device(), "mllm_prefill_attention_varlen_bf16", _ptr(q), _ptr(kst), _ptr(vst), num_kv_heads * rows * D,
+            rows * D, D, rows, _ptr(cu_dev), _ptr(lens), B, H, num_kv_heads, D, T, max_q, 1.0 / math.sqrt(D), _ptr(out))
     return out
 
 
@@ -888,9 +887,9 @@ def decode_attention(q: torch.Tensor, kv_cache: KVCache, num_kv_heads: int,
 def decode_attention_shared(q: torch.Tensor, kv_cache: PagedKVCache, num_kv_heads: int, prefix_len: int,
                             max_kv_len: int | None = None) -> torch.Tensor:
     """decode_attention over a paged cache whose sequences 0 .. B-1 all begin with the same prefix_len
-    rows (PagedKVCache.fork): the prefix is read once, through row 0 of the block table, for the
-    whole batch, every sequence's further rows through its own -> [B, 1, H*D].  Lengths come from the
-    cache (each at least prefix_len, or 0)."""
+    rows (PagedKVCache.fork): the prefix is read once for the whole batch, through the table row of
+    the first sequence that is not empty, every sequence's further rows through its own -> [B, 1, H*D].
+    Lengths come from the cache (each at least prefix_len, or 0)."""
     _check_cuda_bf16("q", q)
     if not isinstance(kv_cache, PagedKVCache) or isinstance(kv_cache, PagedKVCache8):
         raise RuntimeError("decode_attention_shared: needs a bf16 PagedKVCache")
@@ -951,10 +950,10 @@ def _decode_step_shared(q, k, v, cache: PagedKVCache, positions, rope_theta, num
         qn, kn = qn.to(BF16).contiguous(), kn.to(BF16).contiguous()
     q_rot = torch.empty((B, H, D), dtype=BF16, device=q.device)
     kv = cache.descriptor()
-    abi.call("mllm_qkv_epilogue_paged_bf16", _ptr(q), q.stride(0), q.stride(2), q.stride(1), _ptr(k), k.stride(0),
-             k.stride(2), k.stride(1), _ptr(v), v.stride(0), v.stride(2), v.stride(1), B, 1, H, num_kv_heads, D, _ptr(pos),
-             0 if pos.numel() == 1 else pos.stride(0), 0, float(rope_theta), _ptr(cos), _ptr(sin), rsb, 0, _ptr(qn),
-             _ptr(kn), float(eps), _ptr(q_rot), C.byref(kv), _ptr(cache.lengths), 0, abi.stream_handle())
+    _launch(q.get_device(), "mllm_qkv_epilogue_paged_bf16", _ptr(q), q.stride(0), q.stride(2), q.stride(1), _ptr(k),
+            k.stride(0), k.stride(2), k.stride(1), _ptr(v), v.stride(0), v.stride(2), v.stride(1), B, 1, H, num_kv_heads, D,
+            _ptr(pos), 0 if pos.numel() == 1 else pos.stride(0), 0, float(rope_theta), _ptr(cos), _ptr(sin), rsb, 0,
+            _ptr(qn), _ptr(kn), float(eps), _ptr(q_rot), C.byref(kv), _ptr(cache.lengths), 0)
     if capturing:
         cache.lengths[:B] += 1
         L = cache.capture_max_len

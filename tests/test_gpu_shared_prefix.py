@@ -163,3 +163,35 @@ def test_refusals(rt):
         rt.decode_attention_shared(q, rt.PagedKVCache8(2, 2, 128, 128, 2), 2, 0)
     with pytest.raises(RuntimeError, match="bfloat16"):
         rt.decode_attention_shared(q.float(), c, 2, 100)
+
+
+def test_a_padded_batch_may_begin_with_empty_rows(rt):
+    """Empty rows (length 0, tables full of anything) anywhere in the batch: zeros for them, the prefix from a row that
+    has it; a batch of nothing but empty rows is all zeros."""
+    c, lens = _shared_cache(rt, 300, [5, 6, 7, 8], 2, 128, 128, seed=4)
+    q = torch.randn(4, 8, 128, device="cuda").bfloat16()
+    keep = c.block_table.clone()
+    for empty in ([0], [0, 1, 3], [2], [0, 1, 2, 3]):
+        c.block_table.copy_(keep)
+        c.lengths.copy_(torch.tensor(lens, dtype=torch.int32))
+        for b in empty:
+            c.lengths[b] = 0
+            c.block_table[b] = -7
+        got = rt.decode_attention_shared(q, c, 2, 300)
+        _status_ok()
+        _check(c, q, got, [0 if b in empty else n for b, n in enumerate(lens)], 2)
+
+
+def test_on_side_streams_at_once(rt):
+    """Two streams over one cache at the same time, each call with its own workspace."""
+    c, lens = _shared_cache(rt, 3000, [100, 1, 700, 30], 8, 128, 256, seed=6)
+    qs = [torch.randn(4, 32, 128, device="cuda").bfloat16() for _ in range(8)]
+    want = [rt.decode_attention_shared(q, c, 8, 3000) for q in qs]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for i, q in enumerate(qs):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append(rt.decode_attention_shared(q, c, 8, 3000))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
