@@ -147,7 +147,8 @@ __global__ void __launch_bounds__(kThreads, 2)
     float* red_mo = red_l + kConsumerWarps * kMaxGroup;
     uint64_t* full = reinterpret_cast<uint64_t*>(red_mo + kConsumerWarps * kMaxGroup);
     uint64_t* empty = full + NS;
-    __shared__ int s_plan[5];   // tiles of this CTA, its first tile, that tile's sequence and place in it, tiles per pair
+    __shared__ int s_plan[6];   // tiles of this CTA, its first tile, that tile's sequence and place in it, tiles per pair,
+                               // whether every pair has a CTA
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
@@ -162,11 +163,16 @@ __global__ void __launch_bounds__(kThreads, 2)
     // everything before it and then let this grid start: the wait moves to the end of the kernel.
     if (!a.shared) pdl_wait();
     pdl_trigger();
-    if (warp == 0) {
-        const int total = total_tiles<TILE>(a, lane);
+    const int pairs = a.B * a.Hkv;
+    if (a.direct) {
+        if (threadIdx.x == 0) s_plan[5] = 1;
+    } else if (warp == 0) {
+        int longest;
+        const int total = total_tiles<TILE>(a, lane, &longest);
+        const bool direct = direct_pairs(pairs, longest, a.ctas, a.shared);
         const int per = tiles_per_cta(a, total);
         const int p0 = min(total, (int)blockIdx.x * per);
-        const int n = min(per, total - p0);
+        const int n = direct ? 0 : min(per, total - p0);
         int before = 0;   // tiles of the sequences before this batch of 32
         if (n > 0) {
             for (int base = 0; base < a.B; base += 32) {
@@ -194,19 +200,35 @@ __global__ void __launch_bounds__(kThreads, 2)
         if (lane == 0) {
             s_plan[0] = n;
             s_plan[1] = p0;
-            if (blockIdx.x == 0) a.plan[kPlanPer] = per;
+            s_plan[5] = direct ? 1 : 0;
+            if (blockIdx.x == 0) a.plan[kPlanPer] = direct ? 0 : per;   // 0: nothing to join
         }
     }
     __syncthreads();
     Walk w;
-    w.left = s_plan[0];
-    w.pos = s_plan[1];
-    if (w.left > 0) {
-        w.b = s_plan[2];
-        w.g = s_plan[3] / s_plan[4];
-        w.t0 = s_plan[3] - w.g * s_plan[4];
-        w.s = seq_tiles<TILE>(a, w.b);
-        walk_open<TILE>(a, w);
+    if (s_plan[5]) {
+        w.left = w.pos = w.t0 = 0;
+        if ((int)blockIdx.x < pairs) {
+            w.b = blockIdx.x / a.Hkv;
+            w.g = blockIdx.x - w.b * a.Hkv;
+            w.s = seq_tiles<TILE>(a, w.b);
+            w.left = w.s.tiles;
+            walk_open<TILE>(a, w);
+            if (w.left == 0) {   // an empty sequence
+                __nv_bfloat16* out = a.out + ((int64_t)w.b * a.H + (int64_t)w.g * a.n_rep) * D;
+                for (int i = threadIdx.x; i < a.n_rep * D; i += kThreads) out[i] = __float2bfloat16_rn(0.f);
+            }
+        }
+    } else {
+        w.left = s_plan[0];
+        w.pos = s_plan[1];
+        if (w.left > 0) {
+            w.b = s_plan[2];
+            w.g = s_plan[3] / s_plan[4];
+            w.t0 = s_plan[3] - w.g * s_plan[4];
+            w.s = seq_tiles<TILE>(a, w.b);
+            walk_open<TILE>(a, w);
+        }
     }
 
     if (warp == kConsumerWarps) {
@@ -550,7 +572,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                     if (d == 0) a.part_lse[slot * a.n_rep + h] = L != 0.f ? Mu + log2f(L) : -INFINITY;
                 }
             }
-            if (w.t0 == 0 && threadIdx.x == 0) a.plan[kPlanHead + w.b * a.Hkv + w.g] = w.pos;   // where the pair begins
+            if (!s_plan[5] && w.t0 == 0 && threadIdx.x == 0) a.plan[kPlanHead + w.b * a.Hkv + w.g] = w.pos;   // where the pair begins
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // before TMA writes the stage again
             __syncwarp();
             if (lane == 0) mbar_arrive(&empty[stage]);
@@ -579,6 +601,7 @@ __global__ void __launch_bounds__(kCombineWarps * 32) stream_combine_kernel(Stre
     const int b = bh / a.H, h = bh - b * a.H, g = h / a.n_rep, r = h - g * a.n_rep;
     pdl_wait();
     const int per = a.plan[kPlanPer], p0 = a.plan[kPlanHead + b * a.Hkv + g];   // p0 means nothing without tiles
+    if (per == 0) return;                 // every pair had a CTA of its own
     const SeqTiles s = seq_tiles<TILE>(a, b);
     const int n_pre = !a.shared || s.short_len ? 0 : a.plan[b < a.pair_seqs ? kPlanPair : kPlanSingle];
     int c0 = s.tiles ? p0 / per : 0;
@@ -679,14 +702,17 @@ int launch_stream_d(StreamArgs& a, const Kv8View& kv, const CUtensorMap& tmK, co
     const int64_t most = (int64_t)a.B * a.Hkv * ((a.max_len + C::kTile - 1) / C::kTile - a.first_row / C::kTile);
     if (most > 0x7fffffffLL - 65536) return fail(MLLM_ERR_UNSUPPORTED, "decode_attention: batch too large for one call");
     a.ctas = std::min(2 * num_sms, kMaxCtas);
-    const int grid = stream_ctas(most, a.ctas, a.shared);
+    const int grid = std::max(stream_ctas(most, a.ctas, a.shared),
+                              direct_pairs((int64_t)a.B * a.Hkv, 0, a.ctas, a.shared) ? a.B * a.Hkv : 1);
     auto kern = stream_decode_kernel<D, k8>;
     if (int st = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes),
                             "stream_decode smem attribute"))
         return st;
+    a.direct = direct_pairs((int64_t)a.B * a.Hkv, (a.max_len + C::kTile - 1) / C::kTile, a.ctas, a.shared) ? 1 : 0;
     if (int st = check_cuda(launch_pdl(kern, dim3(grid), dim3(kThreads), C::kSmemBytes, s, tmK, tmV, a, kv),
                             "stream_decode_kernel launch"))
         return st;
+    if (a.direct) return MLLM_OK;
     return check_cuda(launch_pdl(stream_combine_kernel<D, C::kTile>,
                                  dim3((unsigned)(((int64_t)a.B * a.H + kCombineWarps - 1) / kCombineWarps)),
                                  dim3(kCombineWarps * 32), 0, s, a),

@@ -605,30 +605,39 @@ def kv8_read(kv_cache: PagedKVCache8, lens: torch.Tensor, rows: int, first: torc
     return k, v
 
 
-def _check_decode(q: torch.Tensor, kv_cache: PagedKVCache, num_kv_heads: int) -> int:
-    """Checks decode queries [B, H, D] against a paged cache; returns the device number."""
+def _decode_args(q: torch.Tensor, kv_cache: PagedKVCache, num_kv_heads: int, max_kv_len: int | None):
+    """Decode queries [B, H, D] or [B, H, 1, D] checked against a paged cache: (q as 16-byte aligned contiguous
+    [B, H, D], its shape, device number, bound on the lengths)."""
+    _check_cuda_bf16("q", q)
+    shape = q.shape
+    if len(shape) == 4 and shape[2] == 1:
+        q = q.squeeze(2)
+        shape = q.shape
+    if len(shape) != 3:
+        raise RuntimeError("Attention: decode queries must be [B, H, D] or [B, H, 1, D]")
+    if not q.is_contiguous() or q.data_ptr() % 16:
+        q = q.clone(memory_format=torch.contiguous_format)
     pool = kv_cache.k_pool
     dev = pool.get_device()
+    pool_shape = pool.shape
     if q.get_device() != dev:
         raise RuntimeError("Attention: q and the cache must be on one device")
-    if pool.size(1) != num_kv_heads or pool.size(3) != q.size(2) or q.size(0) > kv_cache.block_table.size(0):
+    if pool_shape[1] != num_kv_heads or pool_shape[3] != shape[2] or shape[0] > kv_cache.block_table.shape[0]:
         raise RuntimeError("Attention: the cache has other kv heads, another head_dim or fewer sequences")
-    return dev
+    L = max_kv_len or max(kv_cache.host_lengths()[:shape[0]], default=0)
+    return q, shape, dev, max(min(L, kv_cache.capacity), 1)
 
 
-def _decode_kv8(q: torch.Tensor, kv_cache: PagedKVCache8, num_kv_heads: int, max_kv_len: int) -> torch.Tensor:
-    """decode_attention over an 8-bit cache: q [B, H, D] contiguous."""
-    B, H, D = q.shape
-    dev = _check_decode(q, kv_cache, num_kv_heads)
-    if q.data_ptr() % 8:
-        q = q.clone()
+def _decode_kv8(q: torch.Tensor, kv_cache: PagedKVCache8, num_kv_heads: int, max_kv_len: int | None) -> torch.Tensor:
+    """decode_attention over an 8-bit cache."""
+    q, (B, H, D), dev, L = _decode_args(q, kv_cache, num_kv_heads, max_kv_len)
     device = q.device
     out = torch.empty((B, 1, H * D), dtype=BF16, device=device)
     # a workspace of the call's own, from torch's stream-ordered allocator (a captured graph's from its pool)
     nbytes = _workspace_size("mllm_decode_attention_kv8_workspace_size", B, H, num_kv_heads, D)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
     _launch(dev, "mllm_decode_attention_paged_kv8", q.data_ptr(), C.byref(kv_cache.descriptor()), kv_cache.lengths.data_ptr(),
-            B, H, num_kv_heads, D, max_kv_len, 1.0 / math.sqrt(D), out.data_ptr(), ws.data_ptr(), nbytes)
+            B, H, num_kv_heads, D, L, 1.0 / math.sqrt(D), out.data_ptr(), ws.data_ptr(), nbytes)
     return out
 
 
@@ -859,15 +868,14 @@ def decode_attention(q: torch.Tensor, kv_cache: KVCache, num_kv_heads: int,
                      max_kv_len: int | None = None) -> torch.Tensor:
     """One query row per sequence (Q [B,H,1,D] or [B,H,D]) over each sequence's cache rows
     (per-sequence lengths) -> [B, 1, H*D]."""
+    if isinstance(kv_cache, PagedKVCache8):
+        return _decode_kv8(q, kv_cache, num_kv_heads, max_kv_len)
     B, H, D = q.shape[0], q.shape[1], q.shape[-1]
     qq = q.reshape(B, H, D)
     if not qq.is_contiguous():
         qq = qq.contiguous()
     L = max_kv_len or max(kv_cache.host_lengths()[:B])
     L = min(L, kv_cache.capacity)
-    if isinstance(kv_cache, PagedKVCache8):
-        _check_cuda_bf16("q", qq)
-        return _decode_kv8(qq, kv_cache, num_kv_heads, L)
     out = torch.empty((B, 1, H * D), dtype=BF16, device=q.device)
     lib = abi.load()
     nbytes = lib.mllm_decode_attention_workspace_size(B, H, num_kv_heads, D, L)
@@ -890,21 +898,14 @@ def decode_attention_shared(q: torch.Tensor, kv_cache: PagedKVCache, num_kv_head
     rows (PagedKVCache.fork): the prefix is read once for the whole batch, through the table row of
     the first sequence that is not empty, every sequence's further rows through its own -> [B, 1, H*D].
     Lengths come from the cache (each at least prefix_len, or 0)."""
-    _check_cuda_bf16("q", q)
     if not isinstance(kv_cache, PagedKVCache) or isinstance(kv_cache, PagedKVCache8):
         raise RuntimeError("decode_attention_shared: needs a bf16 PagedKVCache")
-    B, H, D = q.shape[0], q.shape[1], q.shape[-1]
-    qq = q.reshape(B, H, D)
-    if not qq.is_contiguous() or qq.data_ptr() % 16:
-        qq = qq.clone(memory_format=torch.contiguous_format)
-    dev = _check_decode(qq, kv_cache, num_kv_heads)
-    L = max_kv_len or max(kv_cache.host_lengths()[:B], default=0)
-    L = max(min(L, kv_cache.capacity), 1)
-    out = torch.empty((B, 1, H * D), dtype=BF16, device=q.device)
-    # a workspace of the call's own, from torch's stream-ordered allocator (a captured graph's from its pool)
+    q, (B, H, D), dev, L = _decode_args(q, kv_cache, num_kv_heads, max_kv_len)
+    device = q.device
+    out = torch.empty((B, 1, H * D), dtype=BF16, device=device)
     nbytes = _workspace_size("mllm_decode_attention_shared_workspace_size", B, H, num_kv_heads, D, prefix_len)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-    _launch(dev, "mllm_decode_attention_shared_paged_bf16", qq.data_ptr(), C.byref(kv_cache.descriptor()),
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)   # of the call's own, as in _decode_kv8
+    _launch(dev, "mllm_decode_attention_shared_paged_bf16", q.data_ptr(), C.byref(kv_cache.descriptor()),
             kv_cache.lengths.data_ptr(), prefix_len, B, H, num_kv_heads, D, L, 1.0 / math.sqrt(D), out.data_ptr(),
             ws.data_ptr(), nbytes)
     return out

@@ -240,6 +240,9 @@ DECODE = [
     (10, 2, 128, [700, 91], 128, 20, 1e-4),      # rows of very different size
     (10, 2, 128, [700, 91], 128, 1, 300.0),      # one weight close to 1
     (16, 2, 64, [40] * 70 + [0] * 3 + [129] * 30, 128, 1, 1.0),   # more sequences than three warps of lengths
+    (8, 2, 128, [768, 0, 5], 128, 1, 1.0),       # the longest that is not cut, and one row more
+    (8, 2, 128, [769, 0, 5], 128, 1, 1.0),
+    (4, 4, 64, [300] * 75, 128, 1, 1.0),         # short, but more pairs than CTAs
 ]
 
 
