@@ -573,7 +573,7 @@ def qkv_epilogue_kv8(q, k, v, kv_cache: PagedKVCache8, cu_seqlens: torch.Tensor,
         _check_vec("q_norm_weight", qn, D, BF16, dev)
         _check_vec("k_norm_weight", kn, D, BF16, dev)
     if out is None:
-        out = torch.empty(shape, dtype=BF16, device=q.device)
+        out = torch.empty_strided(shape, (H * D, D, 1), dtype=BF16, device=q.device)   # torch.empty takes 1 us longer
     elif out.shape != shape or out.dtype is not BF16 or out.get_device() != dev or out.stride(2) != 1:
         raise RuntimeError("Attention: out must be bf16 [T, H, D] with D contiguous on q's device")
     out_stride = out.stride()
@@ -598,7 +598,7 @@ def kv8_read(kv_cache: PagedKVCache8, lens: torch.Tensor, rows: int, first: torc
     if first is not None:
         _check_vec("first", first, n, torch.int32, dev)
     Hkv, D = pool.size(1), pool.size(3)
-    k = torch.empty((n, Hkv, rows, D), dtype=BF16, device=pool.device)
+    k = torch.empty_strided((n, Hkv, rows, D), (Hkv * rows * D, rows * D, D, 1), dtype=BF16, device=pool.device)
     v = torch.empty_like(k)
     _launch(dev, "mllm_kv8_read_bf16", C.byref(kv_cache.descriptor()), _ptr(first), lens.data_ptr(), n, Hkv, D, rows,
             k.data_ptr(), v.data_ptr(), Hkv * rows * D, rows * D, D)
@@ -632,10 +632,10 @@ def _decode_kv8(q: torch.Tensor, kv_cache: PagedKVCache8, num_kv_heads: int, max
     """decode_attention over an 8-bit cache."""
     q, (B, H, D), dev, L = _decode_args(q, kv_cache, num_kv_heads, max_kv_len)
     device = q.device
-    out = torch.empty((B, 1, H * D), dtype=BF16, device=device)
+    out = torch.empty_strided((B, 1, H * D), (H * D, H * D, 1), dtype=BF16, device=device)
     # a workspace of the call's own, from torch's stream-ordered allocator (a captured graph's from its pool)
     nbytes = _workspace_size("mllm_decode_attention_kv8_workspace_size", B, H, num_kv_heads, D)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    ws = torch.empty_strided((nbytes,), (1,), dtype=torch.uint8, device=device)
     _launch(dev, "mllm_decode_attention_paged_kv8", q.data_ptr(), C.byref(kv_cache.descriptor()), kv_cache.lengths.data_ptr(),
             B, H, num_kv_heads, D, L, 1.0 / math.sqrt(D), out.data_ptr(), ws.data_ptr(), nbytes)
     return out
@@ -902,9 +902,9 @@ def decode_attention_shared(q: torch.Tensor, kv_cache: PagedKVCache, num_kv_head
         raise RuntimeError("decode_attention_shared: needs a bf16 PagedKVCache")
     q, (B, H, D), dev, L = _decode_args(q, kv_cache, num_kv_heads, max_kv_len)
     device = q.device
-    out = torch.empty((B, 1, H * D), dtype=BF16, device=device)
+    out = torch.empty_strided((B, 1, H * D), (H * D, H * D, 1), dtype=BF16, device=device)
     nbytes = _workspace_size("mllm_decode_attention_shared_workspace_size", B, H, num_kv_heads, D, prefix_len)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)   # of the call's own, as in _decode_kv8
+    ws = torch.empty_strided((nbytes,), (1,), dtype=torch.uint8, device=device)   # of the call's own, as in _decode_kv8
     _launch(dev, "mllm_decode_attention_shared_paged_bf16", q.data_ptr(), C.byref(kv_cache.descriptor()),
             kv_cache.lengths.data_ptr(), prefix_len, B, H, num_kv_heads, D, L, 1.0 / math.sqrt(D), out.data_ptr(),
             ws.data_ptr(), nbytes)
@@ -1104,7 +1104,7 @@ def apply_logit_rules(logits: torch.Tensor, history=None, history_lens=None, out
     if bias_ids is not None and bias_ids.size(1) == 0:
         bias_ids = bias_values = bias_lens = None
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=logits.device)
+        out = torch.empty_strided(shape, (V, 1), dtype=dtype, device=logits.device)
     elif out.shape != shape or out.dtype is not dtype or out.get_device() != dev or (V > 1 and out.stride(1) != 1) or \
             (B > 1 and out.stride(0) < V):
         raise RuntimeError("logit rules: out must be like logits, its rows apart")
