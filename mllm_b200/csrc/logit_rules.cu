@@ -28,10 +28,9 @@ namespace {
 
 constexpr int kThreads = 512;
 constexpr int kMinStretch = 1024;
-constexpr int kMaxStretch = 24 * 1024;   // 96 KB of counters
+constexpr int kMaxStretch = 26 * 1024;   // 104 KB of counters: two CTAs fit on an SM
 constexpr int kMinCtas = 2;
-constexpr int kCtasPerSm = 4;
-constexpr int kHeld = 4;                 // history tokens a thread loads together
+constexpr int kHeld = 2;                 // history tokens a thread loads together
 constexpr int kMaxBias = 1024;
 constexpr unsigned kSeen = 0x80000000u;  // counter bits: the token is in the prompt part of the history ...
 constexpr unsigned kBiased = 0x40000000u; // ... it has a bias; the rest counts it in the generated part
@@ -96,6 +95,10 @@ __global__ void __launch_bounds__(kThreads, kMinCtas) logit_rules_kernel(RuleArg
     int64_t tok[kHeld];
 #pragma unroll
     for (int u = 0; u < kHeld; ++u) tok[u] = t + u * kThreads < cols ? hist[t + u * kThreads] : -1;
+    const int64_t bias_row = (int64_t)row * a.bias_stride;
+    const int bias_cols = a.bias_ids ? a.bias_cols : 0;
+    int64_t bias_id = t < bias_cols ? a.bias_ids[bias_row + t] : -1;
+    float bias_val = t < bias_cols ? a.bias_vals[bias_row + t] : 0.f;
     constexpr int E = 16 / (int)sizeof(T);           // 4 or 8 tokens per 16 bytes
     constexpr int U = 4;                             // 16-byte loads in flight
     const int nv = kWide ? n / E : 0;
@@ -123,18 +126,26 @@ __global__ void __launch_bounds__(kThreads, kMinCtas) logit_rules_kernel(RuleArg
             if (i >= made) atomicAdd(&s_count[at], 1u);
             else atomicOr(&s_count[at], kSeen);
         };
+        for (int i0 = t; i0 < n_hist; i0 += kHeld * kThreads) {
+            int64_t next[kHeld];   // on their way while the present ones are counted
 #pragma unroll
-        for (int u = 0; u < kHeld; ++u) count(t + u * kThreads, tok[u]);
-        for (int i0 = t + kHeld * kThreads; i0 < n_hist; i0 += kHeld * kThreads) {
-#pragma unroll
-            for (int u = 0; u < kHeld; ++u) tok[u] = i0 + u * kThreads < n_hist ? hist[i0 + u * kThreads] : -1;
+            for (int u = 0; u < kHeld; ++u) {
+                const int i = i0 + (kHeld + u) * kThreads;
+                next[u] = i < n_hist ? hist[i] : -1;
+            }
 #pragma unroll
             for (int u = 0; u < kHeld; ++u) count(i0 + u * kThreads, tok[u]);
+#pragma unroll
+            for (int u = 0; u < kHeld; ++u) tok[u] = next[u];
         }
         for (int i = t; i < n_bias; i += kThreads) {
-            const int at = place(a.bias_ids[(int64_t)row * a.bias_stride + i]);
+            if (i != t) {
+                bias_id = a.bias_ids[bias_row + i];
+                bias_val = a.bias_vals[bias_row + i];
+            }
+            const int at = place(bias_id);
             s_id[i] = at;
-            s_val[i] = a.bias_vals[(int64_t)row * a.bias_stride + i];
+            s_val[i] = bias_val;
             if (at >= 0) atomicOr(&s_count[at], kBiased);
         }
         __syncthreads();
@@ -169,23 +180,28 @@ __global__ void __launch_bounds__(kThreads, kMinCtas) logit_rules_kernel(RuleArg
                 if (i >= nv) break;
                 uint32_t* c = reinterpret_cast<uint32_t*>(&w[u]);
                 if (counted) {
+                    uint32_t hit = 0u;
 #pragma unroll
                     for (int e = 0; e < E; e += 4) {
-                        const uint4 k4 = *reinterpret_cast<const uint4*>(s_count + i * E + e);
-                        const uint32_t k[4] = {k4.x, k4.y, k4.z, k4.w};
-                        if ((k4.x | k4.y | k4.z | k4.w) == 0u) continue;
+                        const uint4 k = *reinterpret_cast<const uint4*>(s_count + i * E + e);
+                        hit |= ((k.x ? 1u : 0u) | (k.y ? 2u : 0u) | (k.z ? 4u : 0u) | (k.w ? 8u : 0u)) << e;
+                    }
+                    hit &= m[u];
+                    while (hit != 0u) {   // a lane's own few: a branch per token would run for all of a warp's
+                        const int e = __ffs(hit) - 1;
+                        hit &= hit - 1u;
+                        constexpr int P = E / 4;   // tokens in 32 bits
+                        const int q = e / P, sh = P == 2 ? 16 * (e & 1) : 0;
+                        const uint32_t bits = q < 2 ? (q == 0 ? c[0] : c[1]) : (q == 2 ? c[2] : c[3]);
+                        T v;
+                        if constexpr (P == 1) v = __uint_as_float(bits);
+                        else v = __ushort_as_bfloat16((unsigned short)(bits >> sh));
+                        store_f32(&v, ruled(load_f32(&v), s_count[i * E + e], i * E + e));
+                        uint32_t now;
+                        if constexpr (P == 1) now = __float_as_uint(v);
+                        else now = (bits & ~(0xFFFFu << sh)) | ((uint32_t)__bfloat16_as_ushort(v) << sh);
 #pragma unroll
-                        for (int d = 0; d < 4; ++d) {
-                            if (k[d] == 0u) continue;
-                            if constexpr (sizeof(T) == 4) {
-                                c[d] = __float_as_uint(ruled(__uint_as_float(c[d]), k[d], i * E + d));
-                            } else {
-                                const int q = (e + d) >> 1, sh = 16 * (d & 1);
-                                const float v = ruled(__uint_as_float((c[q] >> sh) << 16), k[d], i * E + e + d);
-                                const uint32_t b = __bfloat16_as_ushort(__float2bfloat16_rn(v));
-                                c[q] = (c[q] & ~(0xFFFFu << sh)) | (b << sh);
-                            }
-                        }
+                        for (int d = 0; d < 4; ++d) c[d] = d == q ? now : c[d];
                     }
                 }
                 if (m[u] != kAll) {
@@ -277,10 +293,13 @@ extern "C" int mllm_logit_rules(const void* logits, int logits_bf16, int64_t row
     a.bias_lens = bias_lens;
     a.allowed = allowed;
     a.allowed_stride = allowed_stride;
-    // stretches per row: about three CTAs per SM over the batch, within the limits on a stretch
-    const int want = std::max(1, kCtasPerSm * num_sms / batch);
-    int stretch = (vocab + want - 1) / want;
-    stretch = std::min(kMaxStretch, std::max(kMinStretch, (stretch + 255) / 256 * 256));
+    // A row is cut so that all CTAs of the batch fill whole waves of the resident ones, as few waves as the limit on a
+    // stretch allows: every CTA reads its row's whole history, so few long stretches beat many short ones.
+    const int64_t slots = (int64_t)kMinCtas * num_sms;
+    const int64_t least = (vocab + kMaxStretch - 1) / kMaxStretch;
+    const int64_t waves = (least * batch + slots - 1) / slots;
+    const int per_row = (int)std::min<int64_t>(vocab, slots * waves / batch);
+    const int stretch = std::max(kMinStretch, ((vocab + per_row - 1) / per_row + 255) / 256 * 256);
     a.stretch = stretch;
     const dim3 grid((vocab + stretch - 1) / stretch, batch);
     const int smem = a.hist || a.bias_ids ? stretch * 4 : 0;
