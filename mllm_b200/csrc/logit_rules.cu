@@ -9,14 +9,15 @@
 // the row and in L2 after the first CTA) and counts the tokens of its stretch in shared memory, so nothing has to be
 // cleared or kept in global memory and any number of calls may run at once; a bit marks the tokens that have a bias.
 // Then it streams the stretch with 16-byte loads: bits are copied where neither a counter nor the mask says otherwise,
-// and the few tokens with a counter are worked out where they lie.  (Streaming first and redoing the touched tokens in a
-// second pass over the history took 25 us instead of 19: its loads depend on one another and nothing else is left to
-// do meanwhile.)  Everything is taken in a fixed order: counts are whole numbers, and a token's biases are
+// and the few tokens with a counter are worked out where they lie, each lane looping over its own (a branch per token,
+// taken by a warp whenever one of its lanes does, took 22.9 us for 64 bf16 rows instead of 14.2).  Streaming first and
+// redoing the touched tokens in a second pass over the history took 25 us for 64 fp32 rows instead of 19: its loads
+// depend on one another and nothing else is left to do meanwhile.  Everything is taken in a fixed order: counts are whole numbers, and a token's biases are
 // summed in list order by the thread that owns the token.
 //
-// Bound: HBM, the row read and written once: 64 rows of 151936 fp32 logits with up to 5000 tokens of history, 40 biases
-// and a mask take 19 us, 80 MB at 4.1 TB/s; without any rule 9 us (the rows then lie in L2), the rest is the counting that
-// goes before the stretch.
+// Bound: HBM, the row read and written once, behind the counting: 64 rows of 151936 fp32 logits with up to 5000 tokens of
+// history, 40 biases and a mask take 16.3 us, 80 MB at 4.9 TB/s, and with 100 tokens of history 12.7; without any rule
+// 9 us (the rows then lie in L2).  128 rows, which L2 does not hold, take 39.4 us, 161 MB at 4.1 TB/s.
 #include <algorithm>
 #include <cmath>
 
@@ -100,13 +101,13 @@ __global__ void __launch_bounds__(kThreads, kMinCtas) logit_rules_kernel(RuleArg
     int64_t bias_id = t < bias_cols ? a.bias_ids[bias_row + t] : -1;
     float bias_val = t < bias_cols ? a.bias_vals[bias_row + t] : 0.f;
     constexpr int E = 16 / (int)sizeof(T);           // 4 or 8 tokens per 16 bytes
-    constexpr int U = 4;                             // 16-byte loads in flight
+    constexpr int U = 2;                             // 16-byte loads in flight, while as many are worked on
     const int nv = kWide ? n / E : 0;
-    uint4 w[U];
+    uint4 w[U], next_w[U];
     auto load = [&](int i0) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (i0 + u * kThreads < nv) w[u] = reinterpret_cast<const uint4*>(x)[i0 + u * kThreads];
+            if (i0 + u * kThreads < nv) next_w[u] = reinterpret_cast<const uint4*>(x)[i0 + u * kThreads];
     };
     load(t);
     const int n_hist = hist ? checked_len(a.hist_lens, row, a.hist_cols) : 0;
@@ -167,7 +168,9 @@ __global__ void __launch_bounds__(kThreads, kMinCtas) logit_rules_kernel(RuleArg
     if constexpr (kWide) {
         constexpr uint32_t kAll = (1u << E) - 1u;
         for (int i0 = t; i0 < nv; i0 += U * kThreads) {
-            if (i0 != t) load(i0);
+#pragma unroll
+            for (int u = 0; u < U; ++u) w[u] = next_w[u];
+            load(i0 + U * kThreads);
             uint32_t m[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
@@ -261,6 +264,8 @@ extern "C" int mllm_logit_rules(const void* logits, int logits_bf16, int64_t row
         return fail(MLLM_ERR_INVALID_ARGUMENT, "logit_rules: give all of bias_ids, bias_values and bias_lens or none");
     if (bias_ids && (bias_cols < 0 || bias_stride < bias_cols))
         return fail(MLLM_ERR_INVALID_ARGUMENT, "logit_rules: bad bias_cols or bias_stride");
+    if (history && history_cols > (int)~(kSeen | kBiased))
+        return fail(MLLM_ERR_UNSUPPORTED, "logit_rules: more than 2^30 - 1 columns of history");
     if (bias_ids && bias_cols > kMaxBias)
         return fail(MLLM_ERR_UNSUPPORTED, "logit_rules: more than 1024 biases a row");
     if (allowed && allowed_stride < (vocab + 31) / 32)
@@ -268,7 +273,10 @@ extern "C" int mllm_logit_rules(const void* logits, int logits_bf16, int64_t row
     if (batch == 0) return ok();
     if (!logits || !out) return fail(MLLM_ERR_INVALID_ARGUMENT, "logit_rules: null pointer");
     const int es = logits_bf16 ? 2 : 4;
-    if (!aligned(logits, es) || !aligned(out, es) || !aligned(allowed, 4))
+    if (!aligned(logits, es) || !aligned(out, es) || !aligned(allowed, 4) ||
+        !aligned(history, 8) || !aligned(history_lens, 4) || !aligned(output_start, 4) || !aligned(repetition, 4) ||
+        !aligned(presence, 4) || !aligned(frequency, 4) || !aligned(bias_ids, 8) || !aligned(bias_values, 4) ||
+        !aligned(bias_lens, 4))
         return fail(MLLM_ERR_INVALID_ARGUMENT, "logit_rules: misaligned pointer");
     int num_sms = 0;
     if (int st = require_sm100(&num_sms)) return st;
@@ -294,12 +302,13 @@ extern "C" int mllm_logit_rules(const void* logits, int logits_bf16, int64_t row
     a.allowed = allowed;
     a.allowed_stride = allowed_stride;
     // A row is cut so that all CTAs of the batch fill whole waves of the resident ones, as few waves as the limit on a
-    // stretch allows: every CTA reads its row's whole history, so few long stretches beat many short ones.
+    // stretch allows: every CTA reads its row's whole history, so few long stretches beat many short ones (4 fp32 rows
+    // take 5.3 us in one wave and 7.4 in two, 32 rows 9.7 and 12.1).
     const int64_t slots = (int64_t)kMinCtas * num_sms;
-    const int64_t least = (vocab + kMaxStretch - 1) / kMaxStretch;
+    const int64_t least = ((int64_t)vocab + kMaxStretch - 1) / kMaxStretch;
     const int64_t waves = (least * batch + slots - 1) / slots;
-    const int per_row = (int)std::min<int64_t>(vocab, slots * waves / batch);
-    const int stretch = std::max(kMinStretch, ((vocab + per_row - 1) / per_row + 255) / 256 * 256);
+    const int64_t per_row = slots * waves / batch;
+    const int stretch = std::max(kMinStretch, (int)(((int64_t)vocab + per_row - 1) / per_row + 255) / 256 * 256);
     a.stretch = stretch;
     const dim3 grid((vocab + stretch - 1) / stretch, batch);
     const int smem = a.hist || a.bias_ids ? stretch * 4 : 0;

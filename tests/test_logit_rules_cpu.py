@@ -35,6 +35,14 @@ def test_library_refusals(lib):
     assert _call(lib, B=0) == 0
 
 
+def test_library_refuses_long_histories_and_misaligned_lists(lib):
+    full = dict(hist=4096, lens=4096, cols=5, hist_stride=5, ids=4096, vals=4096, b_lens=4096, b_cols=5, b_stride=5)
+    assert _call(lib, **{**full, "cols": 1 << 30, "hist_stride": 1 << 30}) == 2
+    for name, at in (("hist", 4100), ("lens", 4098), ("ids", 4100), ("vals", 4097), ("b_lens", 4098), ("rep", 4098),
+                     ("pres", 4098), ("freq", 4098), ("start", 4098)):
+        assert _call(lib, **{**full, name: at}) == 1 and b"misaligned" in lib.mllm_attn_last_error()
+
+
 def test_python_refuses_host_tensors():
     with pytest.raises(RuntimeError, match="CUDA"):
         rt.apply_logit_rules(torch.zeros(1, 5))
