@@ -505,8 +505,7 @@ MLLM_API int mllm_sample(void* logits, int logits_bf16, int64_t row_stride, int 
  *       be the same memory as logits (with the same stride), else the two must not overlap.
  *   history: int64 device, row b's history_lens[b] <= history_cols tokens at
  *       history + b*history_stride (fewer than 2^30 columns); output_start: int32 device [batch]
- *       (NULL: 0) -- the tokens
- *       before it are the prompt's, which only the repetition penalty counts.
+ *       (NULL: 0) -- the tokens before it are the prompt's, which only the repetition penalty counts.
  *   repetition, presence, frequency: fp32 device [batch] (NULL: 1, 0, 0).
  *   bias_ids / bias_values: int64 / fp32 device, row b's bias_lens[b] <= bias_cols <= 1024 pairs at
  *       + b*bias_stride; a token listed more than once gets every one.

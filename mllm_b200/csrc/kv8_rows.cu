@@ -183,7 +183,7 @@ __device__ __forceinline__ void store_row8(float (&lo)[8], float (&hi)[8], unsig
 
 // Where a token's K and V rows go.  The warp's lanes call it together.
 struct TokenSlot {
-    int seq = 0, first = 0, end = 0;   // the sequence that owns the token, and its tokens
+    int seq = 0, first = 0, end = 0;   // the sequence that owns the token, and its tokens (end: look again from there on)
     int start = 0;                     // its cache rows before the call
     bool owned = false;
 };
@@ -198,9 +198,9 @@ __device__ __forceinline__ void find_sequence(const Epilogue8Args& a, int t, int
         if (ended != 0xffffffffu) break;
     }
     const bool in = s.seq < a.n_seqs;
-    s.first = in ? a.cu_seqlens[s.seq] : t + 1;
-    s.end = in ? a.cu_seqlens[s.seq + 1] : 0x7fffffff;
+    s.first = in ? a.cu_seqlens[s.seq] : 0x7fffffff;
     s.owned = s.first <= t;
+    s.end = s.owned ? a.cu_seqlens[s.seq + 1] : s.first;   // where no sequence's tokens end: with the next one's first
     s.start = s.owned ? a.start[s.seq] : 0;
 }
 

@@ -138,6 +138,32 @@ def test_epilogue_and_read_against_the_formula(rt, H, Hkv, D, tokens, start, beh
         assert same.transpose(1, 2)[keep].all()
 
 
+def test_tokens_in_front_of_the_first_sequence(rt):
+    """Tokens before cu_seqlens[0] belong to no sequence: enough of them that a warp of the streaming form begins
+    with such tokens and goes on to owned ones.  The owned rows are those of a call on the owned tokens alone."""
+    H, Hkv, D, lead, tokens = 4, 1, 64, 4000, [1500, 2500]
+    g = torch.Generator(device="cuda").manual_seed(8)
+    T = lead + sum(tokens)
+    q, k, v = (torch.randn(T, h, D, device="cuda", generator=g).bfloat16() for h in (H, Hkv, Hkv))
+    pos = torch.arange(T, device="cuda")
+    st = torch.zeros(2, dtype=torch.int32, device="cuda")
+    got = []
+    for first in (lead, 0):
+        c = _cache(rt, 2, Hkv, D, max(tokens))
+        for b in range(2):
+            c.reserve(b, tokens[b])
+        cu = torch.tensor([first, first + tokens[0], first + sum(tokens)], dtype=torch.int32, device="cuda")
+        skip = lead - first
+        out = torch.full((T - skip, H, D), 7.0, dtype=torch.bfloat16, device="cuda")
+        rt.qkv_epilogue_kv8(q[skip:], k[skip:], v[skip:], c, cu, st, pos[skip:].contiguous(), 1e4, out=out)
+        _status_ok()
+        assert (out[:first] == 7).all()
+        got.append([out[first:]] + [c.gather(b, tokens[b]) for b in range(2)])
+    assert torch.equal(got[0][0], got[1][0])
+    for x, y in zip(got[0][1:], got[1][1:]):
+        assert torch.equal(x[0], y[0]) and torch.equal(x[1], y[1]) and x[0].abs().max() > 1
+
+
 def test_epilogue_from_positions_equals_the_table(rt):
     """Angles from positions are those of the framework's RoPE table."""
     g = torch.Generator(device="cuda").manual_seed(2)
