@@ -494,11 +494,10 @@ __global__ void __launch_bounds__(kReadThreads, 6) kv8_read_kernel(Read8Args a) 
     const int b = blockIdx.y / a.Hkv, g = blockIdx.y - b * a.Hkv;
     const int c = threadIdx.x % TPR;
     const int r0 = blockIdx.x * (kReadRowsPerThread * RPB) + threadIdx.x / TPR;
-    const int first = a.first ? a.first[b] : 0;
-    int len = a.lens[b];
+    int first = a.first ? a.first[b] : 0, len = a.lens[b];
     if (first < 0 || len < 0) {
         if (threadIdx.x == 0) record_error(kErrBadLength);
-        len = 0;
+        first = len = 0;
     }
     uint2 w[kReadRowsPerThread][2];
     float sc[kReadRowsPerThread][2];

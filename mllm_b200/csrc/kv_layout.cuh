@@ -29,7 +29,7 @@ __device__ __forceinline__ bool kv_locate(const KvLayout& lay, int b, int64_t t,
         row = (int)t;
         return true;
     }
-    if (t > 0x7fffffffLL) {   // no cache addresses so many rows; below, 32-bit division
+    if (t < 0 || t > 0x7fffffffLL) {   // no cache addresses such rows; below, 32-bit division
         record_error(kErrBadLength);
         blk = row = 0;
         return false;

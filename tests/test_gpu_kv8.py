@@ -347,6 +347,19 @@ def test_bad_lengths_and_blocks_are_recorded(rt):
     _status_ok()
 
 
+def test_a_negative_first_row_reads_nothing(rt):
+    from mllm_b200 import abi
+    c = _random_cache(rt, [300, 40], 2, 128, 128, 1, seed=9)
+    for first in (-1, -200, -(2 ** 31)):
+        f = torch.tensor([first, 7], dtype=torch.int32, device="cuda")
+        kr, vr = rt.kv8_read(c, c.lengths[:2], 256, first=f)
+        with pytest.raises(abi.MllmError) as e:
+            _status_ok()
+        assert e.value.status == 7
+        assert (kr[0] == 0).all() and (vr[0] == 0).all() and (kr[1, :, 33:] == 0).all()
+        assert torch.equal(kr[1, :, :33].float(), c.gather(1, 40)[0][:, 7:])
+
+
 @pytest.mark.parametrize("H,Hkv,D,norm", [(8, 2, 128, True), (8, 4, 64, False)])
 def test_prompts_then_steps_through_the_framework(rt, H, Hkv, D, norm):
     """Packed prompts, a second chunk of one of them, then decode steps (eager and from a captured graph): every
