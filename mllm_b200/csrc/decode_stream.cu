@@ -25,8 +25,9 @@
 // differ; the sum l uses exp2(s - m) with its own maximum in fp32.  P is rounded to a half (2^-11), to bf16 for a
 // bf16 cache, since A and B of an MMA have one type; both sums stay fp32.
 //
-// Bound: HBM (2 (D + 1) bytes a row and kv head; 4 D for bf16).  Rows past the end of a sequence are masked to
-// -inf in S and zeroed in V (any bits may lie there); TMA boxes wholly past the end are not loaded.
+// Bound: HBM (2 (D + 1) bytes a row and kv head; 4 D for bf16).  Rows past the end of a sequence, and rows of the
+// prefix in the first tile behind it, are masked to -inf in S and zeroed in V (any bits may lie there); TMA boxes wholly
+// past the end are not loaded.
 #include <algorithm>
 #include <cmath>
 
@@ -462,11 +463,11 @@ __global__ void __launch_bounds__(kThreads, 2)
                     o[i][3] *= oscale[1];
                 }
 
-                // ---- rows past the end: zero this warp's V rows (any bit pattern may lie there) ----
-                if (valid < row0 + C::kWarpRows) {
+                // ---- rows past the end, or of the prefix: zero this warp's V rows (any bit pattern may lie there) ----
+                if (valid < row0 + C::kWarpRows || lo_row > row0) {
                     for (int i = lane; i < C::kWarpRows * CH; i += 32) {
                         const int r = row0 + i / CH, c = i % CH;
-                        if (r >= valid)
+                        if (r >= valid || r < lo_row)
                             asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(chunk_addr(vbase, r, c)), "r"(0)
                                          : "memory");
                     }

@@ -390,7 +390,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 add2(sum[4], sum[5], sum[6], sum[7]);
                 add2(sum[0], sum[1], sum[4], sum[5]);
                 l_run = l_run * alpha + (sum[0] + sum[1]);
-                m_run = m_use;
+                m_run = m_new == -INFINITY ? -INFINITY : m_use;   // a tile of -inf scores sets no maximum
             }
             tc_fence_before();
             mbar_arrive(&bar.p_full[grp]);

@@ -114,6 +114,41 @@ def test_rows_behind_the_prefix_do_not_reach_other_sequences(rt):
     assert torch.equal(want, got)
 
 
+def test_infinities_among_the_prefix_rows(rt):
+    """An infinite V element in the tile where the prefix ends and the own rows begin counts once, as the prefix's."""
+    c, lens = _shared_cache(rt, 200, [9, 0, 30, 5], 2, 64, 128, seed=9)
+    q = torch.randn(4, 8, 64, device="cuda").bfloat16()
+    want = rt.decode_attention_shared(q, c, 2, 200)
+    for b in range(4):
+        c.v_pool[c.blocks_of(b)[1], :, 195 % 128, 3] = float("inf")
+    got = rt.decode_attention_shared(q, c, 2, 200).view(4, 8, 64)
+    _status_ok()
+    assert (got[..., 3] == float("inf")).all()
+    got[..., 3] = want.view(4, 8, 64)[..., 3]
+    assert torch.equal(got, want.view(4, 8, 64))
+
+
+@pytest.mark.parametrize("B", [3, 40])
+def test_tiles_whose_scores_are_all_minus_infinity(rt, B):
+    """Of four tiles of 128 prefix rows three have scores of -inf only, and the others lie near -500 (log2): no tile
+    may set a maximum that those underflow against."""
+    prefix, Hkv, D = 40 * 128, 8, 128
+    c, lens = _shared_cache(rt, prefix, [0] * B, Hkv, D, 128, seed=2)
+    for t, blk in enumerate(c.blocks_of(0)):
+        c.k_pool[blk, :, :, 0] = 0.0 if t % 4 == 2 else -float("inf")
+        c.k_pool[blk, :, :, 1] = -500.0
+    q = torch.zeros(B, 32, D, device="cuda", dtype=torch.bfloat16)
+    q[..., 0], q[..., 1] = 1.0, 8.0
+    got = rt.decode_attention_shared(q, c, Hkv, prefix)
+    _status_ok()
+    k, v = c.gather(0, prefix)
+    rows = (k[0, :, 0] == 0).nonzero().flatten()
+    ref = v[:, rows].double().mean(1)
+    tol = 2.0 ** -8 * ref.abs() + (2.0 ** -8 + 2.0 ** -17) * v[:, rows].double().abs().mean(1)
+    o = got.view(B, Hkv, 4, D).double()
+    assert ((o - ref[None, :, None]).abs() <= tol[None, :, None]).all()
+
+
 def test_captured_and_replayed_with_other_lengths(rt):
     c, lens = _shared_cache(rt, 300, [1, 100, 40], 2, 128, 128, seed=4)
     for b in range(3):
