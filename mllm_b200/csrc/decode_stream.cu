@@ -97,6 +97,18 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
         : "memory");
 }
 
+// A barrier of the consumer warps that says whether any thread came with `flag`.
+__device__ __forceinline__ bool consumers_any(bool flag) {
+    uint32_t any;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, %2, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(any)
+        : "r"((uint32_t)flag), "n"(kConsumerWarps * 32)
+        : "memory");
+    return any != 0u;
+}
+
 // The slots of whole pairs (joined with a prefix) follow two for every CTA there may be.
 __device__ __forceinline__ int64_t whole_slots(const StreamArgs& a) { return 2 * (int64_t)kSharedWaves * a.ctas; }
 
@@ -504,12 +516,11 @@ __global__ void __launch_bounds__(kThreads, 2)
                 if (lane == 0) mbar_arrive(&empty[stage]);
                 if (++stage == NS) { stage = 0; phase ^= 1; }
             }
-            if (!alive) break;
 
             // ---- merge the four warps, in the memory of the stretch's last stage (the next tiles are on their way) ----
             float* red_o = reinterpret_cast<float*>(smem + stage * C::kStageBytes);   // [4][8][D + kPad]
-            asm volatile("bar.sync 1, %0;" ::"n"(kConsumerWarps * 32) : "memory");    // all have read that stage, and
-                                                                                       // the last stretch's statistics
+            // all have read that stage, and the last stretch's statistics; if one gave up a wait, all leave together
+            if (consumers_any(!alive)) break;
 #pragma unroll
             for (int off = 4; off < 32; off <<= 1) {
                 l[0] += __shfl_xor_sync(0xffffffffu, l[0], off);
