@@ -766,6 +766,8 @@ extern "C" int mllm_decode_attention_paged_kv8(const void* q, const mllm_paged_k
     if (n_rep > kMaxGroup) return fail(MLLM_ERR_UNSUPPORTED, "decode_attention_kv8: GQA group larger than 8");
     if (batch > 65535 || (int64_t)batch * num_heads > 0x3fffffff)
         return fail(MLLM_ERR_UNSUPPORTED, "decode_attention_kv8: more than 65535 sequences or 2^30 query rows");
+    if (max_kv_len > 0x7fffff00)
+        return fail(MLLM_ERR_UNSUPPORTED, "decode_attention_kv8: max_kv_len above 2^31 - 256");
     if (!(softmax_scale > 0.f) || !std::isfinite(softmax_scale))
         return fail(MLLM_ERR_INVALID_ARGUMENT, "decode_attention_kv8: softmax_scale must be positive");
     StreamArgs a = {};

@@ -551,6 +551,8 @@ extern "C" int mllm_decode_attention_shared_paged_bf16(const void* q, const mllm
     if (n_rep > kMaxGroup) return fail(MLLM_ERR_UNSUPPORTED, "decode_attention_shared: GQA group larger than 8");
     if (batch > 65535 || (int64_t)batch * num_heads > 0x3fffffff)
         return fail(MLLM_ERR_UNSUPPORTED, "decode_attention_shared: more than 65535 sequences or 2^30 query rows");
+    if (max_kv_len > 0x7fffff00)
+        return fail(MLLM_ERR_UNSUPPORTED, "decode_attention_shared: max_kv_len above 2^31 - 256");
     if (!(softmax_scale > 0.f) || !std::isfinite(softmax_scale))
         return fail(MLLM_ERR_INVALID_ARGUMENT, "decode_attention_shared: softmax_scale must be positive");
     StreamArgs a = {};

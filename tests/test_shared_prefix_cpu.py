@@ -64,6 +64,8 @@ def test_library_refusals():
     assert call(scale=-1.0) == 1 and call(q=None) == 1 and call(lens=None) == 1
     assert call(q=4104) == 1 and b"misaligned" in lib.mllm_attn_last_error()
     assert call(k_pool=None) == 1 and call(block_size=64) == 1 and call(B=70000) == 2
+    long = dict(max_blocks_per_seq=1 << 24, table_stride=1 << 24, L=0x7fffff01)
+    assert call(**long) == 2 and b"max_kv_len" in lib.mllm_attn_last_error() and call(**{**long, "L": 1 << 30}, ws=None) == 4
     assert call(ws=None) == 4 and call(ws=4104) == 4
     assert call(nb=size(2, 8, 2, 128, 100) - 1) == 4
     assert call(B=0) == 0
