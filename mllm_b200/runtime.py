@@ -935,6 +935,11 @@ def _decode_step_shared(q, k, v, cache: PagedKVCache, positions, rope_theta, num
     """decode_step over a cache whose sequences share their first rows: the epilogue appends at the device lengths,
     which then advance, and the attention reads the prefix once."""
     B, H, _, D = q.shape
+    pool = cache.k_pool.shape
+    if B > cache.block_table.shape[0] or pool[1] != num_kv_heads or pool[3] != D or k.shape != (B, num_kv_heads, 1, D) or \
+            v.shape != k.shape:
+        raise RuntimeError("decode_step: k, v and the cache must have num_kv_heads heads of q's head_dim, and a row per "
+                           "sequence")
     capturing = _capturing()
     if capturing and cache.capture_max_len is None:
         raise RuntimeError("decode_step: set the cache's capture_max_len before capturing a graph")
@@ -947,6 +952,10 @@ def _decode_step_shared(q, k, v, cache: PagedKVCache, positions, rope_theta, num
     if rope_table is not None:
         cos, sin = (t.to(torch.float32).contiguous() for t in rope_table)
         rsb = 0 if cos.shape[0] == 1 else 1
+        if cos.shape != sin.shape or tuple(cos.shape) not in ((1, D), (B, D)):
+            raise RuntimeError("RoPE: tables must be [1, D] or [B, D] in a decode step")
+    elif pos.numel() not in (1, B):
+        raise RuntimeError("RoPE: one position, or one per sequence, in a decode step")
     if qn is not None:
         qn, kn = qn.to(BF16).contiguous(), kn.to(BF16).contiguous()
     q_rot = torch.empty((B, H, D), dtype=BF16, device=q.device)

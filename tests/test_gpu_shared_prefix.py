@@ -230,3 +230,17 @@ def test_on_side_streams_at_once(rt):
             got.append(rt.decode_attention_shared(q, c, 8, 3000))
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+def test_a_step_refuses_what_does_not_fit_the_cache(rt):
+    c, lens = _shared_cache(rt, 200, [1, 2], 2, 64, 128, seed=9)
+    c.shared_prefix = 200
+    ok = dict(B=2, H=8, Hkv=2, D=64, kv=2, pos=[201])
+    for bad in (dict(B=3), dict(D=128), dict(Hkv=4, kv=4), dict(kv=4), dict(pos=[1, 2, 3]), dict(rows=3)):
+        a = {**ok, **bad}
+        q = torch.zeros(a["B"], a["H"], 1, a["D"], device="cuda", dtype=torch.bfloat16)
+        kv = torch.zeros(a["B"], a["kv"], 1, a["D"], device="cuda", dtype=torch.bfloat16)
+        table = tuple(torch.zeros(a["rows"], a["D"], device="cuda") for _ in range(2)) if "rows" in a else None
+        with pytest.raises(RuntimeError):
+            rt.decode_step(q, kv, kv, c, torch.tensor(a["pos"], device="cuda"), 1e4, a["Hkv"], rope_table=table)
+        assert c.host_lengths() == lens and c.lengths.tolist() == lens
