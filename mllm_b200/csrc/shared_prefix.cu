@@ -404,9 +404,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int64_t base = (((int64_t)split * a.Hkv + g) * a.B + (int64_t)qt * a.seqs) * a.n_rep;   // row 0's part
         const int rows = min(a.seqs, a.B - qt * a.seqs) * a.n_rep;            // valid rows of this query tile
         if (!alive) l_run = 0.f;
-        my_stat[0] = l_run != 0.f ? m_run : -INFINITY;
-        my_stat[1] = l_run;
-        asm volatile("bar.sync 1, 256;" ::: "memory");
+        asm volatile("bar.sync 1, 256;" ::: "memory");   // before it the other group's products may still read the tiles
+        if (!pair) {
+            my_stat[0] = l_run != 0.f ? m_run : -INFINITY;
+            my_stat[1] = l_run;
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+        }
         if (work) {
             float f = l_run != 0.f ? 1.f / l_run : 0.f, lse = l_run != 0.f ? m_run + log2f(l_run) : -INFINITY;
             if (!pair) {

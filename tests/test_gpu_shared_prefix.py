@@ -90,6 +90,23 @@ def test_against_64_bit_attention(rt, H, Hkv, D, prefix, suffix, block, qf):
     assert torch.equal(got, rt.decode_attention_shared(q, c, Hkv, prefix, max_kv_len=c.capacity))
 
 
+@pytest.mark.parametrize("H,Hkv,D,B", [(32, 8, 128, 13), (32, 8, 128, 40), (32, 4, 64, 9), (4, 4, 64, 1)])
+def test_one_call_after_another_at_many_prefix_lengths(rt, H, Hkv, D, B):
+    """Every number of tiles per stretch, odd and even, so that the two softmax groups of a CTA end at different times in
+    both orders; calls follow one another without a wait between them, in memory that held NaN."""
+    g = torch.Generator(device="cuda").manual_seed(21)
+    q = (1.5 * torch.randn(B, H, D, device="cuda", generator=g)).bfloat16()
+    for prefix in (200, 700, 1261, 1800, 2900, 4100, 6200, 8700, 10167, 13627):
+        c, lens = _shared_cache(rt, prefix, [1 + s % 9 for s in range(B)], Hkv, D, 384, seed=prefix)
+        held = torch.full((1 << 24,), float("nan"), device="cuda")   # what the workspaces lie in next
+        del held
+        got = [rt.decode_attention_shared(q, c, Hkv, prefix) for _ in range(10)]
+        _status_ok()
+        _check(c, q, got[0], lens, Hkv)
+        for x in got[1:]:
+            assert torch.equal(got[0], x)
+
+
 def test_any_part_of_the_common_rows_gives_the_same_answer(rt):
     """The prefix length is the caller's choice: 0 .. all rows in common, inside tiles and blocks."""
     c, lens = _shared_cache(rt, 600, [1, 50, 200], 2, 128, 256, seed=7)
