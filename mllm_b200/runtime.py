@@ -931,15 +931,34 @@ def _decode_step_kv8(q, k, v, cache: PagedKVCache8, positions, rope_theta, num_k
     return _decode_kv8(q_rot, cache, num_kv_heads, min(L, cache.capacity))
 
 
-def _decode_step_shared(q, k, v, cache: PagedKVCache, positions, rope_theta, num_kv_heads, qn, kn, eps, rope_table):
-    """decode_step over a cache whose sequences share their first rows: the epilogue appends at the device lengths,
-    which then advance, and the attention reads the prefix once."""
-    B, H, _, D = q.shape
+# Bytes of a prefix that reading it once has to save for the shared decode to pay for its launches: a step of 32 / 8 heads
+# of 128 takes 18 us with any short prefix against 11 to 15 us fused (up to 32 MB saved), 24 against 24 at 34 MB
+# (2 sequences, 8192 rows), 20 against 23 at 59 MB (8, 2048) and 51 against 236 at 2 GB (16, 32768).
+_SHARED_MIN_BYTES = 40 << 20
+
+
+def _shared_pays(B: int, prefix: int, num_kv_heads: int, D: int) -> bool:
+    return (B - 1) * prefix * num_kv_heads * D * 4 >= _SHARED_MIN_BYTES
+
+
+def _check_shared_step(q, k, v, cache: PagedKVCache, positions, num_kv_heads: int, rope_table) -> None:
+    B, _, _, D = q.shape
     pool = cache.k_pool.shape
     if B > cache.block_table.shape[0] or pool[1] != num_kv_heads or pool[3] != D or k.shape != (B, num_kv_heads, 1, D) or \
             v.shape != k.shape:
         raise RuntimeError("decode_step: k, v and the cache must have num_kv_heads heads of q's head_dim, and a row per "
                            "sequence")
+    if rope_table is not None:
+        if any(tuple(t.shape) not in ((1, D), (B, D)) for t in rope_table) or rope_table[0].shape != rope_table[1].shape:
+            raise RuntimeError("RoPE: tables must be [1, D] or [B, D] in a decode step")
+    elif positions.numel() not in (1, B):
+        raise RuntimeError("RoPE: one position, or one per sequence, in a decode step")
+
+
+def _decode_step_shared(q, k, v, cache: PagedKVCache, positions, rope_theta, num_kv_heads, qn, kn, eps, rope_table):
+    """decode_step over a cache whose sequences share their first rows: the epilogue appends at the device lengths,
+    which then advance, and the attention reads the prefix once."""
+    B, H, _, D = q.shape
     capturing = _capturing()
     if capturing and cache.capture_max_len is None:
         raise RuntimeError("decode_step: set the cache's capture_max_len before capturing a graph")
@@ -952,10 +971,6 @@ def _decode_step_shared(q, k, v, cache: PagedKVCache, positions, rope_theta, num
     if rope_table is not None:
         cos, sin = (t.to(torch.float32).contiguous() for t in rope_table)
         rsb = 0 if cos.shape[0] == 1 else 1
-        if cos.shape != sin.shape or tuple(cos.shape) not in ((1, D), (B, D)):
-            raise RuntimeError("RoPE: tables must be [1, D] or [B, D] in a decode step")
-    elif pos.numel() not in (1, B):
-        raise RuntimeError("RoPE: one position, or one per sequence, in a decode step")
     if qn is not None:
         qn, kn = qn.to(BF16).contiguous(), kn.to(BF16).contiguous()
     q_rot = torch.empty((B, H, D), dtype=BF16, device=q.device)
@@ -980,7 +995,8 @@ def decode_step(q, k, v, kv_cache: KVCache, positions: torch.Tensor, rope_theta:
     projections); positions int64 [1] (shared) or [B] / [B, 1].  The new rows go to slot
     lengths[b] of each sequence and the lengths advance by one.  Returns [B, 1, H*D].  A paged cache
     whose shared_prefix is set (every sequence begins with that many equal rows) is read by
-    decode_attention_shared, after an epilogue launch of its own."""
+    decode_attention_shared, after an epilogue launch of its own, where batch and prefix are large
+    enough for that to be faster."""
     for n, t in (("q", q), ("k", k), ("v", v)):
         _check_cuda_bf16(n, t)
         if t.dim() != 4 or t.size(2) != 1 or t.stride(3) != 1:
@@ -992,8 +1008,10 @@ def decode_step(q, k, v, kv_cache: KVCache, positions: torch.Tensor, rope_theta:
         return _decode_step_kv8(q, k, v, kv_cache, positions, rope_theta, num_kv_heads, q_norm_weight, k_norm_weight,
                                 eps, rope_table)
     if isinstance(kv_cache, PagedKVCache) and kv_cache.shared_prefix > 0:
-        return _decode_step_shared(q, k, v, kv_cache, positions, rope_theta, num_kv_heads, q_norm_weight, k_norm_weight,
-                                   eps, rope_table)
+        _check_shared_step(q, k, v, kv_cache, positions, num_kv_heads, rope_table)
+        if _shared_pays(B, kv_cache.shared_prefix, num_kv_heads, D):
+            return _decode_step_shared(q, k, v, kv_cache, positions, rope_theta, num_kv_heads, q_norm_weight,
+                                       k_norm_weight, eps, rope_table)
     pos = positions.to(torch.int64).reshape(-1)
     pos_sb = 0 if pos.numel() == 1 else pos.stride(0)
     cos = sin = None

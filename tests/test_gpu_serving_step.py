@@ -10,6 +10,7 @@ if not torch.cuda.is_available():
     pytest.skip("needs a GPU", allow_module_level=True)
 
 from mllm_b200 import abi  # noqa: E402
+from mllm_b200 import runtime as rt  # noqa: E402
 from mllm_b200.serving import ContinuousBatcher, DecoderModel, DecoderShape, LogitRules, apply_rules  # noqa: E402
 from tests.test_gpu_serving import _solo_logits  # noqa: E402
 
@@ -47,6 +48,47 @@ def test_shared_prefix_matches_solo_runs(plen, graphs):
         agree += int((ref.argmax(-1) == torch.tensor(t))[clear].sum())
         total += int(clear.sum())
     assert total > 0 and agree == total
+
+
+@pytest.mark.parametrize("graphs", [False, True])
+@pytest.mark.parametrize("plen", [1, 128, 300])
+def test_shared_prefix_read_once_matches_solo_runs(plen, graphs, monkeypatch):
+    """The same through decode_attention_shared, which decode_step leaves aside for batches and prefixes this small."""
+    calls = []
+    shared = rt.decode_attention_shared
+    monkeypatch.setattr(rt, "_SHARED_MIN_BYTES", 0)
+    monkeypatch.setattr(rt, "decode_attention_shared", lambda *a: calls.append(a[3]) or shared(*a))
+    test_shared_prefix_matches_solo_runs(plen, graphs)
+    assert calls and set(calls) == {plen}
+
+
+@pytest.mark.parametrize("B,prefix,used", [(4, 8192, True), (1, 8192, False), (4, 512, False)])
+def test_a_step_reads_the_prefix_once_where_that_pays(B, prefix, used, monkeypatch):
+    """decode_step on a cache with shared_prefix set against the step without it: bf16 outputs of two summation orders
+    (each within 2^-8 of the value and 2^-8 of the mean of |v| < 1, for P), twice."""
+    H, Hkv, D = 32, 8, 128
+    g = torch.Generator(device="cuda").manual_seed(B)
+    calls = []
+    shared = rt.decode_attention_shared
+    monkeypatch.setattr(rt, "decode_attention_shared", lambda *a: calls.append(a[3]) or shared(*a))
+    c = rt.PagedKVCache(num_blocks=prefix // 256 + 2 * B + 1, num_kv_heads=Hkv, head_dim=D, block_size=256, max_seqs=B,
+                        max_blocks_per_seq=prefix // 256 + 2)
+    c.k_pool.normal_(generator=g)
+    c.v_pool.uniform_(-1, 1, generator=g)
+    c.set_lengths([prefix])
+    for b in range(1, B):
+        c.fork(0, b, prefix)
+    q, k, v = (torch.randn(B, h, 1, D, device="cuda", generator=g).bfloat16() for h in (H, Hkv, Hkv))
+    v.clamp_(-1, 1)
+    pos = torch.tensor([prefix], device="cuda")
+    got = []
+    for shared_rows in (prefix, 0):
+        c.shared_prefix = shared_rows
+        c.set_lengths([prefix] * B)
+        got.append(rt.decode_step(q, k, v, c, pos, 1e6, Hkv).double())
+    abi.call("mllm_attn_device_status", None)
+    assert calls == ([prefix] if used else [])
+    assert ((got[0] - got[1]).abs() <= 2 * 2.0 ** -8 * (1 + got[1].abs())).all()
 
 
 @pytest.mark.parametrize("prefix_len", [0, 200])
