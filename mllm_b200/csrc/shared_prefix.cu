@@ -100,12 +100,15 @@ __host__ __device__ inline PrefixCut cut_prefix(int n_tiles, int sms, int pairs,
 
 // SMs per kv head for the prefix, so that it ends with the decode of the sequences' own rows on the other SMs: with P
 // and S the SM-microseconds of the two, F the fixed time of a prefix CTA and N SMs, X SMs take F + P / X, and all is
-// done after (P + S + F X) / N.  Fitted (D = 128): 1.8 us a tile for a pair, 0.9 for a single tile, 4 us for the CTA; 0.5 us
-// for a 64-row tile of the other kernel and 2 us of an SM for each of its CTAs.  D = 64 moves half.
+// done after (P + S + F X) / N.  Fitted (D = 128): 2.2 us a tile for a pair, 1.4 for a single tile (0.9 beside pairs), 4 us
+// for the CTA; 0.55 us for a 64-row tile of the other kernel and 1.8 us of an SM for each of its CTAs.  D = 64 moves half and
+// takes 0.4 of it.  Over 75 shapes timed at every X (2 to 128 sequences, prefixes of 512 to 24000 rows, 64 to 2000 own)
+// this X is 1.2 % off the best one on average and 13 % at most; too few SMs cost most (64 sequences of 40 heads behind
+// 32700 rows: 138 us with 9, 114 with 10, 115 with 11).
 __device__ __forceinline__ int prefix_sms(const PrefixArgs& a, float own_tiles, float dim_scale) {
     const float N = (float)a.num_sms, F = 4.f;
-    const float P = (float)a.Hkv * a.n_tiles * (1.8f * a.pairs + 0.9f * a.single) * dim_scale;
-    const float S = 0.5f * own_tiles * dim_scale + 2.f * fminf(own_tiles, 2.f * N);
+    const float P = (float)a.Hkv * a.n_tiles * (2.2f * a.pairs + (a.pairs ? 0.9f : 1.4f) * a.single) * dim_scale;
+    const float S = 0.55f * own_tiles * dim_scale + 1.8f * fminf(own_tiles, 2.f * N);
     const float b = P + S - N * F;
     const float X = (sqrtf(b * b + 4.f * F * N * P) - b) / (2.f * F);
     return max(1, min(a.num_sms / a.Hkv, (int)(X / a.Hkv + 0.5f)));
@@ -218,7 +221,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int own = total_tiles<kOwnTile>(st, lane);
         if (lane == 0) {
             s_holder = holder;
-            s_cut = cut_prefix(a.n_tiles, prefix_sms(a, (float)own, D == 128 ? 1.f : 0.6f), a.pairs, a.single);
+            s_cut = cut_prefix(a.n_tiles, prefix_sms(a, (float)own, D == 128 ? 1.f : 0.4f), a.pairs, a.single);
             if (blockIdx.x == 0 && blockIdx.y == 0) {
                 st.plan[kPlanPair] = s_cut.splits;
                 st.plan[kPlanSingle] = s_cut.splits_single;
