@@ -444,10 +444,10 @@ MLLM_API int mllm_decode_attention_paged_kv8(const void* q, const mllm_paged_kv8
 /* ----------------------------------------------------------------------------------------
  * Decode attention over a paged cache for a batch that shares a prefix: cache rows 0 ..
  * prefix_len - 1 are the same for every sequence of the call (a system prompt, a document) and are
- * read once for the whole batch, through the block-table row of the first sequence that is not empty; rows prefix_len .. kv_lens[b] - 1 are
- * each sequence's own, through its own table row.  The result is that of
- * mllm_decode_attention_paged_bf16 over caches that hold equal rows there; whether the tables share
- * the blocks or hold copies makes no difference.  prefix_len 0 is the plain decode.
+ * read once for the whole batch, through the block-table row of the first sequence that is not
+ * empty; rows prefix_len .. kv_lens[b] - 1 are each sequence's own, through its own table row.  The
+ * result is that of mllm_decode_attention_paged_bf16 over caches that hold equal rows there; whether
+ * the tables share the blocks or hold copies makes no difference.  prefix_len 0 is the plain decode.
  *   q, out, head_dim, group size, softmax_scale: as mllm_decode_attention_paged_bf16, q 16-byte
  *       aligned.  kv_lens: int32 device [batch], required, prefix_len <= kv_lens[b] <= max_kv_len;
  *       0 gives zeros; any other length records MLLM_ERR_DEVICE_LENGTH.
