@@ -662,7 +662,7 @@ def _epilogue_kv8_batch(q, k, v, cache: PagedKVCache8, positions, rope_theta, qn
         if pos.numel() == B * S:
             pos = pos.reshape(-1).contiguous()
         else:
-            pos = (pos.reshape(1, -1) if pos.dim() < 2 else pos).expand(B, S).reshape(-1)
+            pos = (pos.reshape(1, -1) if pos.dim() < 2 else pos).expand(B, S).reshape(-1).contiguous()   # of one position reshape makes a view
     cu = cache.one_each[:B + 1] if S == 1 else torch.arange(0, B * S + 1, S, dtype=torch.int32, device=q.device)
     qkv_epilogue_kv8(_flat_tokens(q), _flat_tokens(k), _flat_tokens(v), cache, cu, cache.lengths[:B], pos, rope_theta,
                      table, qn, kn, eps, out)

@@ -347,6 +347,18 @@ def test_bad_lengths_and_blocks_are_recorded(rt):
     _status_ok()
 
 
+def test_a_step_at_one_position_for_all(rt):
+    """positions [1] stands for every sequence's, as on the other caches."""
+    got = []
+    for pos in ([300], [300] * 3, [[300]] * 3):
+        c = _random_cache(rt, [300] * 3, 2, 128, 128, 1, seed=9)
+        q, k, v = (torch.randn(3, h, 1, 128, device="cuda", generator=torch.Generator(device="cuda").manual_seed(h)).bfloat16()
+                   for h in (8, 2, 2))
+        got.append(rt.decode_step(q, k, v, c, torch.tensor(pos, device="cuda"), 1e4, 2))
+    _status_ok()
+    assert torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])
+
+
 def test_a_negative_first_row_reads_nothing(rt):
     from mllm_b200 import abi
     c = _random_cache(rt, [300, 40], 2, 128, 128, 1, seed=9)
