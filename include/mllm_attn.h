@@ -461,6 +461,13 @@ MLLM_API int mllm_decode_attention_shared_paged_bf16(const void* q, const mllm_p
                                                      int head_dim, int max_kv_len, float softmax_scale, void* out,
                                                      void* workspace, size_t workspace_bytes, mllm_stream_t stream);
 
+/* The same over an 8-bit cache, whose rows stand for bf16 values: the result is that of
+ * mllm_decode_attention_paged_kv8.  Workspace as above. */
+MLLM_API int mllm_decode_attention_shared_paged_kv8(const void* q, const mllm_paged_kv8* kv, const int32_t* kv_lens,
+                                                    int prefix_len, int batch, int num_heads, int num_kv_heads,
+                                                    int head_dim, int max_kv_len, float softmax_scale, void* out,
+                                                    void* workspace, size_t workspace_bytes, mllm_stream_t stream);
+
 /* ----------------------------------------------------------------------------------------
  * Token sampling on the device.  Replaces src/core/runtime/Sampler.cpp:49-232
  * (Sampler::Sample) for `batch` logit rows at once, with no host round trip (the reference's

@@ -98,6 +98,7 @@ SIGNATURES = {
     "mllm_decode_attention_paged_kv8": (_i, [_p, _kv8, _p, _i, _i, _i, _i, _i, _f, _p, _p, _sz, _p]),
     "mllm_decode_attention_shared_workspace_size": (_sz, [_i, _i, _i, _i, _i]),
     "mllm_decode_attention_shared_paged_bf16": (_i, [_p, _kv, _p, _i, _i, _i, _i, _i, _i, _f, _p, _p, _sz, _p]),
+    "mllm_decode_attention_shared_paged_kv8": (_i, [_p, _kv8, _p, _i, _i, _i, _i, _i, _i, _f, _p, _p, _sz, _p]),
     "mllm_linear_workspace_size": (_sz, [_i, _i, C.POINTER(C.c_int64), _i64]),
     "mllm_linear_bf16": (_i, [_p, _i64, _i, _i64, _i, C.POINTER(C.c_void_p), C.POINTER(C.c_int64),
                               C.POINTER(C.c_int64), _p, _i64, _p, _sz, _p]),

@@ -739,6 +739,18 @@ int launch_stream_bf16(StreamArgs& a, int head_dim, const CUtensorMap& tmK, cons
                            : launch_stream_d<64, false>(a, Kv8View{}, tmK, tmV, num_sms, s);
 }
 
+int launch_stream_kv8(StreamArgs& a, int head_dim, const mllm_paged_kv8* kv, const Kv8View& view, int num_sms, cudaStream_t s) {
+    CUtensorMap tmK, tmV;
+    if (int st = encode_kv8_map(&tmK, kv->k_pool, head_dim, kv->block_size, a.Hkv, kv->num_blocks, kv->row_stride,
+                                kv->head_stride, kv->block_stride, kBoxRows))
+        return st;
+    if (int st = encode_kv8_map(&tmV, kv->v_pool, head_dim, kv->block_size, a.Hkv, kv->num_blocks, kv->row_stride,
+                                kv->head_stride, kv->block_stride, kBoxRows))
+        return st;
+    return head_dim == 128 ? launch_stream_d<128, true>(a, view, tmK, tmV, num_sms, s)
+                           : launch_stream_d<64, true>(a, view, tmK, tmV, num_sms, s);
+}
+
 MLLM_DEFINE_STATUS_READER(decode_stream)
 
 }  // namespace mllm_b200
@@ -783,13 +795,6 @@ extern "C" int mllm_decode_attention_paged_kv8(const void* q, const mllm_paged_k
                                         "mllm_decode_attention_kv8_workspace_size()");
     int num_sms = 0;
     if (int st = require_sm100(&num_sms)) return st;
-    CUtensorMap tmK, tmV;
-    if (int st = encode_kv8_map(&tmK, kv->k_pool, head_dim, kv->block_size, num_kv_heads, kv->num_blocks, kv->row_stride,
-                                kv->head_stride, kv->block_stride, kBoxRows))
-        return st;
-    if (int st = encode_kv8_map(&tmV, kv->v_pool, head_dim, kv->block_size, num_kv_heads, kv->num_blocks, kv->row_stride,
-                                kv->head_stride, kv->block_stride, kBoxRows))
-        return st;
     a.q = (const __nv_bfloat16*)q;
     a.kv_lens = kv_lens;
     a.out = (__nv_bfloat16*)out;
@@ -800,8 +805,6 @@ extern "C" int mllm_decode_attention_paged_kv8(const void* q, const mllm_paged_k
     a.max_len = max_kv_len;
     a.scale_log2 = (float)((double)softmax_scale * 1.4426950408889634);
     stream_place(a, workspace, head_dim, stream_part_rows(n_rep, batch, num_kv_heads, false));
-    if (int st = head_dim == 128 ? launch_stream_d<128, true>(a, view, tmK, tmV, num_sms, (cudaStream_t)stream)
-                                 : launch_stream_d<64, true>(a, view, tmK, tmV, num_sms, (cudaStream_t)stream))
-        return st;
+    if (int st = launch_stream_kv8(a, head_dim, kv, view, num_sms, (cudaStream_t)stream)) return st;
     return ok();
 }

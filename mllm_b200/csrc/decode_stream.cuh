@@ -115,8 +115,12 @@ size_t stream_part_rows(int n_rep, int batch, int num_kv_heads, bool shared);
 size_t stream_workspace_bytes(int D, size_t part_rows, int batch, int num_kv_heads);
 void stream_place(StreamArgs& a, void* workspace, int D, size_t part_rows);
 
-// Runs the split and the combine kernel over a bf16 paged cache.
+struct Kv8View;
+
+// Runs the split and the combine kernel over a bf16 paged cache, or an 8-bit one.
 int launch_stream_bf16(StreamArgs& a, int head_dim, const CUtensorMap& tmK, const CUtensorMap& tmV, int num_sms,
                        cudaStream_t s);
+int launch_stream_kv8(StreamArgs& a, int head_dim, const mllm_paged_kv8* kv, const Kv8View& view, int num_sms,
+                      cudaStream_t s);
 
 }  // namespace mllm_b200

@@ -898,14 +898,16 @@ def decode_attention_shared(q: torch.Tensor, kv_cache: PagedKVCache, num_kv_head
     rows (PagedKVCache.fork): the prefix is read once for the whole batch, through the table row of
     the first sequence that is not empty, every sequence's further rows through its own -> [B, 1, H*D].
     Lengths come from the cache (each at least prefix_len, or 0)."""
-    if not isinstance(kv_cache, PagedKVCache) or isinstance(kv_cache, PagedKVCache8):
-        raise RuntimeError("decode_attention_shared: needs a bf16 PagedKVCache")
+    if not isinstance(kv_cache, PagedKVCache):
+        raise RuntimeError("decode_attention_shared: needs a PagedKVCache or a PagedKVCache8")
     q, (B, H, D), dev, L = _decode_args(q, kv_cache, num_kv_heads, max_kv_len)
     device = q.device
     out = torch.empty_strided((B, 1, H * D), (H * D, H * D, 1), dtype=BF16, device=device)
     nbytes = _workspace_size("mllm_decode_attention_shared_workspace_size", B, H, num_kv_heads, D, prefix_len)
     ws = torch.empty_strided((nbytes,), (1,), dtype=torch.uint8, device=device)   # of the call's own, as in _decode_kv8
-    _launch(dev, "mllm_decode_attention_shared_paged_bf16", q.data_ptr(), C.byref(kv_cache.descriptor()),
+    name = "mllm_decode_attention_shared_paged_kv8" if isinstance(kv_cache, PagedKVCache8) else \
+        "mllm_decode_attention_shared_paged_bf16"
+    _launch(dev, name, q.data_ptr(), C.byref(kv_cache.descriptor()),
             kv_cache.lengths.data_ptr(), prefix_len, B, H, num_kv_heads, D, L, 1.0 / math.sqrt(D), out.data_ptr(),
             ws.data_ptr(), nbytes)
     return out
@@ -928,7 +930,10 @@ def _decode_step_kv8(q, k, v, cache: PagedKVCache8, positions, rope_theta, num_k
     else:
         cache.advance(1, batch=B)
         L = max(cache.host_lengths()[:B])
-    return _decode_kv8(q_rot, cache, num_kv_heads, min(L, cache.capacity))
+    L = min(L, cache.capacity)
+    if cache.shared_prefix > 0 and _shared_pays(B, cache.shared_prefix, num_kv_heads, D, True):
+        return decode_attention_shared(q_rot, cache, num_kv_heads, cache.shared_prefix, L)
+    return _decode_kv8(q_rot, cache, num_kv_heads, L)
 
 
 # Bytes of a prefix that reading it once has to save for the shared decode to pay for its launches: a step of 32 / 8 heads
@@ -937,8 +942,18 @@ def _decode_step_kv8(q, k, v, cache: PagedKVCache8, positions, rope_theta, num_k
 _SHARED_MIN_BYTES = 40 << 20
 
 
-def _shared_pays(B: int, prefix: int, num_kv_heads: int, D: int) -> bool:
-    return (B - 1) * prefix * num_kv_heads * D * 4 >= _SHARED_MIN_BYTES
+# Of an 8-bit cache, whose rows the shared form has to convert: 20 us against 26 with 130 MB saved (32 sequences, 2048
+# rows), 24 against 27 with 117 MB (8, 8192), 24 against 19 with 50 MB (4, 8192); and 52 against 45 with 200 MB for 4
+# sequences behind 32700 rows, where there are too few query rows to each converted one.
+_SHARED_MIN_BYTES8 = 100 << 20
+_SHARED_MIN_BATCH8 = 6
+
+
+def _shared_pays(B: int, prefix: int, num_kv_heads: int, D: int, kv8: bool = False) -> bool:
+    rows = (B - 1) * prefix * num_kv_heads * D
+    if kv8:
+        return B >= _SHARED_MIN_BATCH8 and rows * 2 >= _SHARED_MIN_BYTES8
+    return rows * 4 >= _SHARED_MIN_BYTES
 
 
 def _check_shared_step(q, k, v, cache: PagedKVCache, positions, num_kv_heads: int, rope_table) -> None:

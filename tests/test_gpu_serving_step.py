@@ -117,6 +117,17 @@ def test_8bit_caches_batched_and_alone(prefix_len):
     assert compared > 50
 
 
+def test_8bit_caches_with_the_prefix_read_once(monkeypatch):
+    """The same with the prefix read once, which decode_step leaves aside for batches and prefixes this small."""
+    calls = []
+    shared = rt.decode_attention_shared
+    monkeypatch.setattr(rt, "_SHARED_MIN_BYTES8", 0)
+    monkeypatch.setattr(rt, "_SHARED_MIN_BATCH8", 1)
+    monkeypatch.setattr(rt, "decode_attention_shared", lambda *a: calls.append(a[3]) or shared(*a))
+    test_8bit_caches_batched_and_alone(200)
+    assert calls and set(calls) == {200}
+
+
 @pytest.mark.parametrize("kv8,prefix_len", [(False, 0), (True, 150), (False, 150)])
 def test_rules_hold_for_their_request_only(kv8, prefix_len):
     """A grammar, penalties and biases on some of the requests: the picked tokens are the greedy ones of the recorded

@@ -211,8 +211,8 @@ def test_refusals(rt):
             rt.decode_attention_shared(q, c, 2, bad)
     with pytest.raises(RuntimeError, match="kv heads"):
         rt.decode_attention_shared(q, c, 4, 100)
-    with pytest.raises(RuntimeError, match="bf16"):
-        rt.decode_attention_shared(q, rt.PagedKVCache8(2, 2, 128, 128, 2), 2, 0)
+    with pytest.raises(RuntimeError, match="PagedKVCache"):
+        rt.decode_attention_shared(q, rt.KVCache(2, 2, 128, 16), 2, 0)
     with pytest.raises(RuntimeError, match="bfloat16"):
         rt.decode_attention_shared(q.float(), c, 2, 100)
 

@@ -71,3 +71,32 @@ def test_library_refusals():
     assert call(B=0) == 0
     assert size(2, 8, 2, 128, -1) == 0 and size(2, 7, 2, 128, 5) == 0
     assert size(2, 8, 2, 128, 0) < size(2, 8, 2, 128, 1) <= size(2, 8, 2, 128, 5000)
+
+
+def test_library_refusals_of_an_8bit_cache():
+    build.build()
+    lib = abi.load()
+    size = lib.mllm_decode_attention_shared_workspace_size
+
+    def call(B=2, H=8, Hkv=2, D=128, P=100, L=300, scale=0.1, q=4096, lens=4096, ws=4096, nb=1 << 40, **over):
+        d = dict(k_pool=4096, v_pool=4096, block_stride=2 * 128 * 128, head_stride=128 * 128, row_stride=128, k_exp=4096,
+                 v_exp=4096, exp_block_stride=256, exp_head_stride=128, num_blocks=4, block_size=128, block_table=4096,
+                 table_stride=4, max_blocks_per_seq=4)
+        d.update(over)
+        return lib.mllm_decode_attention_shared_paged_kv8(q, C.byref(abi.PagedKV8(**d)), lens, P, B, H, Hkv, D, L, scale,
+                                                          4096, ws, nb, None)
+    assert call(P=-1) == 1 and call(P=301) == 1 and b"prefix_len" in lib.mllm_attn_last_error()
+    assert call(H=7) == 1 and call(D=96) == 2 and call(H=18) == 2 and call(L=513, P=10) == 1
+    assert call(scale=-1.0) == 1 and call(q=None) == 1 and call(lens=None) == 1 and call(q=4104) == 1
+    assert call(k_exp=None) == 1 and call(k_pool=4104) == 1 and call(row_stride=130) == 1 and call(exp_head_stride=8) == 1
+    assert call(block_size=64) == 1 and call(B=70000) == 2
+    assert call(ws=None) == 4 and call(ws=4104) == 4 and call(nb=size(2, 8, 2, 128, 100) - 1) == 4
+    assert call(B=0) == 0
+
+
+def test_when_reading_the_prefix_once_pays():
+    pays = rt._shared_pays
+    for kv8 in (False, True):
+        assert not pays(1, 1 << 20, 8, 128, kv8) and not pays(32, 0, 8, 128, kv8) and not pays(32, 128, 8, 128, kv8)
+        assert pays(32, 8192, 8, 128, kv8) and pays(64, 32768, 8, 128, kv8)
+    assert pays(3, 8192, 8, 128) and not pays(3, 8192, 8, 128, True) and not pays(4, 32768, 8, 128, True)
