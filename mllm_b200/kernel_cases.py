@@ -10,6 +10,7 @@ Cases (Qwen3-8B attention geometry: 32 q heads, 8 kv heads, head_dim 128, hidden
              (5 q heads each): 8 is one GPU's share at 1 GPU, 1 at 8 GPUs
   decode8    decode over an 8-bit cache (stream_decode_kernel)
   shared     decode over --kv-len rows that B sequences share and --own rows of each (prefix_kernel, stream_decode_kernel)
+  shared8    the same over an 8-bit cache
   epilogue8  QK-RMSNorm + RoPE + quantising append of B x S tokens (kv8_epilogue_stream_kernel)
   logits     penalties, biases and a mask on B rows of Qwen3 logits (logit_rules_kernel)
   linear     q|k|v projection of T tokens, bf16 weights (linear_kernel)
@@ -81,8 +82,8 @@ def _decode(args, dev, g):
     return launch, {"batch": B, "kv_len": L, "bytes": 2 * B * HKV * L * D * 2}
 
 
-def _cache8(B, rows, dev, g):
-    cache = rt.PagedKVCache8(B * -(-rows // 256), HKV, D, max_seqs=B, device=dev)
+def _cache8(B, blocks, dev, g):
+    cache = rt.PagedKVCache8(blocks, HKV, D, max_seqs=B, device=dev)
     for pool in (cache.k_pool, cache.v_pool):
         pool.view(torch.uint8).random_(0, 127, generator=g)       # positive finite e4m3 values
     cache.k_exp.fill_(120)
@@ -92,7 +93,7 @@ def _cache8(B, rows, dev, g):
 
 def _decode8(args, dev, g):
     B, L = args.batch, args.kv_len
-    cache = _cache8(B, L, dev, g)
+    cache = _cache8(B, B * -(-L // 256), dev, g)
     cache.set_lengths([L] * B)
     q = torch.randn(B, H, D, device=dev, generator=g).bfloat16()
 
@@ -103,10 +104,14 @@ def _decode8(args, dev, g):
 
 def _shared(args, dev, g):
     B, P, own = args.batch, args.kv_len, args.own
-    bs = 256
-    cache = rt.PagedKVCache(P // bs + B * (own // bs + 2) + 1, HKV, D, bs, max_seqs=B, device=dev)
-    cache.k_pool.normal_(generator=g)
-    cache.v_pool.normal_(generator=g)
+    bs, kv8 = 256, args.case == "shared8"
+    blocks = P // bs + B * (own // bs + 2) + 1
+    if kv8:
+        cache = _cache8(B, blocks, dev, g)
+    else:
+        cache = rt.PagedKVCache(blocks, HKV, D, bs, max_seqs=B, device=dev)
+        cache.k_pool.normal_(generator=g)
+        cache.v_pool.normal_(generator=g)
     cache.reserve(0, P)
     for b in range(1, B):
         cache.fork(0, b, P)
@@ -115,7 +120,8 @@ def _shared(args, dev, g):
 
     def launch():
         rt.decode_attention_shared(q, cache, HKV, P)
-    return launch, {"batch": B, "prefix": P, "own": own, "bytes": 4 * HKV * D * (P + B * own),
+    return launch, {"batch": B, "prefix": P, "own": own,
+                    "bytes": 2 * HKV * (D + 1 if kv8 else 2 * D) * (P + B * own),
                     "flop": 4 * B * H * D * (P + own)}
 
 
@@ -125,7 +131,7 @@ def _epilogue8(args, dev, g):
     qkv = (torch.randn(T, row, device=dev, generator=g) * 0.5).bfloat16()
     q, k, v = (qkv[:, a:b].view(T, -1, D) for a, b in ((0, H * D), (H * D, (H + HKV) * D), ((H + HKV) * D, row)))
     gamma = (1 + 0.1 * torch.randn(D, device=dev, generator=g)).bfloat16()
-    cache = _cache8(B, S, dev, g)
+    cache = _cache8(B, B * -(-S // 256), dev, g)
     cache.set_lengths([S] * B)
     cu = torch.arange(0, T + 1, S, dtype=torch.int32, device=dev)
     start = torch.zeros(B, dtype=torch.int32, device=dev)
@@ -191,7 +197,7 @@ def _linear(args, dev, g, fp8):
     return launch, {"tokens": T, "bytes": nbytes, "ring": len(ring)}
 
 
-_OPERATORS = {"decode8": _decode8, "shared": _shared, "epilogue8": _epilogue8, "logits": _logits}
+_OPERATORS = {"decode8": _decode8, "shared": _shared, "shared8": _shared, "epilogue8": _epilogue8, "logits": _logits}
 
 
 def main(argv=None):
@@ -200,7 +206,7 @@ def main(argv=None):
     ap.add_argument("--batch", type=int, default=None)
     ap.add_argument("--seq", type=int, default=8192)
     ap.add_argument("--kv-len", type=int, default=4096)
-    ap.add_argument("--own", type=int, default=256, help="shared: rows of each sequence behind the prefix")
+    ap.add_argument("--own", type=int, default=256, help="shared, shared8: rows of each sequence behind the prefix")
     ap.add_argument("--tokens", type=int, default=32)
     ap.add_argument("--kv-heads", type=int, default=1,
                     help="ragged: kv heads (Qwen3-14B has 8); epilogue: kv heads with --heads")
@@ -215,7 +221,7 @@ def main(argv=None):
     if args.graph is None:
         args.graph = args.case in ("linear", "linear_fp8", "ragged", *_OPERATORS)
     if args.batch is None:
-        args.batch = 32 if args.case in ("decode", "decode8", "shared", "logits") else 4
+        args.batch = 32 if args.case in ("decode", "decode8", "shared", "shared8", "logits") else 4
     if not torch.cuda.is_available():
         raise SystemExit("kernel_cases: needs a CUDA device")
     dev = torch.device("cuda", 0)

@@ -19,7 +19,7 @@ a time (Scheduler.cpp:45-77).  Here requests of any length share the GPU:
     (`DecodeGraph`): one launch per step instead of several hundred;
   * a prefix that every request begins with (a system prompt) is prefilled once; the requests share
     its blocks (`PagedKVCache.fork`) and the decode step reads it once for the whole batch
-    (`mllm_decode_attention_shared_paged_bf16`);
+    where that pays (`mllm_decode_attention_shared_paged_bf16`, `..._kv8`);
   * a request may carry `LogitRules`: penalties, biases and a mask of allowed tokens, applied to its
     row of logits on the device (`mllm_logit_rules`) before the token is picked;
   * with kv8 the caches hold 8-bit rows (`runtime.PagedKVCache8`).
