@@ -128,3 +128,26 @@ def test_python_checks():
         rt.kv8_read(c, i, -1)
     with pytest.raises(RuntimeError, match="lens"):
         rt.kv8_read(c, i.long(), 3)
+
+
+def test_a_launch_for_another_device_makes_it_current_around_the_call(monkeypatch):
+    current = [0]
+    seen = []
+
+    class Device:
+        def __init__(self, dev):
+            self.dev = dev
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.dev
+
+        def __exit__(self, *exc):
+            current[0] = self.before
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: current[0], raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda dev: 100 + dev, raising=False)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(rt.abi, "stream_handle", lambda: 100 + current[0])
+    monkeypatch.setattr(rt.abi, "call", lambda name, *args: seen.append((current[0], name, args)))
+    rt._launch(0, "f", 1)
+    rt._launch(3, "g", 2)
+    assert seen == [(0, "f", (1, 100)), (3, "g", (2, 103))] and current == [0]
