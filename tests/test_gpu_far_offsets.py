@@ -100,6 +100,29 @@ def test_shared_prefix_with_blocks_far_apart(rt):
     _status_ok()
 
 
+def test_shared_prefix_of_8bit_blocks_far_apart(rt):
+    H, Hkv, D, P = 8, 2, 128, 300
+    near = rt.PagedKVCache8(12, Hkv, D, 128, 3, max_blocks_per_seq=4)
+    far = rt.PagedKVCache8(2 ** 33 // (Hkv * 128 * D) // 2 + 70, Hkv, D, 128, 3, max_blocks_per_seq=4)
+    assert far.k_pool.numel() > 2 ** 32
+    far._free.reverse()
+    pools = [[c.k_pool.view(torch.uint8), c.v_pool.view(torch.uint8), c.k_exp, c.v_exp] for c in (near, far)]
+    for t, lo, hi in zip(pools[0], (0, 0, 114, 119), (127, 127, 118, 123)):
+        t.copy_(torch.randint(lo, hi, t.shape, device="cuda").to(torch.uint8))
+    for c in (near, far):
+        c.reserve(0, P)
+        for b in (1, 2):
+            c.fork(0, b, P)
+        c.set_lengths([P + 3, P + 100, P])
+    for b in range(3):
+        for i, j in zip(near.blocks_of(b), far.blocks_of(b)):
+            for a, z in zip(*pools):
+                z[j] = a[i]
+    q = torch.randn(3, H, D, device="cuda").bfloat16()
+    assert torch.equal(rt.decode_attention_shared(q, near, Hkv, P), rt.decode_attention_shared(q, far, Hkv, P))
+    _status_ok()
+
+
 def test_logit_rows_far_apart(rt):
     V = 5000
     big = torch.zeros(FAR + V, dtype=torch.bfloat16, device="cuda")
