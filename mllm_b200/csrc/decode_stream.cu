@@ -173,7 +173,9 @@ __global__ void __launch_bounds__(kThreads, 2)
         mbar_fence_init();
     }
     // Behind a prefix kernel (shared) nothing here depends on that kernel, which has itself waited for
-    // everything before it and then let this grid start: the wait moves to the end of the kernel.
+    // everything before it and then let this grid start: lengths, tables and queries are complete, and
+    // no SM's L1 holds older ones, since it is emptied for a grid that starts.  The wait moves to the end of the
+    // kernel.  (A fence here as well took 60 us in place of 56 for 128 sequences behind 8192 rows.)
     if (!a.shared) pdl_wait();
     pdl_trigger();
     const int pairs = a.B * a.Hkv;
@@ -611,11 +613,14 @@ __global__ void __launch_bounds__(kCombineWarps * 32) stream_combine_kernel(Stre
     const int bh = blockIdx.x * kCombineWarps + (threadIdx.x >> 5);
     if (bh >= a.B * a.H) return;
     const int b = bh / a.H, h = bh - b * a.H, g = h / a.n_rep, r = h - g * a.n_rep;
+    // The length does not come from the kernel before this one, which let this grid in after its own wait for whatever
+    // wrote it (so L2 has it); all that does is loaded together.
+    const SeqTiles s = seq_tiles<TILE>(a, b, true);
     pdl_wait();
     const int per = a.plan[kPlanPer], p0 = a.plan[kPlanHead + b * a.Hkv + g];   // p0 means nothing without tiles
+    const int pre = a.shared ? a.plan[b < a.pair_seqs ? kPlanPair : kPlanSingle] : 0;
     if (per == 0) return;                 // every pair had a CTA of its own
-    const SeqTiles s = seq_tiles<TILE>(a, b);
-    const int n_pre = !a.shared || s.short_len ? 0 : a.plan[b < a.pair_seqs ? kPlanPair : kPlanSingle];
+    const int n_pre = s.short_len ? 0 : pre;
     int c0 = s.tiles ? p0 / per : 0;
     int own = s.tiles ? (p0 + s.tiles - 1) / per - c0 + 1 : 0;
     if (s.tiles && (p0 < 0 || c0 + own > kSharedWaves * a.ctas)) {   // the pair's place was never written: its CTA

@@ -42,9 +42,9 @@ struct SeqTiles {
 };
 
 template <int TILE>
-__device__ __forceinline__ SeqTiles seq_tiles(const StreamArgs& a, int b) {
+__device__ __forceinline__ SeqTiles seq_tiles(const StreamArgs& a, int b, bool from_l2 = false) {
     SeqTiles s;
-    int len = a.kv_lens[b];
+    int len = from_l2 ? __ldcg(a.kv_lens + b) : a.kv_lens[b];
     if (len < 0 || len > a.max_len || (len > 0 && len < a.first_row)) {
         record_error(kErrBadLength);
         len = len < 0 ? 0 : min(len, a.max_len);

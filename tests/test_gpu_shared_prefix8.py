@@ -270,3 +270,41 @@ def test_a_step_reads_the_prefix_once_where_that_pays(rt, B, prefix, used, monke
     _status_ok()
     assert calls == ([prefix] if used else [])
     assert ((got[0] - got[1]).abs() <= 2 * 2.0 ** -8 * (1.75 + got[1].abs())).all()
+
+
+@pytest.mark.parametrize("kv8", [True, False])
+@pytest.mark.parametrize("H,Hkv,D,B,prefix", [(8, 2, 128, 3, 300), (32, 4, 64, 40, 700), (4, 4, 64, 1, 64)])
+def test_queries_that_the_kernel_before_has_just_written(rt, H, Hkv, D, B, prefix, kv8):
+    """The epilogue writes new queries into the same memory again and again, the decode reads them behind it: launches that
+    all start early and wait for one another.  Every result is the one with a wait for the device before each call."""
+    N = 40
+    c, lens = _cache(rt, prefix, [1 + s % 9 for s in range(B)], Hkv, D, 128, seed=3)
+    if not kv8:
+        c = _read_back(rt, c, prefix, lens)
+    appends = rt.PagedKVCache8(num_blocks=B, num_kv_heads=Hkv, head_dim=D, block_size=128, max_seqs=B)   # not looked at
+    for b in range(B):
+        appends.reserve(b, 1)
+    cu = torch.arange(B + 1, dtype=torch.int32, device="cuda")
+    start = torch.zeros(B, dtype=torch.int32, device="cuda")
+    pos = torch.arange(B, device="cuda")
+    x = torch.randn(N, B, H + 2 * Hkv, D, device="cuda").bfloat16()
+    q = torch.empty(B, H, D, device="cuda", dtype=torch.bfloat16)
+
+    def step(i):
+        rt.qkv_epilogue_kv8(x[i, :, :H], x[i, :, H:H + Hkv], x[i, :, H + Hkv:], appends, cu, start, pos, 1e4, out=q)
+        return rt.decode_attention_shared(q, c, Hkv, prefix, max_kv_len=max(lens))
+    want = []
+    for i in range(N):
+        torch.cuda.synchronize()
+        want.append(step(i).clone())
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        recorded = [step(i) for i in range(N)]
+    for _ in range(5):
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(recorded, want))
+        again = [step(i) for i in range(N)]
+        assert all(torch.equal(a, b) for a, b in zip(again, want))
+    _status_ok()
