@@ -1074,21 +1074,17 @@ def decode_step(q, k, v, kv_cache: KVCache, positions: torch.Tensor, rope_theta:
     return out
 
 
-def _rows(name: str, t: torch.Tensor, B: int, dtype, dev: int) -> torch.Tensor:
-    """A [B, n] tensor on device number `dev` whose rows are contiguous; a copy of it where the rows overlap (an
-    expanded one)."""
-    if t.get_device() != dev or t.dtype is not dtype or t.dim() != 2 or t.size(0) != B or \
-            (t.size(1) > 1 and t.stride(1) != 1):
+def _rows(name: str, t: torch.Tensor, B: int, dtype, dev: int):
+    """A [B, n] tensor on device number `dev` whose rows are contiguous, or a copy of it where the rows overlap (an
+    expanded one): (the tensor, its row stride, n).  The stride of a single row means nothing."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 2 or shape[0] != B or t.dtype is not dtype or t.get_device() != dev or \
+            (shape[1] > 1 and stride[1] != 1):
         raise RuntimeError(f"{name}: expected a {dtype} [{B}, n] tensor with contiguous rows on cuda:{dev}")
-    return t if B < 2 or t.stride(0) >= t.size(1) else t.contiguous()
-
-
-def _rows_args(t: torch.Tensor | None):
-    """(pointer, row stride, columns); the stride of a single row means nothing."""
-    if t is None:
-        return None, 0, 0
-    n = t.size(1)
-    return t.data_ptr(), max(t.stride(0), n), n
+    n = shape[1]
+    if stride[0] >= n:
+        return t, stride[0], n
+    return t if B < 2 else t.contiguous(), n, n
 
 
 MAX_LOGIT_BIASES = 1024
@@ -1115,11 +1111,12 @@ def apply_logit_rules(logits: torch.Tensor, history=None, history_lens=None, out
         raise RuntimeError("logit rules: logits must be [B, V]")
     B, V = shape = logits.shape
     dev = logits.get_device()
-    logits = _rows("logits", logits, B, dtype, dev)
+    logits, x_stride, _ = _rows("logits", logits, B, dtype, dev)
     if (history is None) != (history_lens is None):
         raise RuntimeError("logit rules: give both history and history_lens or neither")
+    hist_stride = hist_cols = bias_stride = bias_cols = words_stride = 0
     if history is not None:
-        history = _rows("history", history, B, torch.int64, dev)
+        history, hist_stride, hist_cols = _rows("history", history, B, torch.int64, dev)
         _check_vec("history_lens", history_lens, B, torch.int32, dev)
     if output_start is not None:
         _check_vec("output_start", output_start, B, torch.int32, dev)
@@ -1130,36 +1127,36 @@ def apply_logit_rules(logits: torch.Tensor, history=None, history_lens=None, out
     if frequency is not None:
         _check_vec("frequency", frequency, B, torch.float32, dev)
     if bias_ids is not None and bias_values is not None and bias_lens is not None:
-        bias_ids = _rows("bias_ids", bias_ids, B, torch.int64, dev)
-        bias_values = _rows("bias_values", bias_values, B, torch.float32, dev)
+        bias_ids, bias_stride, bias_cols = _rows("bias_ids", bias_ids, B, torch.int64, dev)
+        bias_values, stride, n = _rows("bias_values", bias_values, B, torch.float32, dev)
         _check_vec("bias_lens", bias_lens, B, torch.int32, dev)
-        if bias_values.shape != bias_ids.shape:
+        if n != bias_cols:
             raise RuntimeError("logit rules: bias_ids and bias_values must have the same shape")
-        if B > 1 and bias_values.stride(0) != bias_ids.stride(0):
-            bias_ids, bias_values = bias_ids.contiguous(), bias_values.contiguous()
+        if stride != bias_stride:
+            bias_ids, bias_values, bias_stride = bias_ids.contiguous(), bias_values.contiguous(), n
     if allowed is not None:
-        allowed = _rows("allowed", allowed, B, torch.int32, dev)
-        if allowed.size(1) < (V + 31) // 32:
+        allowed, words_stride, n = _rows("allowed", allowed, B, torch.int32, dev)
+        if n < (V + 31) // 32:
             raise RuntimeError("logit rules: allowed needs ceil(V / 32) words a row")
-    if history is not None and history.size(1) == 0:
+    if history is not None and hist_cols == 0:
         history = history_lens = output_start = repetition = presence = frequency = None
-    if bias_ids is not None and bias_ids.size(1) == 0:
+    if bias_ids is not None and bias_cols == 0:
         bias_ids = bias_values = bias_lens = None
     if out is None:
         out = torch.empty_strided(shape, (V, 1), dtype=dtype, device=logits.device)
-    elif out.shape != shape or out.dtype is not dtype or out.get_device() != dev or (V > 1 and out.stride(1) != 1) or \
-            (B > 1 and out.stride(0) < V):
-        raise RuntimeError("logit rules: out must be like logits, its rows apart")
+        y_stride = V
+    else:
+        y_stride, step = out.stride() if out.dim() == 2 else (0, 0)
+        if out.shape != shape or out.dtype is not dtype or out.get_device() != dev or (V > 1 and step != 1) or \
+                (B > 1 and y_stride < V):
+            raise RuntimeError("logit rules: out must be like logits, its rows apart")
+        y_stride = max(y_stride, V)
     if B == 0 or V == 0:
         return out
-    x, x_stride, _ = _rows_args(logits)
-    hist, hist_stride, hist_cols = _rows_args(history)
-    ids, bias_stride, bias_cols = _rows_args(bias_ids)
-    words, words_stride, _ = _rows_args(allowed)
-    y, y_stride, _ = _rows_args(out)
-    _launch(dev, "mllm_logit_rules", x, int(dtype is BF16), x_stride, B, V, hist, hist_stride, hist_cols, _ptr(history_lens),
-            _ptr(output_start), _ptr(repetition), _ptr(presence), _ptr(frequency), ids, _ptr(bias_values), bias_stride,
-            bias_cols, _ptr(bias_lens), words, words_stride, y, y_stride)
+    _launch(dev, "mllm_logit_rules", logits.data_ptr(), int(dtype is BF16), x_stride, B, V, _ptr(history), hist_stride,
+            hist_cols, _ptr(history_lens), _ptr(output_start), _ptr(repetition), _ptr(presence), _ptr(frequency),
+            _ptr(bias_ids), _ptr(bias_values), bias_stride, bias_cols, _ptr(bias_lens), _ptr(allowed), words_stride,
+            out.data_ptr(), y_stride)
     return out
 
 
