@@ -16,8 +16,9 @@
 // summed in list order by the thread that owns the token.
 //
 // Bound: HBM, the row read and written once, behind the counting: 64 rows of 151936 fp32 logits with up to 5000 tokens of
-// history, 40 biases and a mask take 16.3 us, 80 MB at 4.9 TB/s, and with 100 tokens of history 12.7; without any rule
-// 9 us (the rows then lie in L2).  128 rows, which L2 does not hold, take 39.4 us, 161 MB at 4.1 TB/s.
+// history, 40 biases and a mask take 16.5 us, 80 MB at 4.8 TB/s, and with 100 tokens of history 13.7.  128 rows take
+// 40 us, 161 MB at 4.0 TB/s.  The logits are read as data that is not needed again, so that L2 keeps what is written: with
+// plain loads 64 rows that L2 does not hold took 19.6 us, 16.1 where it does either way.
 #include <algorithm>
 #include <cmath>
 
@@ -107,7 +108,7 @@ __global__ void __launch_bounds__(kThreads, kMinCtas) logit_rules_kernel(RuleArg
     auto load = [&](int i0) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (i0 + u * kThreads < nv) next_w[u] = reinterpret_cast<const uint4*>(x)[i0 + u * kThreads];
+            if (i0 + u * kThreads < nv) next_w[u] = __ldcs(reinterpret_cast<const uint4*>(x) + i0 + u * kThreads);
     };
     load(t);
     const int n_hist = hist ? checked_len(a.hist_lens, row, a.hist_cols) : 0;
