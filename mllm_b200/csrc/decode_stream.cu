@@ -621,13 +621,8 @@ __global__ void __launch_bounds__(kCombineWarps * 32) stream_combine_kernel(Stre
     const int pre = a.shared ? a.plan[b < a.pair_seqs ? kPlanPair : kPlanSingle] : 0;
     if (per == 0) return;                 // every pair had a CTA of its own
     const int n_pre = s.short_len ? 0 : pre;
-    int c0 = s.tiles ? p0 / per : 0;
-    int own = s.tiles ? (p0 + s.tiles - 1) / per - c0 + 1 : 0;
-    if (s.tiles && (p0 < 0 || c0 + own > kSharedWaves * a.ctas)) {   // the pair's place was never written: its CTA
-                                                                      // gave up a wait
-        record_error(kErrTimeout);
-        c0 = own = 0;
-    }
+    int c0, own;
+    if (!own_parts(p0, s.tiles, per, most_ctas(a.ctas, a.shared), &c0, &own)) record_error(kErrTimeout);
     if (own == 1 && n_pre == 0) return;   // written directly
     const int n = own + n_pre;            // 0: nothing to attend to
     auto part = [&](int i) -> int64_t {   // index of part i's row in part_o and part_lse

@@ -109,6 +109,22 @@ __device__ __forceinline__ int tiles_per_cta(const StreamArgs& a, int total) {
     return max((total + n - 1) / n, 1);
 }
 
+// The CTAs whose stretches hold a pair's tiles, from its first tile p0 on the line of tiles: first .. first + count - 1.
+// `ctas` is the most there can be, which the workspace has slots for.  False where p0 is not a place on that line: it was
+// never written, since the CTA that the pair begins in gave up a wait, and the workspace may hold anything there.
+__host__ __device__ __forceinline__ bool own_parts(int p0, int tiles, int per, int ctas, int* first, int* count) {
+    *first = *count = 0;
+    if (tiles == 0) return true;
+    const int64_t last = ((int64_t)p0 + tiles - 1) / per;
+    if (p0 < 0 || last >= ctas) return false;
+    *first = p0 / per;
+    *count = (int)last - *first + 1;
+    return true;
+}
+
+// CTAs that the tiles may be dealt to: those that the workspace has slots for.
+__host__ __device__ __forceinline__ int most_ctas(int ctas, int shared) { return shared ? kSharedWaves * ctas : ctas; }
+
 // The workspace: `part_rows` rows of D floats, their weights, the plan.
 // Rows of parts the even-split decode writes: two slots a CTA, and with a shared prefix one per pair.
 size_t stream_part_rows(int n_rep, int batch, int num_kv_heads, bool shared);
