@@ -172,11 +172,11 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
         mbar_fence_init();
     }
-    // Behind a prefix kernel (shared) nothing here depends on that kernel, which has itself waited for
-    // everything before it and then let this grid start: lengths, tables and queries are complete, and
-    // no SM's L1 holds older ones, since it is emptied for a grid that starts.  The wait moves to the end of the
-    // kernel.  (A fence here as well took 60 us in place of 56 for 128 sequences behind 8192 rows.)
-    if (!a.shared) pdl_wait();
+    // Behind a prefix kernel (shared) nothing here depends on that kernel's results, but lengths, tables, queries and rows
+    // come from what ran before it.  It has waited for that, and published its ticket, before it let this grid in: a
+    // thread that reads the ticket back (an acquire) is ordered behind that wait and goes on beside the prefix kernel; one
+    // that does not waits for the prefix kernel itself.
+    if (!a.shared || !ticket_published(a)) pdl_wait();
     pdl_trigger();
     const int pairs = a.B * a.Hkv;
     if (a.direct) {
@@ -251,6 +251,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         if (lane == 0 && w.left > 0) {
             tma_prefetch_desc(&tmK);
             tma_prefetch_desc(&tmV);
+            if (a.shared) asm volatile("fence.proxy.async.global;" ::: "memory");   // the rows too come behind the ticket
             int stage = 0;
             uint32_t phase = 0;
             bool alive = true;
@@ -613,10 +614,9 @@ __global__ void __launch_bounds__(kCombineWarps * 32) stream_combine_kernel(Stre
     const int bh = blockIdx.x * kCombineWarps + (threadIdx.x >> 5);
     if (bh >= a.B * a.H) return;
     const int b = bh / a.H, h = bh - b * a.H, g = h / a.n_rep, r = h - g * a.n_rep;
-    // The length does not come from the kernel before this one, which let this grid in after its own wait for whatever
-    // wrote it (so L2 has it); all that does is loaded together.
-    const SeqTiles s = seq_tiles<TILE>(a, b, true);
     pdl_wait();
+    if (a.shared && blockIdx.x == 0 && threadIdx.x == 0) *a.ready = 0ull;
+    const SeqTiles s = seq_tiles<TILE>(a, b);
     const int per = a.plan[kPlanPer], p0 = a.plan[kPlanHead + b * a.Hkv + g];   // p0 means nothing without tiles
     const int pre = a.shared ? a.plan[b < a.pair_seqs ? kPlanPair : kPlanSingle] : 0;
     if (per == 0) return;                 // every pair had a CTA of its own
@@ -694,12 +694,15 @@ size_t stream_part_rows(int n_rep, int batch, int num_kv_heads, bool shared) {
     return (2 * (size_t)kMaxCtas * (shared ? kSharedWaves : 1) + (shared ? (size_t)batch * num_kv_heads : 0)) * n_rep;
 }
 
+constexpr size_t kTicketBytes = 16;   // keeps the parts' alignment
+
 size_t stream_workspace_bytes(int D, size_t part_rows, int batch, int num_kv_heads) {
-    return (part_rows * (size_t)(D + 1) * 4 + (kPlanHead + (size_t)batch * num_kv_heads) * 4 + 255) & ~size_t(255);
+    return (kTicketBytes + part_rows * (size_t)(D + 1) * 4 + (kPlanHead + (size_t)batch * num_kv_heads) * 4 + 255) & ~size_t(255);
 }
 
 void stream_place(StreamArgs& a, void* workspace, int D, size_t part_rows) {
-    a.part_o = static_cast<float*>(workspace);
+    a.ready = static_cast<unsigned long long*>(workspace);
+    a.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + kTicketBytes);
     a.part_lse = a.part_o + part_rows * D;
     a.plan = reinterpret_cast<int*>(a.part_lse + part_rows);
 }

@@ -32,7 +32,21 @@ struct StreamArgs {
     int shared;                    // there is a prefix, and its kernel let this grid in
     int pair_seqs;
     int64_t prefix_base;
+    // The prefix kernel waits for all that ran before the call, then publishes `ticket` here, a number of this call only;
+    // whoever reads it back is ordered behind that wait.  The joining kernel clears it, for a graph's next replay.
+    unsigned long long* ready;
+    unsigned long long ticket;
 };
+
+__device__ __forceinline__ void publish_ticket(const StreamArgs& a) {
+    asm volatile("st.release.gpu.global.u64 [%0], %1;" ::"l"(a.ready), "l"(a.ticket) : "memory");
+}
+
+__device__ __forceinline__ bool ticket_published(const StreamArgs& a) {
+    unsigned long long t;
+    asm volatile("ld.acquire.gpu.global.u64 %0, [%1];" : "=l"(t) : "l"(a.ready) : "memory");
+    return t == a.ticket;
+}
 
 // Rows [first_row, len) of a sequence in tiles of TILE cache rows.  A length outside [0, max_len] is recorded and
 // clamped; a sequence shorter than the prefix (an empty one too) has no rows here, and no prefix either.
@@ -42,9 +56,9 @@ struct SeqTiles {
 };
 
 template <int TILE>
-__device__ __forceinline__ SeqTiles seq_tiles(const StreamArgs& a, int b, bool from_l2 = false) {
+__device__ __forceinline__ SeqTiles seq_tiles(const StreamArgs& a, int b) {
     SeqTiles s;
-    int len = from_l2 ? __ldcg(a.kv_lens + b) : a.kv_lens[b];
+    int len = a.kv_lens[b];
     if (len < 0 || len > a.max_len || (len > 0 && len < a.first_row)) {
         record_error(kErrBadLength);
         len = len < 0 ? 0 : min(len, a.max_len);
@@ -125,7 +139,7 @@ __host__ __device__ __forceinline__ bool own_parts(int p0, int tiles, int per, i
 // CTAs that the tiles may be dealt to: those that the workspace has slots for.
 __host__ __device__ __forceinline__ int most_ctas(int ctas, int shared) { return shared ? kSharedWaves * ctas : ctas; }
 
-// The workspace: `part_rows` rows of D floats, their weights, the plan.
+// The workspace: the ticket, `part_rows` rows of D floats, their weights, the plan.
 // Rows of parts the even-split decode writes: two slots a CTA, and with a shared prefix one per pair.
 size_t stream_part_rows(int n_rep, int batch, int num_kv_heads, bool shared);
 size_t stream_workspace_bytes(int D, size_t part_rows, int batch, int num_kv_heads);

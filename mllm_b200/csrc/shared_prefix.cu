@@ -27,6 +27,8 @@
 //
 // P is bf16 for the second product (A and B of an MMA have one type, and V is bf16); sums and O are fp32.
 #include <algorithm>
+#include <atomic>
+#include <chrono>
 #include <cmath>
 #include <type_traits>
 
@@ -315,6 +317,8 @@ __global__ void __launch_bounds__(Split<k8>::kThreads, 1)
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
     pdl_wait();
+    // what ran before the call is complete: say so to the decode of the sequences' own rows, which runs beside this grid
+    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) publish_ticket(st);
     // ---- the plan, the same in every CTA: from the tiles that the other kernel will find ----
     __shared__ PrefixCut s_cut;
     __shared__ int s_holder;
@@ -617,6 +621,18 @@ size_t shared_part_rows(int B, int H, int Hkv, int prefix) {
     return stream_part_rows(n_rep, B, Hkv, true) + parts * Hkv * B * n_rep;
 }
 
+// A number that no other call of this process has, and that bytes left in a workspace do not hold by chance: a counter
+// through a bijection of 64 bits (the finaliser of splitmix64, Steele, Lea and Flood 2014).
+unsigned long long next_ticket() {
+    static std::atomic<unsigned long long> calls{
+        (unsigned long long)std::chrono::steady_clock::now().time_since_epoch().count() << 20};
+    unsigned long long z = calls.fetch_add(1, std::memory_order_relaxed) * 0x9E3779B97F4A7C15ull;
+    z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
+    z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
+    z ^= z >> 31;
+    return z != 0ull ? z : next_ticket();   // 0 is what a call leaves behind
+}
+
 struct PrefixMaps {
     CUtensorMap q, k, v, v_end;   // of an 8-bit cache q only
 };
@@ -727,6 +743,7 @@ int decode_shared(const char* who, const void* q, const mllm_paged_kv* kv16, con
         pa.lay = a.lay;
         a.pair_seqs = 2 * p.pairs * p.seqs;
         a.shared = 1;
+        a.ticket = next_ticket();
         int st;
         if (head_dim == 128)
             st = p.pairs ? launch_prefix_d<128, true, k8>(pa, a, p, m, view, s)
