@@ -9,8 +9,8 @@
 //
 // e is the smallest integer in [kExpMin, kExpMax] with max|row| <= 448 * 2^e, the maximum taken over the
 // row's finite elements.  Below 2^kExpMin * 2^-9 elements become zero; the bound keeps 2^e and 2^-e normal
-// fp32 numbers and value * 2^e a normal bf16 number.  A non-finite element is stored as NaN (the format
-// has no infinity, and saturating one would hide it).
+// fp32 numbers and value * 2^e a normal bf16 number; for the latter, elements above kRowMax are stored as that.  A
+// non-finite element is stored as NaN (the format has no infinity, and saturating one would hide it).
 #pragma once
 
 #include <cuda_fp16.h>
@@ -26,6 +26,7 @@ namespace mllm_b200 {
 
 constexpr int kExpMin = -100;
 constexpr int kExpMax = 120;
+constexpr float kRowMax = 240.f * 0x1p120f;   // 256 * 2^120 is beyond bf16's largest number
 
 // 2^e for -126 <= e <= 127.
 __device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }

@@ -152,16 +152,21 @@ __device__ __forceinline__ void store_row8(float (&lo)[8], float (&hi)[8], unsig
     for (int e = 0; e < 8; ++e) top = fmax3_abs_nan(lo[e], hi[e], top);
 #pragma unroll
     for (int o = LPR / 2; o > 0; o >>= 1) top = fmax3_abs_nan(top, __shfl_xor_sync(gmask, top, o), 0.f);
-    const bool odd = !(top < INFINITY);   // the row (the group's lanes agree) has elements that are not finite
+    // The row (the group's lanes agree) has elements that are not finite, or that would be rounded to 256 * 2^kExpMax,
+    // which is no bf16 number.
+    const bool odd = !(top < 248.f * 0x1p120f);
     if (odd) {
-        // they are stored as NaN (the conversion would saturate an infinity), the others as if they were not there
+        // the former are stored as NaN (the conversion would saturate an infinity), the others as if they were not there;
+        // the latter as the largest that is one
         top = 0.f;
+        auto hold = [&](float& x) {
+            if (fabsf(x) < INFINITY) x = fminf(fmaxf(x, -kRowMax), kRowMax), top = fmaxf(top, fabsf(x));
+            else x = NAN;
+        };
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            if (fabsf(lo[e]) < INFINITY) top = fmaxf(top, fabsf(lo[e]));
-            else lo[e] = NAN;
-            if (fabsf(hi[e]) < INFINITY) top = fmaxf(top, fabsf(hi[e]));
-            else hi[e] = NAN;
+            hold(lo[e]);
+            hold(hi[e]);
         }
 #pragma unroll
         for (int o = LPR / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(gmask, top, o));
