@@ -20,10 +20,12 @@
 // rows; one byte permute sorts them, and output columns 2i and 2i + 1 land in the two row halves of the MMA.
 // q is scaled per head by a power of two into the range of a half (exact for elements within 2^-27 of the head's
 // largest; smaller ones lose bits that lie 2^-40 below it) and the scale is taken out of S in fp32.
-// Row scales: S gets 2^ek before the softmax.  2^ev multiplies P, so P^T = exp2(s + ev - mo) with mo the running
-// maximum of s + ev: the largest weight times scale is 1 and none overflows a half, however the rows' scales
-// differ; the sum l uses exp2(s - m) with its own maximum in fp32.  P is rounded to a half (2^-11), to bf16 for a
-// bf16 cache, since A and B of an MMA have one type; both sums stay fp32.
+// Row scales: S gets 2^ek before the softmax.  2^ev multiplies P, so P^T = exp2(s + ev - mo + 15) with mo the running
+// maximum of s + ev: the largest weight times scale is 2^15, the top of a half's range (65504), and none overflows it,
+// however the rows' scales differ; the merge takes the 2^15 out.  With the largest at 1, what lies 2^-25 below it would
+// become zero here but not in the sum l: with one dominant row, 2^18 others behind it in a warp lost 0.6 % of the output.
+// Now that takes 2^-40.  The sum l uses exp2(s - m) with its own maximum in fp32.  P is rounded to a half (2^-11), to
+// bf16 for a bf16 cache, since A and B of an MMA have one type; both sums stay fp32.
 //
 // Bound: HBM (2 (D + 1) bytes a row and kv head; 4 D for bf16).  Rows past the end of a sequence, and rows of the
 // prefix in the first tile behind it, are masked to -inf in S and zeroed in V (any bits may lie there); TMA boxes wholly
@@ -41,6 +43,7 @@ constexpr int kBoxRows = 64;
 constexpr int kConsumerWarps = 4;
 constexpr int kThreads = (kConsumerWarps + 1) * 32;
 constexpr int kPad = 4;            // floats between the merge rows of two heads (bank spread)
+constexpr float kTopP = 15.f;      // log2 of the largest weight times scale of an 8-bit cache's rows as a half
 
 template <int D, bool k8>
 struct Cfg {
@@ -444,6 +447,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                         const float mon = fmaxf(mo[e], mot[e]);
                         mou[e] = mon == -INFINITY ? 0.f : mon;
                         oscale[e] = ex2_approx(mo[e] - mou[e]);
+                        mou[e] -= kTopP;
                         mo[e] = mon;
                     } else {
                         mou[e] = mu[e];
@@ -576,8 +580,9 @@ __global__ void __launch_bounds__(kThreads, 2)
                     x[3] = fmaf(r.w, ow, x[3]);
                 }
                 const float f = L != 0.f ? ex2_approx(MOu - Mu) / L : 0.f;
+                constexpr float kTop = k8 ? 1.f / (1 << (int)kTopP) : 1.f;   // before f, which may be near the smallest numbers
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] *= f;
+                for (int e = 0; e < 4; ++e) x[e] = x[e] * kTop * f;
                 if (final_row) {
                     uint32_t* orow = reinterpret_cast<uint32_t*>(a.out + ((int64_t)w.b * a.H + w.g * a.n_rep + h) * D + d);
                     orow[0] = pack_bf16x2(x[0], x[1]);

@@ -1,9 +1,21 @@
-"""The 8-bit cache at the top of bf16's range.  Needs a B200."""
+"""The 8-bit cache at the ends of its formats' ranges: weights far below the largest, in sums over very many rows, and
+elements at the top of bf16's range.  Needs a B200.
+
+Tolerances as in test_gpu_kv8.py; but a weight times scale is rounded to a half with the largest at 2^15, so one below
+2^-29 of the largest (2^-14 as a half) is off by 2^-25 / 2^15 = 2^-40 of the largest at most.  A warp sums at most L / 4
+rows in fp32, one product of 16 rows after another: L / 64 steps, each off by one unit in the last place of the sum of
+magnitudes at most (2^-23; how the tensor cores round is not specified), and the weights in L / 32 additions a thread, each
+rounded (2^-24): (L / 64) 2^-23 + (L / 32) 2^-24 = L 2^-28 of the mean magnitude."""
+import math
+
 import pytest
 
 pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip("torch")
+
+BF16_HALF, F16_HALF, F32 = 2.0 ** -8, 2.0 ** -11, 2.0 ** -18
+
 
 @pytest.fixture(scope="module")
 def rt(cuda_device):
@@ -16,6 +28,42 @@ def rt(cuda_device):
 def _status_ok():
     from mllm_b200 import abi
     abi.call("mllm_attn_device_status", None)
+
+
+@pytest.mark.parametrize("L,B,top_exp", [(1 << 20, 300, 0), (1 << 18, 300, 8), (5000, 1, 8), (300, 1, 0)])
+def test_one_dominant_row_among_many(rt, L, B, top_exp):
+    """Each of the others has 2^-18 to 2^-29 of the dominant row's weight (and 2^-8 of its scale); together they are
+    up to several times as much.  Enough sequences that a warp goes through most of one's rows behind that row."""
+    H, D, at = 8, 64, 5
+    c = rt.PagedKVCache8(num_blocks=-(-L // 1024), num_kv_heads=1, head_dim=D, block_size=1024, max_seqs=B)
+    c.set_lengths([L])
+    one = torch.zeros(D, device="cuda")
+    one[0] = -1.0
+    v = 1.0 + 0.5 * (torch.arange(D, device="cuda") % 5)
+    c.k_pool.copy_(one.to(rt.FP8))
+    c.v_pool.copy_(v.to(rt.FP8))
+    c.k_exp.fill_(127)
+    c.v_exp.fill_(127)
+    blk, row = c.blocks_of(0)[at // 1024], at % 1024
+    c.k_pool.view(torch.uint8)[blk, 0, row] = 0
+    c.v_pool.view(torch.uint8)[blk, 0, row] = torch.full((D,), -(2.0 ** -top_exp), device="cuda").to(rt.FP8).view(torch.uint8)
+    c.v_exp[blk, 0, row] = 127 + top_exp
+    for b in range(1, B):
+        c.fork(0, b, L)
+    q = torch.zeros(B, H, D, device="cuda", dtype=torch.bfloat16)
+    q[:, :, 0] = torch.tensor([100.0, 110, 120, 130, 139, 141, 150, 160])   # over 8: 18 to 28.9 in log2
+    got = rt.decode_attention(q, c, 1, max_kv_len=L).view(B, H, D).double()
+    _status_ok()
+    k, vv = (x[0].double() for x in c.gather(0, L))
+    s = q[0].double() @ k.T / math.sqrt(D)
+    w = torch.softmax(s, -1)
+    ref, mean_abs = w @ vv, w @ vv.abs()
+    ev = torch.ones(L, device="cuda", dtype=torch.float64)
+    ev[at] = 2.0 ** top_exp
+    ds = F32 * (q[0].double().abs() @ k.abs().T).amax(-1, keepdim=True) / math.sqrt(D)
+    small = 2.0 ** -40 * (w * ev).amax(-1, keepdim=True) * (vv.abs() / ev[:, None]).sum(0)
+    tol = BF16_HALF * ref.abs() + (F16_HALF + 2 * ds + F32 + L * 2.0 ** -28) * mean_abs + small
+    assert ((got - ref).abs() <= tol).all(), ((got - ref).abs() / tol).amax((0, 2))
 
 
 def test_rows_at_the_top_of_the_range(rt):
