@@ -191,7 +191,8 @@ class LogitRules:
     """What restricts a request's next token (runtime.apply_logit_rules): the repetition penalty counts
     prefix, prompt and generated tokens, presence and frequency the generated ones; `bias` adds to
     tokens; `allowed(tokens)` gives, for the tokens generated so far, a truth value per token of the
-    vocabulary (a grammar's next tokens), or None for no restriction."""
+    vocabulary (a grammar's next tokens), or None for no restriction.  A request whose `allowed` raises,
+    or gives something else, ends there with that error; the others go on."""
     repetition: float = 1.0
     presence: float = 0.0
     frequency: float = 0.0
@@ -213,11 +214,19 @@ def _pack_mask(allow, vocab: int) -> np.ndarray:
     return np.packbits(np.pad(allow, (0, -vocab % 32)), bitorder="little").view(np.int32)
 
 
-def apply_rules(logits: torch.Tensor, rules: list, prompts: list[list[int]], generated: list[list[int]]) -> torch.Tensor:
+def _allowed_words(rules: LogitRules | None, generated: list[int], vocab: int) -> np.ndarray | None:
+    """The packed mask of a row's allowed tokens, or None for all of them."""
+    allow = rules.allowed(list(generated)) if rules is not None and rules.allowed else None
+    return None if allow is None else _pack_mask(allow, vocab)
+
+
+def apply_rules(logits: torch.Tensor, rules: list, prompts: list[list[int]], generated: list[list[int]],
+                masks: list | None = None) -> torch.Tensor:
     """`logits` [B, vocab] with every row's rules (None: none) applied; the row's history is its prompt
-    and generated tokens."""
+    and generated tokens.  `masks`: the rows' packed masks (None: none) in place of what their rules'
+    `allowed` gives."""
     B, V = logits.shape
-    if len(rules) != B or len(prompts) != B or len(generated) != B:
+    if len(rules) != B or len(prompts) != B or len(generated) != B or (masks is not None and len(masks) != B):
         raise ValueError("apply_rules: one entry per row of logits")
     dev = logits.device
     given = [r or LogitRules() for r in rules]
@@ -237,9 +246,10 @@ def apply_rules(logits: torch.Tensor, rules: list, prompts: list[list[int]], gen
         kw.update(bias_ids=up([list(r.bias) + [-1] * (m - len(r.bias)) for r in given], torch.int64),
                   bias_values=up([list(r.bias.values()) + [0.0] * (m - len(r.bias)) for r in given], torch.float32),
                   bias_lens=up([len(r.bias) for r in given], torch.int32))
-    masks = [r.allowed(list(t)) if r.allowed else None for r, t in zip(given, generated)]
+    if masks is None:
+        masks = [_allowed_words(r, t, V) for r, t in zip(given, generated)]
     if any(k is not None for k in masks):
-        words = np.stack([np.full((V + 31) // 32, -1, np.int32) if k is None else _pack_mask(k, V) for k in masks])
+        words = np.stack([np.full((V + 31) // 32, -1, np.int32) if k is None else k for k in masks])
         kw["allowed"] = torch.from_numpy(words).to(dev, non_blocking=True)
     return rt.apply_logit_rules(logits, **kw)
 
@@ -253,6 +263,7 @@ class Request:
     rules: LogitRules | None = None
     tokens: list[int] = field(default_factory=list)
     logits: list[torch.Tensor] = field(default_factory=list)   # kept when record_logits is set
+    error: Exception | None = None    # what ended the request early: its rules failed
 
     @property
     def rows(self) -> int:
@@ -266,7 +277,9 @@ class ContinuousBatcher:
     docstring).  `model` provides forward(ids, positions, caches) -> [B, vocab] logits and
     new_caches(num_blocks, block_size, max_seqs, max_blocks_per_seq).  `prefix`: tokens that every
     request begins with; they are prefilled once, into a row of their own, whose blocks the requests
-    share."""
+    share.  A request whose rules fail ends with the tokens it has and the failure in its `error`; an
+    exception from anywhere else leaves the batch as it was before the prefill or decode step that raised
+    it, so that the step can be taken again."""
 
     def __init__(self, model, max_batch: int, num_blocks: int, block_size: int = 256,
                  max_blocks_per_seq: int | None = None, record_logits: bool = False, graphs: bool = True,
@@ -319,24 +332,38 @@ class ContinuousBatcher:
         self.waiting.append(r)
         return r.rid
 
+    def _masks(self, requests: list[Request], vocab: int) -> list:
+        """The requests' packed masks; one whose rules fail gets the failure as its error."""
+        masks = []
+        for r in requests:
+            try:
+                masks.append(_allowed_words(r.rules, r.tokens, vocab))
+            except Exception as e:               # the caller's own code: it ends its request, not the batch
+                r.error = e
+                masks.append(None)
+        return masks
+
     def _pick(self, logits: torch.Tensor, requests: list[Request]) -> list[int]:
+        """The next token of every request; that of one with an error means nothing."""
         if any(r.rules for r in requests):
+            masks = self._masks(requests, logits.shape[1])
             logits = apply_rules(logits, [r.rules for r in requests], [self.prefix + r.prompt for r in requests],
-                                 [r.tokens for r in requests])
+                                 [r.tokens for r in requests], masks)
         if logits.is_cuda:
             return rt.sample(logits, use_greedy=True).tolist()
         return logits.argmax(-1).tolist()
 
     def _emit(self, r: Request, token: int, logits_row) -> None:
+        if r.error is not None:
+            return
         r.tokens.append(token)
         if self.record_logits:
             r.logits.append(logits_row.detach().float().cpu())
 
     def _finished(self, r: Request) -> bool:
-        return len(r.tokens) >= r.max_new_tokens or (r.eos is not None and r.tokens and r.tokens[-1] == r.eos)
+        return r.error is not None or len(r.tokens) >= r.max_new_tokens or (r.eos is not None and r.tokens and r.tokens[-1] == r.eos)
 
     def _admit(self) -> None:
-        dev = self._device()
         first = len(self.live)
         joined: list[Request] = []
         while self.waiting and first + len(joined) < self.max_batch:
@@ -353,22 +380,34 @@ class ContinuousBatcher:
             joined.append(r)
         if not joined:
             return
+        try:
+            logits = self._prefill(joined, first)
+            tokens = self._pick(logits, joined)
+        except BaseException:
+            for row in range(first, first + len(joined)):
+                for c in self.caches:
+                    c.release(row)
+            self.waiting[:0] = joined
+            raise
+        for r, t, row in zip(joined, tokens, logits):
+            self._emit(r, t, row)
+            self.live.append(r)
+
+    def _prefill(self, joined: list[Request], first: int) -> torch.Tensor:
+        """The prompts of the joining requests, into rows first ..; the logits of their last tokens."""
+        dev = self._device()
         if hasattr(self.model, "forward_packed"):
             # every joining prompt in one pass: rows first .. first+k-1, one launch per kernel
             views = [c.slot(first, len(joined)) for c in self.caches]
             ids = torch.tensor([t for r in joined for t in r.prompt], dtype=torch.int64, device=dev)
-            logits = self.model.forward_packed(ids, [len(r.prompt) for r in joined], views)
-        else:
-            rows = []
-            for i, r in enumerate(joined):
-                views = [c.slot(first + i) for c in self.caches]
-                ids = torch.tensor([r.prompt], dtype=torch.int64, device=dev)
-                pos = torch.arange(len(r.prompt), dtype=torch.int64, device=dev) + len(self.prefix)
-                rows.append(self.model.forward(ids, pos, views))
-            logits = torch.cat(rows)
-        for r, t, row in zip(joined, self._pick(logits, joined), logits):
-            self._emit(r, t, row)
-            self.live.append(r)
+            return self.model.forward_packed(ids, [len(r.prompt) for r in joined], views)
+        rows = []
+        for i, r in enumerate(joined):
+            views = [c.slot(first + i) for c in self.caches]
+            ids = torch.tensor([r.prompt], dtype=torch.int64, device=dev)
+            pos = torch.arange(len(r.prompt), dtype=torch.int64, device=dev) + len(self.prefix)
+            rows.append(self.model.forward(ids, pos, views))
+        return torch.cat(rows)
 
     def _retire(self) -> None:
         i = 0
@@ -399,15 +438,21 @@ class ContinuousBatcher:
         ids = torch.tensor([[r.tokens[-1]] for r in self.live], dtype=torch.int64, device=dev)
         lens = self.caches[0].host_lengths()[:n]
         pos = torch.tensor(lens, dtype=torch.int64, device=dev)   # the new token's position
-        g = self._decode_graph(n)
-        if g is not None:
-            logits = g.replay(ids, pos)
+        try:
+            g = self._decode_graph(n)
+            if g is not None:
+                logits = g.replay(ids, pos)
+                for c in self.caches:
+                    c.advance_host(1, n)
+                self.graph_steps += 1
+            else:
+                logits = self.model.forward(ids, pos, self.caches)
+            tokens = self._pick(logits, self.live)
+        except BaseException:
             for c in self.caches:
-                c.advance_host(1, n)
-            self.graph_steps += 1
-        else:
-            logits = self.model.forward(ids, pos, self.caches)
-        for r, t, row in zip(self.live, self._pick(logits, self.live), logits):
+                c.set_lengths(lens)
+            raise
+        for r, t, row in zip(self.live, tokens, logits):
             self._emit(r, t, row)
         self.steps += 1
 
@@ -433,7 +478,8 @@ class ContinuousBatcher:
         return g
 
     def run(self) -> dict[int, list[int]]:
-        """Step until every submitted request has finished; returns the tokens of each."""
+        """Step until every submitted request has finished; returns the tokens of each (of one that its
+        rules ended, `done[rid].error` says why)."""
         while self.waiting or self.live:
             before = (len(self.waiting), len(self.live))
             self.step()
