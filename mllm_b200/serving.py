@@ -192,7 +192,7 @@ class LogitRules:
     prefix, prompt and generated tokens, presence and frequency the generated ones; `bias` adds to
     tokens; `allowed(tokens)` gives, for the tokens generated so far, a truth value per token of the
     vocabulary (a grammar's next tokens), or None for no restriction.  A request whose `allowed` raises,
-    or gives something else, ends there with that error; the others go on."""
+    gives something else or leaves no token to pick ends there with that error; the others go on."""
     repetition: float = 1.0
     presence: float = 0.0
     frequency: float = 0.0
@@ -202,6 +202,8 @@ class LogitRules:
     def __post_init__(self):
         if not (self.repetition > 0 and all(math.isfinite(x) for x in (self.repetition, self.presence, self.frequency))):
             raise ValueError("LogitRules: penalties must be finite and repetition positive")
+        if any(math.isnan(x) for x in self.bias.values()):
+            raise ValueError("LogitRules: a bias must be a number")
         if len(self.bias) > rt.MAX_LOGIT_BIASES:
             raise ValueError(f"LogitRules: at most {rt.MAX_LOGIT_BIASES} biases")
 
@@ -218,6 +220,16 @@ def _allowed_words(rules: LogitRules | None, generated: list[int], vocab: int) -
     """The packed mask of a row's allowed tokens, or None for all of them."""
     allow = rules.allowed(list(generated)) if rules is not None and rules.allowed else None
     return None if allow is None else _pack_mask(allow, vocab)
+
+
+def _may_pick(rules: LogitRules | None, words: np.ndarray | None, token: int) -> bool:
+    """Whether a token picked from a row of logits is one that its mask and biases allow: where they leave none, the
+    row is all -inf and any token may come out."""
+    if rules is None:
+        return True
+    if words is not None and not (int(words[token // 32]) >> (token % 32)) & 1:
+        return False
+    return rules.bias.get(token, 0.0) > -math.inf
 
 
 def apply_rules(logits: torch.Tensor, rules: list, prompts: list[list[int]], generated: list[list[int]],
@@ -345,13 +357,16 @@ class ContinuousBatcher:
 
     def _pick(self, logits: torch.Tensor, requests: list[Request]) -> list[int]:
         """The next token of every request; that of one with an error means nothing."""
+        masks = [None] * len(requests)
         if any(r.rules for r in requests):
             masks = self._masks(requests, logits.shape[1])
             logits = apply_rules(logits, [r.rules for r in requests], [self.prefix + r.prompt for r in requests],
                                  [r.tokens for r in requests], masks)
-        if logits.is_cuda:
-            return rt.sample(logits, use_greedy=True).tolist()
-        return logits.argmax(-1).tolist()
+        tokens = (rt.sample(logits, use_greedy=True) if logits.is_cuda else logits.argmax(-1)).tolist()
+        for r, words, t in zip(requests, masks, tokens):
+            if r.error is None and not _may_pick(r.rules, words, t):
+                r.error = ValueError("LogitRules: no token is left to pick")
+        return tokens
 
     def _emit(self, r: Request, token: int, logits_row) -> None:
         if r.error is not None:

@@ -126,3 +126,30 @@ def test_a_step_that_raises_can_be_taken_again(host_rules, monkeypatch, at, pref
     for i, (p, n) in zip(ids, specs):
         assert bat.done[i].tokens == _counted(p, n) and bat.done[i].error is None
     assert all(c.free_blocks == free for c in bat.caches)
+
+
+def _nothing(after):
+    return lambda tokens: _everything(tokens) & (len(tokens) != after)
+
+
+@pytest.mark.parametrize("after", [0, 2])
+def test_a_request_whose_rules_leave_no_token_ends(host_rules, after):
+    """An empty mask, or biases of -inf on all that the mask allows: nothing may be picked, token 0 no more than others."""
+    few = np.zeros(CountingModel.vocab, dtype=bool)
+    few[[0, 7, 300]] = True
+    banned = LogitRules(bias={0: -np.inf, 7: -np.inf, 300: -np.inf, 5: 1.0},
+                        allowed=lambda tokens: few if len(tokens) == after else _everything(tokens))
+    specs = [([40], 5, None), ([5, 6, 7], 4, LogitRules(allowed=_nothing(after))), ([100] * 90, 3, LogitRules(allowed=_everything)),
+             ([600], 4, banned), ([60], 4, LogitRules(bias={61: -np.inf}))]
+    done = _run(specs)
+    for r, (p, n, _) in list(zip(done, specs))[:3:2]:
+        assert r.tokens == _counted(p, n) and r.error is None
+    for r, tokens in ((done[1], _counted([7], after)), (done[3], [5] * after)):   # 5: a tie with the model's choice, and lower
+        assert r.tokens == tokens and type(r.error) is ValueError and "no token" in str(r.error)
+    assert done[4].error is None and len(done[4].tokens) == 4 and 61 not in done[4].tokens   # a ban that leaves others
+
+
+def test_a_bias_is_a_number():
+    with pytest.raises(ValueError, match="bias"):
+        LogitRules(bias={3: float("nan")})
+    LogitRules(bias={3: -float("inf"), 4: float("inf")})
