@@ -206,7 +206,8 @@ class PagedKVCache:
     def fork(self, src: int, dst: int, rows: int) -> None:
         """Give the empty row `dst` the first `rows` rows of sequence `src`: it shares src's full blocks
         (a block is freed when its last owner is) and gets a copy of the rows in a block that ends
-        inside.  Shared rows must not be written again; appending to either sequence does not."""
+        inside.  Shared rows must not be written again; appending to either sequence does not, and neither
+        can be shortened into a block they share (release it instead)."""
         if src == dst or self._blocks[dst] or self._host_lengths[dst]:
             raise RuntimeError("PagedKVCache: fork target row is not empty")
         full, part = divmod(rows, self.block_size)
@@ -268,11 +269,20 @@ class PagedKVCache:
         while other rows are live)."""
         return PagedSlot(self, seq, count)
 
+    def _check_own(self, seq: int, rows: int) -> None:
+        """Refuses to take a sequence back into a block that others share: the next append would write their rows."""
+        at = rows // self.block_size
+        blocks = self._blocks[seq]
+        if rows < self._host_lengths[seq] and at < len(blocks) and self._owners[blocks[at]] > 1:
+            raise RuntimeError("PagedKVCache: a sequence cannot be shortened into a block that others share")
+
     # -- the KVCache interface the attention functions use --
     def host_lengths(self) -> list[int]:
         return list(self._host_lengths)
 
     def set_lengths(self, lens: list[int]) -> None:
+        for b, n in enumerate(lens):
+            self._check_own(b, n)
         for b, n in enumerate(lens):
             self.reserve(b, n)
         self._host_lengths[:len(lens)] = list(lens)
@@ -355,6 +365,8 @@ class PagedSlot(PagedKVCache):
     def set_lengths(self, lens: list[int]) -> None:
         if len(lens) > self._count:
             raise RuntimeError("PagedSlot: more lengths than sequences in the view")
+        for b, n in enumerate(lens):
+            self._parent._check_own(self._seq + b, n)
         for b, n in enumerate(lens):
             self._parent.reserve(self._seq + b, n)
             self._parent._host_lengths[self._seq + b] = n
