@@ -151,7 +151,7 @@ class PagedKVCache:
     this is the serving-format step beyond it."""
 
     capture_max_len = None   # set while a CUDA graph of decode steps is captured (decode_step)
-    shared_prefix = 0        # rows that all the sequences of a decode step begin with (decode_step)
+    shared_prefix = 0        # rows that the sequences of a decode step were forked with (decode_step)
 
     def __init__(self, num_blocks: int, num_kv_heads: int, head_dim: int, block_size: int = 256,
                  max_seqs: int = 64, max_blocks_per_seq: int | None = None, device="cuda"):
@@ -168,6 +168,10 @@ class PagedKVCache:
         self._host_lengths = [0] * max_seqs
         self._free = list(range(num_blocks - 1, -1, -1))   # pop() hands out block 0 first
         self._owners = [0] * num_blocks                     # sequences whose table holds the block (fork)
+        # per sequence (line, rows): its first `rows` rows are those of that line, the last one being its own.  Sequences
+        # that hold a line in common have the rows in common up to the smaller number.
+        self._lines = [[(b, math.inf)] for b in range(max_seqs)]
+        self._next_line = max_seqs
 
     @property
     def capacity(self) -> int:
@@ -222,9 +226,20 @@ class PagedKVCache:
             blocks.append(self._take_block())
             self._copy_rows(self._blocks[src][full], blocks[-1], part)
         self._blocks[dst] = blocks
+        self._lines[dst] = [(i, min(n, rows)) for i, n in self._lines[src] if rows > 0] + self._own_line()
         self.block_table[dst, :len(blocks)] = torch.tensor(blocks, dtype=torch.int32)
         self._host_lengths[dst] = rows
         self.lengths[dst] = rows
+
+    def _own_line(self) -> list:
+        self._next_line += 1
+        return [(self._next_line - 1, math.inf)]
+
+    def _rows_in_common(self, batch: int, rows: int, first: int = 0) -> bool:
+        """Whether sequences first .. first + batch - 1 came by their first `rows` rows together (fork)."""
+        lines = self._lines[first:first + batch]
+        return any(n >= rows and all((i, n) in line or any(j == i and m >= rows for j, m in line) for line in lines)
+                   for i, n in lines[0])
 
     def _copy_rows(self, src: int, dst: int, rows: int) -> None:
         for pool in (self.k_pool, self.v_pool):
@@ -243,6 +258,7 @@ class PagedKVCache:
             self._zero_blocks(idx)
             self._free.extend(reversed(blocks))
         self._blocks[seq] = []
+        self._lines[seq] = self._own_line()
         self._host_lengths[seq] = 0
         self.lengths[seq] = 0
 
@@ -261,6 +277,7 @@ class PagedKVCache:
         self.block_table[dst].copy_(self.block_table[src])
         self.lengths[dst] = self.lengths[src]
         self._blocks[dst], self._blocks[src] = self._blocks[src], []
+        self._lines[dst], self._lines[src] = self._lines[src], self._own_line()
         self._host_lengths[dst], self._host_lengths[src] = self._host_lengths[src], 0
         self.lengths[src] = 0
 
@@ -276,6 +293,16 @@ class PagedKVCache:
         if rows < self._host_lengths[seq] and at < len(blocks) and self._owners[blocks[at]] > 1:
             raise RuntimeError("PagedKVCache: a sequence cannot be shortened into a block that others share")
 
+    def _take_length(self, seq: int, rows: int) -> None:
+        """The host copy of a sequence's length; what lies behind a smaller one will be written anew, so that the rows in
+        common with others end there."""
+        if rows < self._host_lengths[seq]:
+            line = self._lines[seq][-1][0]
+            old = [(i, min(n, rows)) for i, n in self._lines[seq] if rows > 0]
+            known = any(i == line for b, other in enumerate(self._lines) if b != seq for i, _ in other)
+            self._lines[seq] = old + self._own_line() if known else old[:-1] + [(line, math.inf)]
+        self._host_lengths[seq] = rows
+
     # -- the KVCache interface the attention functions use --
     def host_lengths(self) -> list[int]:
         return list(self._host_lengths)
@@ -285,7 +312,8 @@ class PagedKVCache:
             self._check_own(b, n)
         for b, n in enumerate(lens):
             self.reserve(b, n)
-        self._host_lengths[:len(lens)] = list(lens)
+        for b, n in enumerate(lens):
+            self._take_length(b, n)
         self.lengths[:len(lens)].copy_(torch.tensor(lens, dtype=torch.int32), non_blocking=True)
 
     def advance(self, n: int | list[int], batch: int | None = None) -> None:
@@ -359,6 +387,9 @@ class PagedSlot(PagedKVCache):
     def move(self, src: int, dst: int) -> None:
         raise RuntimeError("PagedSlot: move rows on the parent cache")
 
+    def _rows_in_common(self, batch: int, rows: int, first: int = 0) -> bool:
+        return self._parent._rows_in_common(batch, rows, self._seq + first)
+
     def host_lengths(self) -> list[int]:
         return self._parent.host_lengths()[self._seq:self._seq + self._count]
 
@@ -369,7 +400,7 @@ class PagedSlot(PagedKVCache):
             self._parent._check_own(self._seq + b, n)
         for b, n in enumerate(lens):
             self._parent.reserve(self._seq + b, n)
-            self._parent._host_lengths[self._seq + b] = n
+            self._parent._take_length(self._seq + b, n)
         self.lengths[:len(lens)].copy_(torch.tensor(lens, dtype=torch.int32), non_blocking=True)
 
     def advance(self, n, batch: int | None = None) -> None:
@@ -943,7 +974,8 @@ def _decode_step_kv8(q, k, v, cache: PagedKVCache8, positions, rope_theta, num_k
         cache.advance(1, batch=B)
         L = max(cache.host_lengths()[:B])
     L = min(L, cache.capacity)
-    if cache.shared_prefix > 0 and _shared_pays(B, cache.shared_prefix, num_kv_heads, D, True):
+    if cache.shared_prefix > 0 and _shared_pays(B, cache.shared_prefix, num_kv_heads, D, True) and \
+            cache._rows_in_common(B, cache.shared_prefix):
         return decode_attention_shared(q_rot, cache, num_kv_heads, cache.shared_prefix, L)
     return _decode_kv8(q_rot, cache, num_kv_heads, L)
 
@@ -1021,9 +1053,9 @@ def decode_step(q, k, v, kv_cache: KVCache, positions: torch.Tensor, rope_theta:
     append + decode attention in one launch.  q [B,H,1,D], k/v [B,Hkv,1,D] (strided views of the
     projections); positions int64 [1] (shared) or [B] / [B, 1].  The new rows go to slot
     lengths[b] of each sequence and the lengths advance by one.  Returns [B, 1, H*D].  A paged cache
-    whose shared_prefix is set (every sequence begins with that many equal rows) is read by
-    decode_attention_shared, after an epilogue launch of its own, where batch and prefix are large
-    enough for that to be faster."""
+    whose shared_prefix is set is read by decode_attention_shared, after an epilogue launch of its own,
+    where the sequences came by that many rows together (PagedKVCache.fork) and batch and prefix are
+    large enough for that to be faster; else each sequence's rows are read through its own table row."""
     for n, t in (("q", q), ("k", k), ("v", v)):
         _check_cuda_bf16(n, t)
         if t.dim() != 4 or t.size(2) != 1 or t.stride(3) != 1:
@@ -1036,7 +1068,8 @@ def decode_step(q, k, v, kv_cache: KVCache, positions: torch.Tensor, rope_theta:
                                 eps, rope_table)
     if isinstance(kv_cache, PagedKVCache) and kv_cache.shared_prefix > 0:
         _check_shared_step(q, k, v, kv_cache, positions, num_kv_heads, rope_table)
-        if _shared_pays(B, kv_cache.shared_prefix, num_kv_heads, D):
+        if _shared_pays(B, kv_cache.shared_prefix, num_kv_heads, D) and \
+                kv_cache._rows_in_common(B, kv_cache.shared_prefix):
             return _decode_step_shared(q, k, v, kv_cache, positions, rope_theta, num_kv_heads, q_norm_weight,
                                        k_norm_weight, eps, rope_table)
     pos = positions.to(torch.int64).reshape(-1)
