@@ -1000,9 +1000,12 @@ def _shared_pays(B: int, prefix: int, num_kv_heads: int, D: int, kv8: bool = Fal
     return rows * 4 >= _SHARED_MIN_BYTES
 
 
-def _check_shared_step(q, k, v, cache: PagedKVCache, positions, num_kv_heads: int, rope_table) -> None:
-    B, _, _, D = q.shape
+def _check_step(q, k, v, cache: PagedKVCache, positions, num_kv_heads: int, rope_table) -> None:
+    """What a step of an append and a decode of their own can refuse, before the first of them is launched."""
+    B, H, _, D = q.shape
     pool = cache.k_pool.shape
+    if H > 8 * num_kv_heads:
+        raise RuntimeError("decode_step: GQA group larger than 8")
     if B > cache.block_table.shape[0] or pool[1] != num_kv_heads or pool[3] != D or k.shape != (B, num_kv_heads, 1, D) or \
             v.shape != k.shape:
         raise RuntimeError("decode_step: k, v and the cache must have num_kv_heads heads of q's head_dim, and a row per "
@@ -1064,10 +1067,11 @@ def decode_step(q, k, v, kv_cache: KVCache, positions: torch.Tensor, rope_theta:
     if H % num_kv_heads != 0:
         raise RuntimeError("Attention: num_heads must be divisible by num_kv_heads.")
     if isinstance(kv_cache, PagedKVCache8):
+        _check_step(q, k, v, kv_cache, positions, num_kv_heads, rope_table)
         return _decode_step_kv8(q, k, v, kv_cache, positions, rope_theta, num_kv_heads, q_norm_weight, k_norm_weight,
                                 eps, rope_table)
     if isinstance(kv_cache, PagedKVCache) and kv_cache.shared_prefix > 0:
-        _check_shared_step(q, k, v, kv_cache, positions, num_kv_heads, rope_table)
+        _check_step(q, k, v, kv_cache, positions, num_kv_heads, rope_table)
         if _shared_pays(B, kv_cache.shared_prefix, num_kv_heads, D) and \
                 kv_cache._rows_in_common(B, kv_cache.shared_prefix):
             return _decode_step_shared(q, k, v, kv_cache, positions, rope_theta, num_kv_heads, q_norm_weight,
