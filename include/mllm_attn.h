@@ -509,7 +509,7 @@ MLLM_API int mllm_sample(void* logits, int logits_bf16, int64_t row_stride, int 
  * A token that no rule touches keeps its bits; a forbidden one is -inf whatever its logit (NaN
  * too); a row that allows nothing is all -inf.
  *   logits / out: bf16 (logits_bf16 != 0) or fp32, row b at + b*row_stride / b*out_stride; out may
- *       be the same memory as logits (with the same stride), else the two must not overlap.
+ *       be the same memory as logits (with the same stride); else rows that overlap are refused.
  *   history: int64 device, row b's history_lens[b] <= history_cols tokens at
  *       history + b*history_stride (fewer than 2^30 columns); output_start: int32 device [batch]
  *       (NULL: 0) -- the tokens before it are the prompt's, which only the repetition penalty counts.

@@ -235,6 +235,18 @@ __global__ void __launch_bounds__(kThreads, kMinCtas) logit_rules_kernel(RuleArg
     }
 }
 
+// Whether any row of `len` bytes of one tensor meets one of the other's (rows sa and sb bytes apart): both in ascending
+// order.
+bool rows_meet(uintptr_t a, uintptr_t sa, uintptr_t b, uintptr_t sb, int rows, uintptr_t len) {
+    for (int i = 0, j = 0; i < rows && j < rows;) {
+        const uintptr_t pa = a + i * sa, pb = b + j * sb;
+        if (pa + len <= pb) ++i;
+        else if (pb + len <= pa) ++j;
+        else return true;
+    }
+    return false;
+}
+
 }  // namespace
 
 MLLM_DEFINE_STATUS_READER(logit_rules)
@@ -279,6 +291,10 @@ extern "C" int mllm_logit_rules(const void* logits, int logits_bf16, int64_t row
         !aligned(presence, 4) || !aligned(frequency, 4) || !aligned(bias_ids, 8) || !aligned(bias_values, 4) ||
         !aligned(bias_lens, 4))
         return fail(MLLM_ERR_INVALID_ARGUMENT, "logit_rules: misaligned pointer");
+    const bool in_place = logits == out && (batch == 1 || row_stride == out_stride);
+    if (!in_place && rows_meet((uintptr_t)logits, (uintptr_t)row_stride * es, (uintptr_t)out, (uintptr_t)out_stride * es, batch,
+                               (uintptr_t)vocab * es))
+        return fail(MLLM_ERR_INVALID_ARGUMENT, "logit_rules: out overlaps the logits without being the same rows");
     int num_sms = 0;
     if (int st = require_sm100(&num_sms)) return st;
     RuleArgs a = {};

@@ -1150,7 +1150,8 @@ def apply_logit_rules(logits: torch.Tensor, history=None, history_lens=None, out
         where negative), a generated token's lowered by the second, and by the third for each time
       bias_ids int64 / bias_values fp32 [B, n <= 1024] with bias_lens int32 [B]: added to tokens
       allowed int32 [B, ceil(V / 32)]: bit v % 32 of word v // 32 allows token v; others become -inf
-    All on the device.  Returns `out` (a new tensor by default; `logits` itself works in place)."""
+    All on the device.  Returns `out` (a new tensor by default; `logits` itself works in place, another
+    view of its rows is refused)."""
     if not logits.is_cuda:
         raise RuntimeError("logit rules: logits must be a CUDA tensor (no CPU fallback)")
     dtype = logits.dtype
