@@ -851,11 +851,12 @@ def qkv_epilogue_packed(q, k, v, kv_cache, q_lens: list[int], rope_theta: float,
     if pos.numel() != T:
         raise RuntimeError("packed sequences: one position per token")
     if isinstance(kv_cache, PagedKVCache8):
+        for b in range(B):
+            kv_cache.reserve(b, before[b] + q_lens[b])
         q_out = torch.empty((H, T, D), dtype=BF16, device=q.device)
-        start = kv_cache.lengths[:B].clone()
-        kv_cache.advance(list(q_lens), batch=B)
-        qkv_epilogue_kv8(q, k, v, kv_cache, cu_dev, start, pos.reshape(-1), rope_theta, None, q_norm_weight,
+        qkv_epilogue_kv8(q, k, v, kv_cache, cu_dev, kv_cache.lengths[:B], pos.reshape(-1), rope_theta, None, q_norm_weight,
                          k_norm_weight, eps, q_out.transpose(0, 1))
+        kv_cache.advance(list(q_lens), batch=B)   # behind all that the epilogue may refuse
         return q_out
     qn = kn = None
     if q_norm_weight is not None:

@@ -1,4 +1,4 @@
-"""What decode_step refuses over an 8-bit cache, before it has appended or reserved anything.  CPU only."""
+"""What decode_step and the prompts' epilogue refuse over an 8-bit cache, before they have appended anything.  CPU only."""
 import pytest
 import torch
 
@@ -26,3 +26,18 @@ def test_refused_before_anything_changes(cls, prefix, bad, monkeypatch):
     with pytest.raises(RuntimeError):
         rt.decode_step(q, kv, kv, c, torch.tensor(a["pos"]), 1e4, a["Hkv"], rope_table=table)
     assert c.host_lengths() == [128] * 3 and c.lengths.tolist() == [128] * 3 and c.free_blocks == free
+
+
+@pytest.mark.parametrize("bad", [dict(kv=4), dict(D=128), dict(norm=(64, 32)), dict(pos=[0, 1, 2, 3])])
+def test_packed_prompts_refused_before_the_lengths_advance(bad, monkeypatch):
+    monkeypatch.setattr(rt, "_check_cuda_bf16", lambda *a: None)
+    monkeypatch.setattr(rt, "_launch", lambda *a: pytest.fail("launched"))
+    c = rt.PagedKVCache8(9, 2, 64, block_size=128, max_seqs=3, device="cpu")
+    c.set_lengths([5, 6, 7])
+    a = {**dict(kv=2, D=64, norm=None), **bad}
+    q, kv = (torch.zeros(5, h, a["D"], dtype=torch.bfloat16) for h in (8, a["kv"]))
+    norm = [torch.ones(n) for n in a["norm"]] if a["norm"] else [None, None]
+    pos = torch.tensor(a["pos"]) if "pos" in a else None                  # four positions for five tokens
+    with pytest.raises(RuntimeError):
+        rt.qkv_epilogue_packed(q, kv, kv, c, [3, 2], 1e4, positions=pos, q_norm_weight=norm[0], k_norm_weight=norm[1])
+    assert c.host_lengths() == [5, 6, 7] and c.lengths.tolist() == [5, 6, 7]
