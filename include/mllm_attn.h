@@ -446,7 +446,7 @@ MLLM_API int mllm_decode_attention_paged_kv8(const void* q, const mllm_paged_kv8
  * prefix_len - 1 are the same for every sequence of the call (a system prompt, a document) and are
  * read once for the whole batch, through the block-table row of the first sequence that is not
  * empty; rows prefix_len .. kv_lens[b] - 1 are each sequence's own, through its own table row.  The
- * result is that of mllm_decode_attention_paged_bf16 over caches that hold equal rows there; whether
+ * result is that of mllm_decode_attention_paged_bf16 (to rounding) over caches that hold equal rows there; whether
  * the tables share the blocks or hold copies makes no difference.  prefix_len 0 is the plain decode.
  *   q, out, head_dim, group size, softmax_scale: as mllm_decode_attention_paged_bf16, q 16-byte
  *       aligned.  kv_lens: int32 device [batch], required, prefix_len <= kv_lens[b] <= max_kv_len;
@@ -462,7 +462,8 @@ MLLM_API int mllm_decode_attention_shared_paged_bf16(const void* q, const mllm_p
                                                      void* workspace, size_t workspace_bytes, mllm_stream_t stream);
 
 /* The same over an 8-bit cache, whose rows stand for bf16 values: the result is that of
- * mllm_decode_attention_paged_kv8.  Workspace as above. */
+ * mllm_decode_attention_paged_kv8 to rounding (the weights of the prefix's rows are rounded to bf16, there
+ * to a half).  Workspace as above. */
 MLLM_API int mllm_decode_attention_shared_paged_kv8(const void* q, const mllm_paged_kv8* kv, const int32_t* kv_lens,
                                                     int prefix_len, int batch, int num_heads, int num_kv_heads,
                                                     int head_dim, int max_kv_len, float softmax_scale, void* out,

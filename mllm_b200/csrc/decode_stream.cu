@@ -178,7 +178,8 @@ __global__ void __launch_bounds__(kThreads, 2)
     // Behind a prefix kernel (shared) nothing here depends on that kernel's results, but lengths, tables, queries and rows
     // come from what ran before it.  It has waited for that, and published its ticket, before it let this grid in: a
     // thread that reads the ticket back (an acquire) is ordered behind that wait and goes on beside the prefix kernel; one
-    // that does not waits for the prefix kernel itself.
+    // that does not waits for the prefix kernel itself.  The loads behind it start later for that: 59 us in place of
+    // 55 for 128 sequences behind 8192 rows, 25.1 in place of 24.6 for 32.
     if (!a.shared || !ticket_published(a)) pdl_wait();
     pdl_trigger();
     const int pairs = a.B * a.Hkv;

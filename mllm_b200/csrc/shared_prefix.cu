@@ -23,7 +23,7 @@
 // through a tensor map that ends with the prefix, so that their contents cannot matter.
 // Over an 8-bit cache four more warps fetch the rows and store them as the exact bf16 values where TMA would have put
 // them; all else is the same, and so are the bits of a stretch's results.  For a pair that hides behind the softmax (128 sequences
-// behind 8192 rows: 58 us, bf16 57), a single tile's pace it sets (4 behind 32700: 53 us, bf16 40).
+// behind 8192 rows: 61 us, bf16 59), a single tile's pace it sets (4 behind 32700: 53 us, bf16 41).
 //
 // P is bf16 for the second product (A and B of an MMA have one type, and V is bf16); sums and O are fp32.
 #include <algorithm>

@@ -210,7 +210,7 @@ class PagedKVCache:
     def fork(self, src: int, dst: int, rows: int) -> None:
         """Give the empty row `dst` the first `rows` rows of sequence `src`: it shares src's full blocks
         (a block is freed when its last owner is) and gets a copy of the rows in a block that ends
-        inside.  Shared rows must not be written again; appending to either sequence does not, and neither
+        inside, as they are now: rows that are reserved and written later reach it in full blocks only.  Shared rows must not be written again; appending to either sequence does not, and neither
         can be shortened into a block they share (release it instead)."""
         if src == dst or self._blocks[dst] or self._host_lengths[dst]:
             raise RuntimeError("PagedKVCache: fork target row is not empty")
