@@ -210,7 +210,8 @@ class PagedKVCache:
     def fork(self, src: int, dst: int, rows: int) -> None:
         """Give the empty row `dst` the first `rows` rows of sequence `src`: it shares src's full blocks
         (a block is freed when its last owner is) and gets a copy of the rows in a block that ends
-        inside, as they are now: rows that are reserved and written later reach it in full blocks only.  Shared rows must not be written again; appending to either sequence does not, and neither
+        inside, as they are now: rows that are reserved and written later reach it in full blocks only.
+        Shared rows must not be written again; appending to either sequence does not, and neither
         can be shortened into a block they share (release it instead)."""
         if src == dst or self._blocks[dst] or self._host_lengths[dst]:
             raise RuntimeError("PagedKVCache: fork target row is not empty")
@@ -226,7 +227,8 @@ class PagedKVCache:
             blocks.append(self._take_block())
             self._copy_rows(self._blocks[src][full], blocks[-1], part)
         self._blocks[dst] = blocks
-        self._lines[dst] = [(i, min(n, rows)) for i, n in self._lines[src] if rows > 0] + self._own_line()
+        same = rows if self._host_lengths[src] >= rows else full * self.block_size
+        self._lines[dst] = [(i, min(n, same)) for i, n in self._lines[src] if same > 0] + self._own_line()
         self.block_table[dst, :len(blocks)] = torch.tensor(blocks, dtype=torch.int32)
         self._host_lengths[dst] = rows
         self.lengths[dst] = rows

@@ -99,3 +99,13 @@ def test_a_step_reads_the_prefix_once_only_where_it_is_in_common(cls, monkeypatc
         q, kv = (torch.zeros(3, h, 1, 64, dtype=torch.bfloat16) for h in (4, 2))
         with pytest.raises(Stop, match="shared" if forked else "own"):
             rt.decode_step(q, kv, kv, c, torch.tensor([200]), 1e4, 2)
+
+
+def test_reserved_rows_are_in_common_in_full_blocks_only():
+    """What is written behind the fork reaches shared blocks, not the copy of the last one."""
+    c = rt.PagedKVCache(9, 1, 64, block_size=128, max_seqs=3, device="cpu")
+    c.reserve(0, 300)
+    c.fork(0, 1, 300)
+    c.fork(1, 2, 100)                                    # sequence 1 has 300 rows: what it copies is there
+    assert c._rows_in_common(2, 256) and not c._rows_in_common(2, 257)
+    assert c._rows_in_common(2, 100, first=1) and c._rows_in_common(3, 100) and not c._rows_in_common(3, 101)
