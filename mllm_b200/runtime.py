@@ -288,34 +288,30 @@ class PagedKVCache:
         while other rows are live)."""
         return PagedSlot(self, seq, count)
 
-    def _check_own(self, seq: int, rows: int) -> None:
-        """Refuses to take a sequence back into a block that others share: the next append would write their rows."""
-        at = rows // self.block_size
-        blocks = self._blocks[seq]
-        if rows < self._host_lengths[seq] and at < len(blocks) and self._owners[blocks[at]] > 1:
-            raise RuntimeError("PagedKVCache: a sequence cannot be shortened into a block that others share")
-
-    def _take_length(self, seq: int, rows: int) -> None:
-        """The host copy of a sequence's length; what lies behind a smaller one will be written anew, so that the rows in
-        common with others end there."""
-        if rows < self._host_lengths[seq]:
-            line = self._lines[seq][-1][0]
-            old = [(i, min(n, rows)) for i, n in self._lines[seq] if rows > 0]
-            known = any(i == line for b, other in enumerate(self._lines) if b != seq for i, _ in other)
-            self._lines[seq] = old + self._own_line() if known else old[:-1] + [(line, math.inf)]
-        self._host_lengths[seq] = rows
+    def _shorten(self, lens: list[int], first: int = 0) -> None:
+        """For sequences from `first` on that `lens` takes back: refuses a length that falls into a block others share, since
+        the next append would write their rows; what lies behind will be written anew, so that the rows in common with
+        others end there."""
+        short = [(b, n) for b, n in enumerate(lens, first) if n < self._host_lengths[b]]
+        for b, n in short:
+            at, blocks = n // self.block_size, self._blocks[b]
+            if at < len(blocks) and self._owners[blocks[at]] > 1:
+                raise RuntimeError("PagedKVCache: a sequence cannot be shortened into a block that others share")
+        for b, n in short:
+            line = self._lines[b][-1][0]
+            old = [(i, min(m, n)) for i, m in self._lines[b] if n > 0]
+            known = any(i == line for c, other in enumerate(self._lines) if c != b for i, _ in other)
+            self._lines[b] = old + self._own_line() if known else old[:-1] + [(line, math.inf)]
 
     # -- the KVCache interface the attention functions use --
     def host_lengths(self) -> list[int]:
         return list(self._host_lengths)
 
     def set_lengths(self, lens: list[int]) -> None:
-        for b, n in enumerate(lens):
-            self._check_own(b, n)
+        self._shorten(lens)
         for b, n in enumerate(lens):
             self.reserve(b, n)
-        for b, n in enumerate(lens):
-            self._take_length(b, n)
+        self._host_lengths[:len(lens)] = list(lens)
         self.lengths[:len(lens)].copy_(torch.tensor(lens, dtype=torch.int32), non_blocking=True)
 
     def advance(self, n: int | list[int], batch: int | None = None) -> None:
@@ -398,11 +394,10 @@ class PagedSlot(PagedKVCache):
     def set_lengths(self, lens: list[int]) -> None:
         if len(lens) > self._count:
             raise RuntimeError("PagedSlot: more lengths than sequences in the view")
-        for b, n in enumerate(lens):
-            self._parent._check_own(self._seq + b, n)
+        self._parent._shorten(lens, self._seq)
         for b, n in enumerate(lens):
             self._parent.reserve(self._seq + b, n)
-            self._parent._take_length(self._seq + b, n)
+            self._parent._host_lengths[self._seq + b] = n
         self.lengths[:len(lens)].copy_(torch.tensor(lens, dtype=torch.int32), non_blocking=True)
 
     def advance(self, n, batch: int | None = None) -> None:
