@@ -20,8 +20,8 @@
 // rows; one byte permute sorts them, and output columns 2i and 2i + 1 land in the two row halves of the MMA.
 // q is scaled per head by a power of two into the range of a half (exact for elements within 2^-27 of the head's
 // largest; smaller ones lose bits that lie 2^-40 below it) and the scale is taken out of S in fp32.
-// Row scales: S gets 2^ek before the softmax.  2^ev multiplies P, so P^T = exp2(s + ev - mo + 15) with mo the running
-// maximum of s + ev: the largest weight times scale is 2^15, the top of a half's range (65504), and none overflows it,
+// Row scales: S gets 2^ek before the softmax.  2^ev multiplies P, so P^T = exp2(s - m + ev - mo + 15) with mo the running
+// maximum of s - m + ev: the largest weight times scale is 2^15, the top of a half's range (65504), and none overflows it,
 // however the rows' scales differ; the merge takes the 2^15 out.  With the largest at 1, what lies 2^-25 below it would
 // become zero here but not in the sum l: with one dominant row, 2^18 others behind it in a warp lost 0.6 % of the output.
 // Now that takes 2^-40.  The sum l uses exp2(s - m) with its own maximum in fp32.  P is rounded to a half (2^-11), to
@@ -362,7 +362,8 @@ __global__ void __launch_bounds__(kThreads, 2)
             float o[KS][4];
 #pragma unroll
             for (int i = 0; i < KS; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-            float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, mo[2] = {-INFINITY, -INFINITY};
+            float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+            float mo[2] = {-INFINITY, -INFINITY};   // maximum of the weights times scales, against m
 
             for (int t = w.t0; t < w.t1; ++t) {
                 if (!mbar_wait(&full[stage], phase)) { alive = false; break; }
@@ -404,7 +405,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 
                 // ---- online softmax: element (nb, h, e) is row row0 + 16 nb + 8 h + grp, head 2 tig + e ----
                 float ev[NB][2];
-                float mt[2] = {-INFINITY, -INFINITY}, mot[2] = {-INFINITY, -INFINITY};
+                float mt[2] = {-INFINITY, -INFINITY};
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
@@ -424,45 +425,57 @@ __global__ void __launch_bounds__(kThreads, 2)
                         sa[nb][2 * h + 1] = v1;
                         mt[0] = fmaxf(mt[0], v0);
                         mt[1] = fmaxf(mt[1], v1);
-                        if constexpr (k8) {
-                            mot[0] = fmaxf(mot[0], v0 + ev[nb][h]);
-                            mot[1] = fmaxf(mot[1], v1 + ev[nb][h]);
-                        }
                     }
                 }
 #pragma unroll
                 for (int off = 4; off < 32; off <<= 1) {
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        mt[e] = fmaxf(mt[e], __shfl_xor_sync(0xffffffffu, mt[e], off));
-                        if constexpr (k8) mot[e] = fmaxf(mot[e], __shfl_xor_sync(0xffffffffu, mot[e], off));
-                    }
+                    for (int e = 0; e < 2; ++e) mt[e] = fmaxf(mt[e], __shfl_xor_sync(0xffffffffu, mt[e], off));
                 }
-                float mu[2], mou[2], oscale[2];
+                float oscale[2];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const float mn = fmaxf(m[e], mt[e]);
-                    mu[e] = mn == -INFINITY ? 0.f : mn;
-                    l[e] *= ex2_approx(m[e] - mu[e]);
-                    if constexpr (k8) {
-                        const float mon = fmaxf(mo[e], mot[e]);
-                        mou[e] = mon == -INFINITY ? 0.f : mon;
+                    const float mu = mn == -INFINITY ? 0.f : mn;
+                    const float shift = m[e] - mu;
+                    oscale[e] = ex2_approx(shift);
+                    l[e] *= oscale[e];
+                    mo[e] += shift;
+                    m[e] = mn;
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb) {
+                        sa[nb][e] -= mu;
+                        sa[nb][2 + e] -= mu;
+                    }
+                }
+                float mou[2];
+                if constexpr (k8) {   // of s - m + ev, not of s + ev: that would round ev away beside a score of 2^24
+                    float mot[2] = {mo[0], mo[1]};
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) mot[e] = fmaxf(mot[e], sa[nb][2 * h + e] + ev[nb][h]);
+#pragma unroll
+                    for (int off = 4; off < 32; off <<= 1)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) mot[e] = fmaxf(mot[e], __shfl_xor_sync(0xffffffffu, mot[e], off));
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        mou[e] = mot[e] == -INFINITY ? 0.f : mot[e];
                         oscale[e] = ex2_approx(mo[e] - mou[e]);
                         mou[e] -= kTopP;
-                        mo[e] = mon;
-                    } else {
-                        mou[e] = mu[e];
-                        oscale[e] = ex2_approx(m[e] - mu[e]);
+                        mo[e] = mot[e];
                     }
-                    m[e] = mn;
                 }
                 uint32_t pb[NB][2];
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const float p0 = ex2_approx(sa[nb][2 * h] - mu[0]);
-                        const float p1 = ex2_approx(sa[nb][2 * h + 1] - mu[1]);
+                        const float p0 = ex2_approx(sa[nb][2 * h]);
+                        const float p1 = ex2_approx(sa[nb][2 * h + 1]);
                         l[0] += p0;
                         l[1] += p1;
                         uint32_t packed;
@@ -539,7 +552,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                 for (int e = 0; e < 2; ++e) {
                     red_m[warp * kMaxGroup + 2 * tig + e] = m[e];
                     red_l[warp * kMaxGroup + 2 * tig + e] = l[e];
-                    red_mo[warp * kMaxGroup + 2 * tig + e] = k8 ? mo[e] : m[e];
+                    red_mo[warp * kMaxGroup + 2 * tig + e] = k8 ? mo[e] : 0.f;
                 }
             }
             // column of o[i][2h + .]: 8-bit rows 16 i + 2 grp + h, bf16 rows 16 i + 8 h + grp
@@ -562,25 +575,29 @@ __global__ void __launch_bounds__(kThreads, 2)
                                            : 2 * (int64_t)blockIdx.x + (w.pos == s_plan[1] ? 0 : 1);
             for (int i = threadIdx.x; i < a.n_rep * (D / 4); i += kConsumerWarps * 32) {
                 const int h = i / (D / 4), d = 4 * (i % (D / 4));
-                float M = red_m[h], MO = red_mo[h];
+                float M = red_m[h];
 #pragma unroll
-                for (int v = 1; v < kConsumerWarps; ++v) {
-                    M = fmaxf(M, red_m[v * kMaxGroup + h]);
-                    MO = fmaxf(MO, red_mo[v * kMaxGroup + h]);
+                for (int v = 1; v < kConsumerWarps; ++v) M = fmaxf(M, red_m[v * kMaxGroup + h]);
+                const float Mu = M == -INFINITY ? 0.f : M;
+                float mov[kConsumerWarps], MO = -INFINITY;   // the warps' mo against M
+#pragma unroll
+                for (int v = 0; v < kConsumerWarps; ++v) {
+                    mov[v] = red_mo[v * kMaxGroup + h] + (red_m[v * kMaxGroup + h] - Mu);
+                    MO = fmaxf(MO, mov[v]);
                 }
-                const float Mu = M == -INFINITY ? 0.f : M, MOu = MO == -INFINITY ? 0.f : MO;
+                const float MOu = MO == -INFINITY ? 0.f : MO;
                 float L = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int v = 0; v < kConsumerWarps; ++v) {
                     L += red_l[v * kMaxGroup + h] * ex2_approx(red_m[v * kMaxGroup + h] - Mu);
-                    const float ow = ex2_approx(red_mo[v * kMaxGroup + h] - MOu);
+                    const float ow = ex2_approx(mov[v] - MOu);
                     const float4 r = *reinterpret_cast<const float4*>(red_o + (v * kMaxGroup + h) * (D + kPad) + d);
                     x[0] = fmaf(r.x, ow, x[0]);
                     x[1] = fmaf(r.y, ow, x[1]);
                     x[2] = fmaf(r.z, ow, x[2]);
                     x[3] = fmaf(r.w, ow, x[3]);
                 }
-                const float f = L != 0.f ? ex2_approx(MOu - Mu) / L : 0.f;
+                const float f = L != 0.f ? ex2_approx(MOu) / L : 0.f;
                 constexpr float kTop = k8 ? 1.f / (1 << (int)kTopP) : 1.f;   // before f, which may be near the smallest numbers
 #pragma unroll
                 for (int e = 0; e < 4; ++e) x[e] = x[e] * kTop * f;

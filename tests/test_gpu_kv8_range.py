@@ -99,3 +99,32 @@ def test_rows_at_the_top_of_the_range(rt):
         assert torch.equal(torch.isnan(got), bad)
         assert (got[~bad] == ref[~bad]).all()
     _status_ok()
+
+
+@pytest.mark.parametrize("power", [10, 20, 23, 24, 25, 27, 30, 60])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_scores_of_any_size(rt, power, sign):
+    """Scores so large that neighbouring numbers are far apart: one row has all the weight, and its V comes out as it is."""
+    L, D = 400, 64
+    c = rt.PagedKVCache8(num_blocks=4, num_kv_heads=2, head_dim=D, block_size=128, max_seqs=1)
+    c.set_lengths([L])
+    g = torch.Generator(device="cuda").manual_seed(power)
+    k = torch.zeros(2, 512, D, device="cuda")
+    k[:, :, 0] = torch.randint(-6, 6, (2, 512), device="cuda", generator=g) * 16.0
+    top = [77, 301]
+    for h in range(2):
+        k[h, top[h], 0] = 112 * sign                     # the only one: the others are 16 and more below
+    v = (torch.randn(2, 512, D, device="cuda", generator=g) * 100).clamp(-448, 448).to(rt.FP8).float()
+    for pool, rows in ((c.k_pool, k), (c.v_pool, v)):
+        for i, blk in enumerate(c.blocks_of(0)):
+            pool[blk] = rows[:, 128 * i:128 * i + 128].to(rt.FP8)
+    c.k_exp.fill_(127)
+    c.v_exp.copy_(torch.randint(120, 130, c.v_exp.shape, device="cuda", generator=g, dtype=torch.int32).to(torch.uint8))
+    q = torch.zeros(1, 8, D, device="cuda", dtype=torch.bfloat16)
+    q[:, :, 0] = sign * 2.0 ** power / 8                 # scores of 14 to 2^power, in steps of 2^(power - 2)
+    got = rt.decode_attention(q, c, 2, max_kv_len=L)[0, 0].view(2, 4, D).double()
+    _status_ok()
+    rows = c.gather(0, L)[1].double()
+    for h in range(2):
+        want = rows[h, top[h]]
+        assert ((got[h] - want).abs() <= (BF16_HALF + F32) * want.abs()).all()
